@@ -167,10 +167,9 @@ def prepare(case, seed):
         lens = _lengths(c)
         table, n_pages = _tables(c, seed)
         rows = sum(n for _, n in lens)
-        seq = np.repeat(np.arange(len(lens)), [n for _, n in lens]).astype(np.int32)
         pos = np.concatenate([np.arange(h, h + n) for h, n in lens]).astype(np.int32)
         s = {"case": c, "lens": lens, "table": torch.from_numpy(table).to(DEVICE), "tok_pos": torch.from_numpy(pos).to(DEVICE),
-             "tok_seq": torch.from_numpy(seq).to(DEVICE), "q": (1.5 * _random(gen, (rows, c["heads"] * c["dim"]), torch.float32)).to(dtype),
+             "q": (1.5 * _random(gen, (rows, c["heads"] * c["dim"]), torch.float32)).to(dtype),
              "k": _random(gen, (n_pages, c["kv"], PAGE, c["dim"]), dtype), "v": _random(gen, (n_pages, c["kv"], PAGE, c["vdim"]), dtype),
              "sink": _random(gen, (c["heads"],), torch.float32) if c["sink"] else None, "scale": c["dim"] ** -0.5}
         if own:       # one plan serves all layers of a step, and the decode steps behind it until the batch changes
@@ -235,8 +234,8 @@ def _attention_own(s, c):
     q = s["q"]
     out = torch.empty((q.shape[0], c["heads"] * c["vdim"]), dtype=q.dtype, device=q.device)
     part = torch.empty((s["plan"].part_floats(c["vdim"]),), dtype=torch.float32, device=q.device)
-    s["kernels"].attn(q, out, s["tok_pos"], s["tok_seq"], s["table"], s["k"], s["v"], s["plan"], part, c["dim"], s["scale"], s["err"],
-                      softcap=c["cap"] or None, sink=s["sink"], v_dim=c["vdim"])
+    s["kernels"].attn(q, out, s["tok_pos"], s["table"], s["k"], s["v"], s["plan"], part, s["scale"], s["err"], softcap=c["cap"] or None,
+                      sink=s["sink"])
     return out
 
 
