@@ -1,0 +1,250 @@
+"""Which pages the sequences of a step have in common, and how attention goes over them once for all.
+
+The reference holds one sequence (model_f32.go:310-317) and has nothing of the kind. Sequences that were forked from one
+another hold the same pages at their front. `share_tree` finds them from the block table alone: two sequences share a page
+where their page ids are the same from the front on, as far as both hold the whole page before the step. The result is a tree:
+a node is a run of pages that two or more sequences share, a leaf what one sequence has for itself. Softmax attention over a
+sequence's keys splits exactly over the nodes on its path (each gives a maximum, a sum and a weighted sum of values, which are
+joined at the end), so a node's pages are read once, with the queries of all its members as the rows of one product.
+
+`SharePlan` lays that work out for the kernels: a tile is a few tokens of a node with all the query heads of one key/value head,
+an item a tile with a run of the node's pages, and every block has a list of items of about the same cost. An item leaves its
+rows' partial results in a scratch buffer; a list says which of them belong to a token and key/value head.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import numpy as np
+import torch
+
+from .needs import PAGE
+
+MAX_DEPTH = 4       # levels of shared runs; what lies deeper is read by each sequence for itself
+MIN_SAVED = 4       # pages that a node must save its members to be worth another partial result for each row
+ITEM_WORDS = 8      # int32 words of an item: first token in the list, tokens, last token, kv head, first page, page end (-1: to the
+                    # last token), first row of the scratch, row of the block table
+
+
+@dataclass(frozen=True)
+class TileShape:
+    """What a kernel works on: rows (tokens x query heads of a key/value head) of a tile, blocks that stay and walk their lists.
+    `halves`: a tile of at most half the rows is worked on twice, by pages of either parity, and leaves two partial results."""
+    rows: int
+    workers: int
+    halves: bool = False
+    item_pages: float = 1.0      # what an item costs beside its pages, in pages
+    half_cost: float = 1.0       # what a page of a tile of at most half the rows costs, a full tile's page being 1
+    min_pages: int = 2           # an item is not cut to fewer
+
+
+def share_tree(table: np.ndarray, whole: np.ndarray):
+    """`table` [seqs, width] page ids (-1: none), `whole` [seqs]: pages that each holds wholly before the step. Returns the order of the
+    sequences in which every node's members stand side by side, the nodes [(first, end, first page, end page)] in that order, parents
+    first, and for every place of the order the first page that the sequence there has for itself."""
+    n, width = table.shape
+    if n == 1:
+        return np.zeros(1, dtype=np.int64), [], np.zeros(1, dtype=np.int64)
+    # rows as byte strings: equal fronts come to stand side by side, whatever the order between different pages
+    order = np.argsort(np.ascontiguousarray(table).view(f"S{4 * width}").ravel(), kind="stable")
+    t, w = table[order], np.asarray(whole, dtype=np.int64)[order]
+    differ = (t[1:] != t[:-1]) | (t[1:] < 0)
+    same = np.where(differ.any(1), differ.argmax(1), width)
+    lcp = np.minimum(np.minimum(same, w[1:]), w[:-1]).tolist()
+    nodes, own = [], [0] * n
+    stack = [(0, n, 0, 0)]
+    while stack:
+        lo, hi, page, depth = stack.pop()
+        if hi - lo == 1:
+            own[lo] = page
+            continue
+        m = min(lcp[lo:hi - 1])
+        if m > page and (m - page) * (hi - lo - 1) >= MIN_SAVED:
+            nodes.append((lo, hi, page, m))
+            page, depth = m, depth + 1
+        if depth == MAX_DEPTH:
+            own[lo:hi] = [page] * (hi - lo)
+            continue
+        at = lo
+        for i in range(lo, hi):
+            if i == hi - 1 or lcp[i] == m:
+                stack.append((at, i + 1, page, depth))
+                at = i + 1
+    return order, nodes, np.asarray(own, dtype=np.int64)
+
+
+def saved_pages(nodes) -> int:
+    """Pages that a step need not read again."""
+    return sum((hi - lo - 1) * (b - a) for lo, hi, a, b in nodes)
+
+
+class SharePlan:
+    """The items of one attention over a step's rows, in one int32 buffer on the device. Good for every layer of the step with these
+    head counts, and for later steps of the same sequences with as many new tokens each: a leaf's last item goes on to where its
+    tokens stand now."""
+
+    def __init__(self, n_seqs: int, n_rows: int, n_heads: int, n_kv: int, shape: TileShape, width: int, parts: dict, device,
+                 capacity: "PlanCapacity | None" = None):
+        self.n_seqs, self.n_rows, self.n_heads, self.n_kv, self.shape, self.width = n_seqs, n_rows, n_heads, n_kv, shape, width
+        self.n_items, self.n_list, self.part_rows = len(parts["items"]), len(parts["list"]), parts["part_rows"]
+        self.parts = parts
+        cap = capacity or PlanCapacity(self.n_items, self.n_list, self.part_rows)
+        self.capacity = cap
+        if not self.fits(cap):
+            raise ValueError(f"a plan of {self.n_items} items, {self.n_list} list entries and {self.part_rows} rows of scratch; there is "
+                             f"room for {cap.items}, {cap.entries} and {cap.rows}")
+        if device is not None:
+            host = self.host()
+            self.dev = torch.from_numpy(host).to(device)
+            self._views()
+
+    def fits(self, cap: "PlanCapacity") -> bool:
+        return self.n_items <= cap.items and self.n_list <= cap.entries and self.part_rows <= cap.rows
+
+    def _sizes(self):
+        s, c = self.shape, self.capacity
+        # (items start at a multiple of four words: they are read sixteen bytes at a time)
+        return [-(-(s.workers + 1) // 4) * 4, ITEM_WORDS * c.items, self.n_rows, self.n_rows * self.n_kv + 1, c.entries]
+
+    def host(self) -> np.ndarray:
+        """The buffer's words: where each block's items begin, the items, the tokens in the tree's order, where each token and
+        key/value head's entries begin, the entries (rows of the scratch)."""
+        sizes, p = self._sizes(), self.parts
+        out, off = np.zeros(sum(sizes), dtype=np.int32), 0
+        for n, part in zip(sizes, (p["first"], p["items"].ravel(), p["toks"], p["list_first"], p["list"])):
+            out[off:off + len(part)] = part
+            off += n
+        return out
+
+    def _views(self):
+        at, views = 0, []
+        for n in self._sizes():
+            views.append(self.dev[at:at + n])
+            at += n
+        self.first, self.items, self.toks, self.list_first, self.list = views
+
+    def part_floats(self, v_dim: int) -> int:
+        """float32 elements of the scratch for values `v_dim` wide: a row's sums over the values, then its maximum and sum."""
+        return self.capacity.rows * (v_dim + 2)
+
+    @classmethod
+    def build(cls, table, held, new, n_heads: int, n_kv: int, shape: TileShape, device, capacity=None, tree=None) -> "SharePlan":
+        """`table` [seqs, width] page ids on the host; `held` and `new`: tokens that each sequence holds before the step and brings (0:
+        none). `tree`: what `share_tree` gave for these sequences, if it is at hand."""
+        table = np.asarray(table)
+        if table.ndim != 2 or table.dtype.kind not in "iu" or table.shape[0] == 0:
+            raise ValueError(f"a block table of page ids [sequences, pages], not {table.dtype} {table.shape}")
+        table = np.ascontiguousarray(table, dtype=np.int32)
+        held, new = np.asarray(held, dtype=np.int64), np.asarray(new, dtype=np.int64)
+        n_seqs, width = table.shape
+        if held.shape != (n_seqs,) or new.shape != (n_seqs,) or held.min() < 0 or new.min() < 0:
+            raise ValueError(f"{n_seqs} sequences need as many counts of tokens held and new, none negative")
+        if n_kv < 1 or n_heads % n_kv:
+            raise ValueError(f"{n_heads} heads cannot share {n_kv} key/value heads")
+        rep = n_heads // n_kv
+        if rep > shape.rows:
+            raise ValueError(f"{rep} query heads on one key/value head; a tile has {shape.rows} rows")
+        if np.any(-(-(held + new) // PAGE) > width):
+            raise ValueError(f"a sequence of {int((held + new).max())} tokens does not fit {width} pages")
+        order, nodes, own = tree if tree is not None else share_tree(table, held // PAGE)
+        parts = _lay_out(order, nodes, own, held, new, rep, n_kv, shape)
+        return cls(n_seqs, int(new.sum()), n_heads, n_kv, shape, width, parts, device, capacity)
+
+
+@dataclass(frozen=True)
+class PlanCapacity:
+    """Room for plans that take one another's place at the same addresses (a captured step's)."""
+    items: int
+    entries: int      # of the list
+    rows: int         # of the scratch
+
+    @classmethod
+    def of_decode(cls, n_seqs: int, n_heads: int, n_kv: int, shape: TileShape) -> "PlanCapacity":
+        """What any plan of one token for each of `n_seqs` sequences needs at most: every level of the tree has each token once, in
+        at most one tile more than its nodes need, and every block cuts one tile at most."""
+        rep = n_heads // n_kv
+        per = max(1, shape.rows // rep)
+        tiles = n_seqs + MAX_DEPTH * (n_seqs // 2 + -(-n_seqs // per))
+        twice = 2 if shape.halves else 1
+        cuts = shape.workers * min(per, n_seqs)
+        entries = twice * (n_kv * n_seqs * (1 + MAX_DEPTH) + cuts)
+        return cls(n_kv * tiles + shape.workers, entries, entries * rep)
+
+
+def _lay_out(order, nodes, own, held, new, rep: int, n_kv: int, shape: TileShape) -> dict:
+    starts = np.cumsum(new) - new                                # first row of every sequence in the packed step
+    n_o = new[order]
+    ends_o = np.cumsum(n_o)
+    T = int(ends_o[-1])
+    first_o = ends_o - n_o
+    toks = np.repeat(starts[order] - first_o, n_o) + np.arange(T)          # rows of the step in the tree's order
+    # ---- nodes and leaves alike: tokens [off, off + n) of `toks` over pages [page, end) of sequence `seq`'s table
+    lo = np.asarray([a for a, _, _, _ in nodes], dtype=np.int64)
+    hi = np.asarray([b for _, b, _, _ in nodes], dtype=np.int64)
+    off = np.concatenate([first_o[lo], first_o])
+    n = np.concatenate([ends_o[hi - 1] - first_o[lo], n_o])
+    page = np.concatenate([np.asarray([a for _, _, a, _ in nodes], dtype=np.int64), own])
+    end = np.concatenate([np.asarray([b for _, _, _, b in nodes], dtype=np.int64), np.full(len(order), -1)])
+    seq = np.concatenate([order[lo], order])
+    # ---- tiles: a few tokens each, all query heads of a key/value head
+    per = shape.rows // rep
+    n_tiles = -(-n // per)
+    s = np.repeat(np.arange(len(n)), n_tiles)
+    i = np.arange(len(s)) - np.repeat(np.cumsum(n_tiles) - n_tiles, n_tiles)
+    t_off = off[s] + i * per
+    t_n = np.minimum(per, n[s] - i * per)
+    t_last = toks[t_off + t_n - 1] if len(s) else np.zeros(0, dtype=np.int64)
+    seq_of_row = np.repeat(np.arange(len(new)), new)
+    last_pos = held[seq_of_row[t_last]] + t_last - starts[seq_of_row[t_last]] if len(s) else t_last
+    t_end = np.where(end[s] < 0, last_pos // PAGE + 1, end[s])
+    t_pages = t_end - page[s]
+    half = (t_n * rep <= shape.rows // 2) if shape.halves else np.zeros(len(s), dtype=bool)
+    cost = t_pages * np.where(half, shape.half_cost, 1.0) + shape.item_pages
+    # ---- a tile for every key/value head; the line of all their costs is cut into equal lengths, one for each block
+    u = np.repeat(np.arange(len(s)), n_kv)
+    g = np.tile(np.arange(n_kv), len(s))
+    c = cost[u]
+    at = np.cumsum(c) - c
+    total = float(c.sum())
+    per_block = max(total / shape.workers, shape.min_pages + shape.item_pages)
+    k0 = np.floor(at / per_block).astype(np.int64)
+    k1 = np.floor((at + c - 1e-6) / per_block).astype(np.int64)
+    n_cut = k1 - k0
+    cu = np.repeat(np.arange(len(u)), n_cut)
+    k = np.arange(len(cu)) - np.repeat(np.cumsum(n_cut) - n_cut, n_cut) + k0[cu] + 1
+    pages_u = t_pages[u]
+    cut = np.rint((k * per_block - at[cu]) / c[cu] * pages_u[cu]).astype(np.int64)
+    fine = (cut >= shape.min_pages) & (pages_u[cu] - cut >= shape.min_pages)
+    cu, cut = cu[fine], cut[fine]
+    # items: every unit from its start and from each of its cuts on
+    iu = np.concatenate([np.arange(len(u)), cu])
+    begin = np.concatenate([np.zeros(len(u), dtype=np.int64), cut])
+    by = np.lexsort((begin, iu))
+    iu, begin = iu[by], begin[by]
+    last = np.append(iu[1:] != iu[:-1], True) if len(iu) else np.zeros(0, dtype=bool)
+    stop = np.where(last, pages_u[iu], np.append(begin[1:], 0))
+    middle = at[iu] + c[iu] * (begin + stop) / (2.0 * np.maximum(1, pages_u[iu]))
+    worker = np.minimum(shape.workers - 1, (middle / per_block).astype(np.int64))
+    tile = u[iu]
+    rows = t_n[tile] * rep * np.where(half[tile], 2, 1)
+    part0 = np.cumsum(rows) - rows
+    items = np.empty((len(iu), ITEM_WORDS), dtype=np.int32)
+    items[:, 0], items[:, 1], items[:, 2], items[:, 3] = t_off[tile], t_n[tile], t_last[tile], g[iu]
+    items[:, 4] = page[s[tile]] + begin
+    items[:, 5] = np.where(last & (end[s[tile]] < 0), -1, page[s[tile]] + stop)
+    items[:, 6], items[:, 7] = part0, seq[s[tile]]
+    first = np.searchsorted(worker, np.arange(shape.workers + 1))
+    # ---- which rows of the scratch belong to a token and key/value head
+    n_i = t_n[tile]
+    it = np.repeat(np.arange(len(iu)), n_i)
+    inside = np.arange(len(it)) - np.repeat(np.cumsum(n_i) - n_i, n_i)
+    key = toks[t_off[tile][it] + inside] * n_kv + g[iu][it]
+    entry = part0[it] + inside * rep
+    if shape.halves:
+        twice = half[tile][it]
+        key = np.concatenate([key, key[twice]])
+        entry = np.concatenate([entry, entry[twice] + (n_i * rep)[it][twice]])
+    by = np.argsort(key, kind="stable")
+    list_first = np.zeros(T * n_kv + 1, dtype=np.int64)
+    np.cumsum(np.bincount(key, minlength=T * n_kv), out=list_first[1:])
+    return {"first": first, "items": items, "toks": toks, "list_first": list_first, "list": entry[by], "part_rows": int(rows.sum())}

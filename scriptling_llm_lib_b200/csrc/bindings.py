@@ -10,10 +10,13 @@ from __future__ import annotations
 import ctypes
 import os
 from ctypes import c_float, c_int, c_longlong, c_void_p
+from itertools import chain
 from operator import index as as_int      # a caller's number as the int it stands for; what is none (None, a float) is refused
 
 import torch
 
+from ..cache.needs import PAGE
+from ..cache.share import TileShape
 from .build import load_library
 
 
@@ -338,6 +341,13 @@ class KernelSet:
         if getattr(self, "_gate", None) is None:
             self._gate = GateKernels(self.dtype)
         return self._gate
+
+    @property
+    def shared(self) -> "SharedAttention":
+        """Attention over pages that several of a step's sequences share (its own libraries, loaded on first use)."""
+        if getattr(self, "_shared", None) is None:
+            self._shared = SharedAttention(self.dtype)
+        return self._shared
 
     @property
     def decode(self) -> "DecodeKernels":
@@ -1691,6 +1701,137 @@ class GateKernels:
         """x float32 = cap * tanh(x * scale / cap), in place; without a cap (None or 0), x * scale."""
         _check(self._fn("softcap")(_ptr(x, torch.float32, "x"), ctypes.c_longlong(x.numel()), c_float(cap or 0.0), c_float(scale),
                                    _stream()), "softcap")
+
+
+def _one_device(what: str, **tensors):
+    """All of these on the current CUDA device (a launch goes to the current device's stream)."""
+    here = torch.cuda.current_device() if torch.cuda.is_available() else None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise KernelError(f"{what}: {name} is on {t.device}; the kernels run on a CUDA device only")
+        if t.device.index != here:
+            raise KernelError(f"{what}: {name} is on {t.device} while cuda:{here} is the current device")
+
+
+class SharedAttention:
+    """Attention of a step whose sequences share pages, each shared run of pages read once for all that share it; any number of new
+    tokens a sequence. `shape` says how the kernel for these widths wants its plan (cache/share.py), `attn` runs it."""
+    MAX_REP = 64         # query heads on a key/value head
+
+    def __init__(self, dtype: torch.dtype):
+        if dtype not in _SUFFIX:
+            raise KernelError(f"no kernels for {dtype}; supported: float32, bfloat16")
+        self.dtype, self.suffix = dtype, _SUFFIX[dtype]
+        self.lib = load_library(f"share_{self.suffix}")
+        for n in ("share_attn", "share_merge"):
+            getattr(self.lib, f"sllm_{n}_{self.suffix}").restype = c_int
+
+    @staticmethod
+    def takes(head_dim: int, v_dim: int, rep: int = 1) -> bool:
+        """Keys and values of these widths, `rep` query heads on a key/value head."""
+        return all(w % 4 == 0 and 4 <= w <= 256 for w in (head_dim, v_dim)) and 1 <= rep <= SharedAttention.MAX_REP
+
+    def shape(self, head_dim: int, v_dim: int, sm_count: int | None = None) -> TileShape:
+        """The tiles of a plan for these widths."""
+        if not self.takes(head_dim, v_dim):
+            raise KernelError(f"shared attention takes widths in multiples of 4 up to 256, not keys of {head_dim} and values of {v_dim}")
+        if sm_count is None:
+            sm_count = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+        return TileShape(rows=64, workers=2 * sm_count)
+
+    def attn(self, q, out, tok_pos, block_table, kpages, vpages, plan, part, scale, err_flag, softcap=None, sink=None):
+        """out [T, H * vd] = attention of the step's queries q [T, H * hd or more] (rows may stand apart) at positions tok_pos over the
+        paged keys [pages, G, 64, hd] and values [pages, G, 64, vd] that block_table [sequences, pages] names; this step's own keys are
+        there already. `plan`: a SharePlan for this step's rows, heads and `shape`; `part`: float32 scratch of plan.part_floats(vd)
+        elements. `softcap`: a score s becomes softcap * tanh(s / softcap) before the softmax; `sink` float32 [H]: exp(sink[h]) joins
+        head h's denominator with no key and no value. A page id outside the storage or a position outside the table sets err_flag."""
+        H, G, T = plan.n_heads, plan.n_kv, plan.n_rows
+        if kpages.dim() != 4 or vpages.dim() != 4 or kpages.shape[:3] != vpages.shape[:3] or tuple(kpages.shape[1:3]) != (G, PAGE):
+            raise KernelError(f"shared attention: pages {tuple(kpages.shape)} and {tuple(vpages.shape)} for {G} key/value heads")
+        hd, vd = kpages.shape[3], vpages.shape[3]
+        if not self.takes(hd, vd, H // G):
+            raise KernelError(f"shared attention takes widths in multiples of 4 up to 256 and up to {self.MAX_REP} query heads on a key/value "
+                              f"head, not keys of {hd}, values of {vd} and {H} heads on {G}")
+        if q.dim() != 2 or q.shape[0] != T or q.shape[1] < H * hd or (q.stride(1) != 1 and q.shape[1] > 1) or q.stride(0) % 4 or q.dtype != self.dtype:
+            raise KernelError(f"shared attention: queries {tuple(q.shape)} {q.dtype} (row stride {q.stride(0)}) for {T} rows of {H} heads of {hd}")
+        if tuple(out.shape) != (T, H * vd) or tuple(tok_pos.shape) != (T,) or block_table.dim() != 2 or block_table.shape[0] < plan.n_seqs:
+            raise KernelError(f"shared attention: out {tuple(out.shape)}, positions {tuple(tok_pos.shape)} and block table "
+                              f"{tuple(block_table.shape)} for {T} rows of {plan.n_seqs} sequences")
+        if (sink is not None and tuple(sink.shape) != (H,)) or part.numel() < plan.part_floats(vd):
+            raise KernelError(f"shared attention: a sink for each of {H} heads and a scratch of {plan.part_floats(vd)} floats")
+        _one_device("shared attention", q=q, out=out, positions=tok_pos, block_table=block_table, keys=kpages, values=vpages, plan=plan.dev,
+                    scratch=part, sink=sink, err_flag=err_flag)
+        shape = self.shape(hd, vd)
+        if plan.shape != shape:
+            raise KernelError(f"shared attention: the plan is laid out for {plan.shape}, these widths want {shape}")
+        if T == 0:
+            return
+        rows = plan.capacity.rows
+        _check(getattr(self.lib, f"sllm_share_attn_{self.suffix}")(
+            c_void_p(q.data_ptr()), q.stride(0), _ptr(tok_pos, torch.int32, "tok_pos"), _ptr(block_table, torch.int32, "block_table"),
+            block_table.shape[1], _ptr(kpages, self.dtype, "kpages"), _ptr(vpages, self.dtype, "vpages"), c_longlong(kpages.shape[0]),
+            _ptr(plan.first, torch.int32, "plan"), _ptr(plan.items, torch.int32, "plan"), _ptr(plan.toks, torch.int32, "plan"),
+            as_int(shape.workers), _ptr(part, torch.float32, "part"), c_longlong(rows), as_int(H), as_int(G), hd, vd, c_float(scale),
+            c_float(softcap or 0.0), _ptr(err_flag, torch.int32, "err_flag"), _stream()), "share_attn")
+        _check(getattr(self.lib, f"sllm_share_merge_{self.suffix}")(
+            _ptr(part, torch.float32, "part"), c_longlong(rows), _ptr(plan.list_first, torch.int32, "plan"), _ptr(plan.list, torch.int32, "plan"),
+            _ptr(out, self.dtype, "out"), _ptr(sink, torch.float32, "sink"), as_int(T), as_int(H), as_int(G), vd, _stream()), "share_merge")
+
+
+class PageKernels:
+    """Copies of cache pages and of the fixed-size states of slots, whatever their element type: one launch for up to 16 pairs of tensors."""
+    AREAS = 16
+
+    def __init__(self):
+        self.lib = load_library("pages")
+        self.lib.sllm_page_copy.restype = c_int
+
+    def _copy(self, what, areas, src, dst, rows, max_rows, err_flag):
+        n = src.shape[0] if src.dim() == 1 else -1
+        if n < 0 or tuple(dst.shape) != (n,) or (rows is not None and tuple(rows.shape) != (n,)):
+            raise KernelError(f"{what}: ids {tuple(src.shape)} and {tuple(dst.shape)}"
+                              + (f", rows {tuple(rows.shape)}" if rows is not None else "") + " are one list each, of equal lengths")
+        _one_device(what, src=src, dst=dst, rows=rows, err_flag=err_flag)
+        if n == 0:
+            return
+        for i in range(0, len(areas), self.AREAS):
+            some = areas[i:i + self.AREAS]
+            words = (c_longlong * (11 * len(some)))(*chain.from_iterable(some))
+            _check(self.lib.sllm_page_copy(words, len(some), _ptr(src, torch.int32, "src"), _ptr(dst, torch.int32, "dst"),
+                                           _ptr(rows, torch.int32, "rows"), n, as_int(max_rows), _ptr(err_flag, torch.int32, "err_flag"),
+                                           _stream()), what)
+
+    def copy_pages(self, pairs, src, dst, rows, err_flag):
+        """For every (a, b) of `pairs`, storages [units, pages, kv heads, 64, width] of one layout (the same tensor, or another number of
+        pages), every unit u and every i: the first rows[i] positions of each head of b[u, dst[i]] become those of a[u, src[i]] (`rows`
+        None: whole pages); nothing else of b changes. src, dst, rows: int32 lists on the device. One page may be copied to many; no id
+        stands twice in dst, nor in src and dst where a and b are the same storage. An id outside a storage, or a number of positions
+        outside 0..64, sets err_flag, and that pair is not copied."""
+        areas = []
+        for a, b in pairs:
+            if a.dim() != 5 or b.dim() != 5 or a.dtype != b.dtype or a.shape[0] != b.shape[0] or a.shape[2:] != b.shape[2:] or a.shape[3] != PAGE:
+                raise KernelError(f"copy_pages: storages {tuple(a.shape)} {a.dtype} and {tuple(b.shape)} {b.dtype}")
+            _one_device("copy_pages", storage=a, to=b)
+            width, units, heads = a.element_size() * a.shape[4], a.shape[0], a.shape[2]
+            if a.numel() and b.numel():
+                item = width * PAGE * heads
+                areas.append((_ptr(a).value, _ptr(b).value, item * a.shape[1], item * b.shape[1], item, width * PAGE, width, units, heads,
+                              a.shape[1], b.shape[1]))
+        self._copy("copy_pages", areas, src, dst, rows, PAGE, err_flag)
+
+    def copy_slots(self, pairs, src, dst, err_flag):
+        """For every (a, b) of `pairs`, tensors [slots, ...] of one layout, and every i: b[dst[i]] = a[src[i]]. Ids as for `copy_pages`."""
+        areas = []
+        for a, b in pairs:
+            if a.dim() < 1 or a.dtype != b.dtype or a.shape[1:] != b.shape[1:]:
+                raise KernelError(f"copy_slots: tensors {tuple(a.shape)} {a.dtype} and {tuple(b.shape)} {b.dtype}")
+            _one_device("copy_slots", tensor=a, to=b)
+            if a.numel() and b.numel():
+                item = a.element_size() * (a.numel() // a.shape[0])
+                areas.append((_ptr(a).value, _ptr(b).value, 0, 0, item, item, item, 1, 1, a.shape[0], b.shape[0]))
+        self._copy("copy_slots", areas, src, dst, None, 1, err_flag)
 
 
 class CastKernels:

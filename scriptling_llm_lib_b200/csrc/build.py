@@ -44,6 +44,9 @@ LIBRARIES: dict[str, tuple[str, tuple[str, ...]]] = {
     "mix_bf16": ("lib_mix_bf16.cu", ("common.cuh", "tcgen05.cuh", "state_step.cuh", "mix_kernels.cuh", "mix_launchers.inc")),
     "ssd_f32": ("lib_ssd_f32.cu", ("common.cuh", "tcgen05.cuh", "state_step.cuh", "ssd_kernels.cuh", "ssd_launchers.inc")),
     "ssd_bf16": ("lib_ssd_bf16.cu", ("common.cuh", "tcgen05.cuh", "state_step.cuh", "ssd_kernels.cuh", "ssd_launchers.inc")),
+    "pages": ("lib_pages.cu", ("common.cuh",)),
+    "share_f32": ("lib_share_f32.cu", ("common.cuh", "share_kernels.cuh", "share_launchers.inc")),
+    "share_bf16": ("lib_share_bf16.cu", ("common.cuh", "share_kernels.cuh", "share_launchers.inc")),
     "gate_f32": ("lib_gate_f32.cu", ("common.cuh", "gate_kernels.cuh", "gate_launchers.inc")),
     "gate_bf16": ("lib_gate_bf16.cu", ("common.cuh", "gate_kernels.cuh", "gate_launchers.inc")),
 }
