@@ -47,12 +47,11 @@
 // Prompts of 2,048 tokens, 16 heads: keys 64, values 128, window 1,024 on 4 key/value heads 36.9 us (a page of two query tiles a block
 // with one S each, four softmax warps a tile: 52.5); keys 192, values 128, every earlier key 40.8 (70.8); 400 tokens behind 4,000
 // 24 and 73 (55 and 196); 48 tokens 6.6 (8.7). Scores read ahead of announcing P, or weights made while the maxima meet: 5% slower.
-#include "tcgen05.cuh"
+#include "attn_tcgen05.cuh"
 
 #define FT_BQ 128
 #define FT_BK 64           // = SLLM_PAGE
 #define FT_THREADS 192       // warp 0: TMA, warp 1: MMA, warps 2-5: softmax (thread = query row)
-#define FT_LOG2E 1.4426950408889634f
 
 struct FtArgs {
   bf16* out;            // [T, H*64]
@@ -103,79 +102,6 @@ __device__ __forceinline__ bool ft_item(const FtArgs& p, int round, FtItem& it) 
   return true;
 }
 __device__ __forceinline__ int ft_tile(const FtItem& it, int j) { return j < it.kept ? j : j + it.skip; }
-
-__device__ __forceinline__ float ft_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// tanh(x) = 1 - 2 / (1 + 2^(2 x log2 e)): two special-function instructions, absolute error of a few 1e-7, exact limits
-__device__ __forceinline__ float ft_tanh(float x) {
-  float t = ft_ex2(x * (2.0f * FT_LOG2E)), r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + t));
-  return fmaf(-2.0f, r, 1.0f);
-}
-// A raw score s (the product's sum, before the scale) capped in place: the softmax below multiplies by the scale, so the
-// capped score is handed on as (cap / scale) * tanh(s * scale / cap).
-__device__ __forceinline__ uint32_t ft_cap(uint32_t s, float cap_out, float cap_in) {
-  return __float_as_uint(cap_out * ft_tanh(__uint_as_float(s) * cap_in));
-}
-// the first n of 32 output elements (n a multiple of 8) times the sigmoid of their gate logits (16-byte aligned)
-__device__ __forceinline__ void ft_gate(uint32_t (&v)[32], const bf16* g, int n) {
-#pragma unroll
-  for (int c = 0; c < 4; c++) {
-    if (8 * c >= n) break;
-    const uint4 w = *(const uint4*)(g + 8 * c);
-    const bf16* e = (const bf16*)&w;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      float s;
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + ft_ex2(-FT_LOG2E * __bfloat162float(e[i]))));
-      v[8 * c + i] = __float_as_uint(__uint_as_float(v[8 * c + i]) * s);
-    }
-  }
-}
-__device__ __forceinline__ float ft_max3(float a, float b, float c) {
-  float y;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-  return y;
-}
-// two floats at once: d = a * b + c and d = a + b on pairs held in 64-bit registers
-__device__ __forceinline__ uint64_t ft_pack2(float lo, float hi) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-  return d;
-}
-__device__ __forceinline__ void ft_unpack2(uint64_t v, float& lo, float& hi) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t ft_fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t ft_add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-// two floats as the packed upper halves of their bits, and what that leaves of them (exactly): bfloat16 parts by truncation
-__device__ __forceinline__ uint32_t ft_cut_pair(float& u, float& v) {
-  const uint32_t a = __float_as_uint(u), b = __float_as_uint(v);
-  u -= __uint_as_float(a & 0xffff0000u);
-  v -= __uint_as_float(b & 0xffff0000u);
-  return __byte_perm(a, b, 0x7632);
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-// D[tmem] (+)= A[tmem] * B[smem]: A's row m in lane m, two bfloat16 of K per 32-bit column
-__device__ __forceinline__ void umma_bf16_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-               ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate) : "memory");
-}
 
 // Heads of up to FT_HD dims for keys and values alike, in multiples of 8: TMA fills a box's columns past the storage row with
 // zeros, what a query box holds past its head meets those zeros, and only p.vd columns are written out.
@@ -533,19 +459,6 @@ __device__ __forceinline__ bool fp_active(const FpTile& s, int t) { return s.val
 __device__ __forceinline__ int fp_place(const FpTile& s, int t) { return t < s.kept ? t : t - s.t_lo + s.kept; }
 __device__ __forceinline__ int fp_tile_at(const FpTile& s, int j) { return j < s.kept ? j : j - s.kept + s.t_lo; }
 
-// maximum of a row's 64 scores, four chains of three-input maxima
-__device__ __forceinline__ float ft_rowmax(const uint32_t (&s)[64]) {
-  float m[4];
-#pragma unroll
-  for (int c = 0; c < 4; c++) m[c] = ft_max3(__uint_as_float(s[16 * c]), __uint_as_float(s[16 * c + 1]), __uint_as_float(s[16 * c + 2]));
-#pragma unroll
-  for (int i = 3; i < 15; i += 2)
-#pragma unroll
-    for (int c = 0; c < 4; c++) m[c] = ft_max3(m[c], __uint_as_float(s[16 * c + i]), __uint_as_float(s[16 * c + i + 1]));
-#pragma unroll
-  for (int c = 0; c < 4; c++) m[c] = fmaxf(m[c], __uint_as_float(s[16 * c + 15]));
-  return fmaxf(ft_max3(m[0], m[1], m[2]), m[3]);
-}
 // scores of keys the query at qpos does not see become -inf (tile t holds keys 64 t ... 64 t + 63)
 __device__ __forceinline__ void ft_mask(uint32_t (&s)[64], int t, int qpos, int qfirst, int keep) {
   bool need = (t * FT_BK + FT_BK - 1 > qpos) || (t * FT_BK < qfirst && t * FT_BK + FT_BK > keep);
@@ -557,11 +470,6 @@ __device__ __forceinline__ void ft_mask(uint32_t (&s)[64], int t, int qpos, int 
     }
   }
 }
-__device__ __forceinline__ void ft_ld64(uint32_t taddr, uint32_t (&s)[64]) {
-  tmem_ld32(taddr, *(uint32_t(*)[32])&s[0]);
-  tmem_ld32(taddr + 32, *(uint32_t(*)[32])&s[32]);
-}
-
 // One query's sums over columns c0 .. c0 + 31 of the values, key by key and over those alone that it sees. For a row whose sums are not
 // finite: on the tensor cores a page's values all enter them, with weights of zero, and 0 times what is not finite is NaN.
 __device__ __noinline__ void fp_sums_by_key(const FtArgs& p, const bf16* q, const int* bt, int g, int qpos, int qfirst, float msc, int c0, float (&acc)[32]) {

@@ -1,0 +1,434 @@
+// Attention of a step whose sequences share pages on tcgen05 tensor cores (bfloat16; keys and values of up to 128 dims in multiples of
+// 8): every shared run of pages is read once for all rows that see it. The mathematics and the plan are in share_kernels.cuh and
+// cache/share.py; results are partial and joined by share_merge_kernel.
+//
+// One block per SM stays and walks its list of items; barriers, tensor memory, the ring of pages and two query buffers live across items.
+// A tile has up to 256 rows (tokens x query heads of one key/value head) and two halves of the block work on it, each with an issuing
+// warp, four softmax warps and 256 columns of tensor memory. A tile of more than 128 rows gives each half 128 rows and the same
+// pages, so that a page is fetched once for 256 rows; a tile of at most 128 rows is worked on by both halves, which take its pages
+// in turn and leave two partial results: the chain of a page (scores, maximum, weights, product with the values), which bounds a tile of
+// few rows, then runs twice at a time. Both halves go through the one ring; a half that does not use a page gives it back as it passes.
+//
+// Rows of a tile belong to several sequences and stand anywhere in the step, so a warp gathers them (16 bytes a lane, asynchronously,
+// into the 128-byte swizzle) where keys and values come by TMA, a page and head at a time. S = Q K^T (128 x 64) and O += P V as
+// in attn_prefill_tcgen05.cu: thread = row = tensor-memory lane, P back into tensor memory as bfloat16 pairs (the weights' only
+// rounding; their sum is taken before it), O rescaled only when a row's maximum has outgrown its reference by 2^8. Warps whose rows are all past the tile's end pass the barriers and
+// compute nothing. Waits are bounded (2 s), after which the kernel raises *err, lets its copies land, frees its tensor memory and returns.
+#include "attn_tcgen05.cuh"
+#include "share_plan.cuh"
+
+#define FS_THREADS 384       // warp 0: TMA, warps 1-2: the products of either half, warp 3: queries, warps 4-7 and 8-11: softmax of either half
+#define FS_ROWS 128          // rows of a half
+#define FS_BK SLLM_PAGE
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+// 16 bytes from global to shared memory, or 16 zero bytes
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool copy) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(copy ? 16 : 0) : "memory");
+}
+
+// Keys of up to KD and values of up to VD dims (64 or 128 either): narrower ones are filled up with zeros on the chip.
+template <int KD, int VD, int STAGES>
+__global__ void __launch_bounds__(FS_THREADS, 1)
+attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ShareArgs p,
+                  uint32_t smem_bytes) {
+  constexpr uint32_t Q_BYTES = FS_ROWS * KD * 2, K_BYTES = FS_BK * KD * 2, V_BYTES = FS_BK * VD * 2;
+  constexpr uint32_t QA = FS_ROWS * 128, KA = FS_BK * 128;     // bytes of one 64-wide block of Q and of a K or V page
+  constexpr int NK = KD / 64, NV = VD / 64;
+  // tensor-memory columns of a half (256): values of 64 have S0 0-63, S1 64-127, O 128-191, P0 192-223, P1 224-255; values of 128,
+  // whose O takes 128-255, have one S 0-63 and P0 64-95, P1 96-127
+  constexpr int NBUF = VD > 64 ? 1 : 2;
+  constexpr uint32_t P_COL0 = VD > 64 ? 64 : 192, P_STEP = 32, SUB_COLS = 256;
+  static_assert(STAGES >= 4, "a half that takes every other page has its next page's scores issued ahead");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  // [two Q][K stages][V stages][barriers]
+  const uint32_t sQ = smem_u32(smem), sK = sQ + 2 * Q_BYTES, sV = sK + STAGES * K_BYTES;
+  uint64_t* bars = (uint64_t*)(smem + 2 * Q_BYTES + STAGES * (K_BYTES + V_BYTES));
+  // q_full[2], q_empty[2], kv_full[ST], kv_empty[ST], then for either half s_full[2], s_empty[2], p_full[2], o_full[2]
+  const uint32_t b_qfull = smem_u32(bars), b_qempty = b_qfull + 16, b_kvfull = b_qempty + 16, b_kvempty = b_kvfull + 8 * STAGES,
+                 b_sub = b_kvempty + 8 * STAGES;
+  constexpr uint32_t SUB_BARS = 64, B_SEMPTY = 16, B_PFULL = 32, B_OFULL = 48;
+  uint32_t* tmem_slot = (uint32_t*)(bars + 4 + 2 * STAGES + 16);
+  volatile int* abort = (volatile int*)(tmem_slot + 1);
+  if ((uint8_t*)(abort + 1) > smem_raw + smem_bytes) {      // the 1 KB alignment took more than the launch left room for
+    if (threadIdx.x == 0) atomicExch(p.err, 3);
+    return;
+  }
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int a = 0; a < 2; a++) {
+      mbar_init(b_qfull + 8 * a, 1);
+      mbar_init(b_qempty + 8 * a, 2);                // either issuing warp
+    }
+    for (int s = 0; s < STAGES; s++) {
+      mbar_init(b_kvfull + 8 * s, 1);
+      mbar_init(b_kvempty + 8 * s, 2);
+    }
+    for (int x = 0; x < 2; x++)
+      for (int a = 0; a < 2; a++) {
+        mbar_init(b_sub + SUB_BARS * x + 8 * a, 1);
+        mbar_init(b_sub + SUB_BARS * x + B_SEMPTY + 8 * a, 4);
+        mbar_init(b_sub + SUB_BARS * x + B_PFULL + 8 * a, 4);
+        mbar_init(b_sub + SUB_BARS * x + B_OFULL + 8 * a, 1);
+      }
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_launch_dependents();               // (behind the allocation: a dependent's block must not take the columns first)
+  pdl_wait();
+
+  // Every role walks the same items and counts by itself the pages fetched (JU), the pages its half has taken (J) and the query
+  // buffers used (Q: one by a tile of at most 128 rows, two by a larger one); a barrier's phase follows from those counts.
+  const int rep = p.H / p.G, i0 = p.first[blockIdx.x], i1 = p.first[blockIdx.x + 1];
+  if (warp == 0) {
+    int JU = 0;
+    bool ok = true;
+    for (int i = i0; ok && i < i1; i++) {
+      const ShareItem it = share_item(p, i);
+      const int* row = p.block_table + (size_t)it.seq * p.max_pages;
+      for (int t0 = it.p0; ok && t0 < it.p1; t0 += 32) {
+        // (a page that is none is fetched past the storage's end: zeros)
+        const int mine = t0 + lane < it.p1 ? share_page(p, row, t0 + lane) : 0, n = min(32, it.p1 - t0);
+        for (int j = 0; j < n; j++) {
+          const int page = __shfl_sync(0xffffffffu, mine, j), s = JU % STAGES;
+          if (lane == 0) {
+            ok = mbar_wait(b_kvempty + 8 * s, ((JU / STAGES) & 1) ^ 1, abort);
+            if (ok) {
+              const int at = page < 0 ? p.n_pages : page;
+              mbar_expect_tx(b_kvfull + 8 * s, K_BYTES + V_BYTES);
+#pragma unroll
+              for (int a = 0; a < NK; a++) tma_load_3d(sK + s * K_BYTES + a * KA, &map_k, 64 * a, it.g * FS_BK, at, b_kvfull + 8 * s);
+#pragma unroll
+              for (int a = 0; a < NV; a++) tma_load_3d(sV + s * V_BYTES + a * KA, &map_v, 64 * a, it.g * FS_BK, at, b_kvfull + 8 * s);
+            }
+          }
+          ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+          if (!ok) break;
+          JU++;
+        }
+      }
+    }
+    if (lane == 0 && *abort) {            // let the copies that are under way land before the block leaves
+      volatile int never = 0;
+      for (int j = max(0, JU - STAGES); j < JU; j++) mbar_wait(b_kvfull + 8 * (j % STAGES), (j / STAGES) & 1, &never);
+    }
+  } else if (warp == 3) {
+    constexpr int VECS = KD / 8;                    // 16-byte vectors of a row
+    const int k_vecs = p.hd / 8, k_used = (p.hd + 15) / 16 * 2;      // what the row has, and what the products' steps of 16 dims read
+    int Q = 0;
+    bool ok = true;
+    for (int i = i0; ok && i < i1; i++) {
+      const ShareItem it = share_item(p, i);
+      const int n_rows = it.n_tok * rep;
+      for (int b0 = 0; ok && b0 < n_rows; b0 += FS_ROWS, Q++) {
+        const int b = Q & 1;
+        // the products that read what the buffer held are done
+        if (lane == 0) ok = mbar_wait(b_qempty + 8 * b, ((Q >> 1) & 1) ^ 1, abort);
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        if (!ok) break;
+        const int c = lane % VECS;
+        if (c < k_used) {
+#pragma unroll 4
+          for (int r = lane / VECS; r < min(FS_ROWS, n_rows - b0); r += 32 / VECS) {
+            const int rho = b0 + r, tok = p.toks[it.tok0 + rho / rep];
+            cp_async16(sQ + b * Q_BYTES + (c >> 3) * QA + r * 128 + (((c & 7) ^ (r & 7)) << 4),
+                       (const bf16*)p.q + (size_t)tok * p.q_ld + (size_t)(it.g * rep + rho % rep) * p.hd + (c < k_vecs ? 8 * c : 0), c < k_vecs);
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_qfull + 8 * b);
+      }
+    }
+  } else if (warp <= 2) {
+    const bool one = elect_one();
+    const int x = warp - 1;
+    constexpr uint32_t idesc_s = umma_idesc_bf16(FS_ROWS, FS_BK);          // S = Q K^T: both K-major
+    constexpr uint32_t idesc_o = umma_idesc_bf16_bmn(FS_ROWS, VD);         // O = P V: V is MN-major (dims contiguous)
+    const uint32_t b_sfull = b_sub + SUB_BARS * x, b_sempty = b_sfull + B_SEMPTY, b_pfull = b_sfull + B_PFULL, b_ofull = b_sfull + B_OFULL;
+    const uint32_t t_sub = tmem_base + x * SUB_COLS;
+    int JU0 = 0, J0 = 0, Q = 0;
+    bool ok = true;
+    for (int i = i0; ok && i < i1; i++) {
+      const ShareItem it = share_item(p, i);
+      const bool pair = it.n_tok * rep > FS_ROWS;
+      const int n = it.p1 - it.p0, step = pair ? 1 : 2, u0 = pair ? 0 : x, n_mine = n > u0 ? (n - u0 + step - 1) / step : 0;
+      const int mine = pair ? Q + x : Q, b = mine & 1;
+      ok = mbar_wait(b_qfull + 8 * b, (mine >> 1) & 1, abort);
+      if (ok && pair) {                     // the other half's buffer: not read, given back
+        const int other = Q + 1 - x;
+        ok = mbar_wait(b_qfull + 8 * (other & 1), (other >> 1) & 1, abort);
+        if (ok && one) mbar_arrive(b_qempty + 8 * (other & 1));
+      }
+      if (!ok) break;
+      Q += pair ? 2 : 1;
+      if (n_mine <= 0 && one) mbar_arrive(b_qempty + 8 * b);
+      auto issue_s = [&](int j) -> bool {
+        const int JUg = JU0 + u0 + j * step, s = JUg % STAGES, Jg = J0 + j, sb = Jg % NBUF;
+        if (!mbar_wait(b_kvfull + 8 * s, (JUg / STAGES) & 1, abort)) return false;
+        // S(Jg) takes the place of S(Jg - NBUF), which the softmax threads have taken into their registers: with two buffers their
+        // P(Jg - 2) was waited for; the single buffer has a barrier for it
+        if (NBUF == 1 && !mbar_wait(b_sempty + 8 * sb, ((Jg / NBUF) & 1) ^ 1, abort)) return false;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < KD / 16; k++)         // 16 dims a step: four steps in each 64-wide block
+          if (16 * k < p.hd && one)
+            umma_bf16(t_sub + sb * 64, umma_desc_sw128(sQ + b * Q_BYTES + (k >> 2) * QA + (k & 3) * 32),
+                      umma_desc_sw128(sK + s * K_BYTES + (k >> 2) * KA + (k & 3) * 32), idesc_s, k ? 1u : 0u);
+        if (one) {
+          umma_commit(b_sfull + 8 * sb);
+          if (j == n_mine - 1) umma_commit(b_qempty + 8 * b);     // the item's last product of this half that reads Q
+        }
+        return true;
+      };
+      if (n_mine > 0) ok = issue_s(0);
+      for (int u = 0, j = 0; u < n && ok; u++) {
+        const int JUg = JU0 + u, s = JUg % STAGES;
+        if (!pair && (u & 1) != x) {           // the other half's page
+          ok = mbar_wait(b_kvfull + 8 * s, (JUg / STAGES) & 1, abort);
+          if (ok && one) mbar_arrive(b_kvempty + 8 * s);
+          continue;
+        }
+        if (j + 1 < n_mine) {
+          ok = issue_s(j + 1);
+          if (!ok) break;
+        }
+        const int Jg = J0 + j, a = Jg & 1;
+        ok = mbar_wait(b_pfull + 8 * a, (Jg >> 1) & 1, abort);   // P of this page is written, and O has been rescaled if it had to be
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < FS_BK / 16; k++)
+          if (one)
+            umma_bf16_ta(t_sub + 128, t_sub + P_COL0 + a * P_STEP + k * 8, umma_desc_sw128_mn(sV + s * V_BYTES + k * 2048, NV > 1 ? KA : 0),
+                         idesc_o, (j | k) ? 1u : 0u);
+        if (one) {
+          umma_commit(b_ofull + 8 * a);
+          umma_commit(b_kvempty + 8 * s);
+        }
+        j++;
+      }
+      JU0 += max(0, n);
+      J0 += n_mine;
+    }
+  } else {
+    const int x = (warp >> 2) - 1;                 // which half
+    const int q = warp & 3;                        // tensor-memory quarter of this warp
+    const int r = q * 32 + lane;                   // row of this thread in the half
+    const float sc = p.scale * FT_LOG2E;
+    const uint32_t t_lane = tmem_base + x * SUB_COLS + ((uint32_t)(q * 32) << 16);
+    const uint32_t b_sfull = b_sub + SUB_BARS * x, b_sempty = b_sfull + B_SEMPTY, b_pfull = b_sfull + B_PFULL, b_ofull = b_sfull + B_OFULL;
+    float* const ml = p.part + (size_t)p.part_rows * p.vd;
+    int JU0 = 0, J0 = 0;
+    bool ok = true;
+    for (int i = i0; ok && i < i1; i++) {
+      const ShareItem it = share_item(p, i);
+      const int n_rows = it.n_tok * rep;
+      const bool pair = n_rows > FS_ROWS;
+      const int n = it.p1 - it.p0, step = pair ? 1 : 2, u0 = pair ? 0 : x, n_mine = n > u0 ? (n - u0 + step - 1) / step : 0;
+      const int rho = pair ? x * FS_ROWS + r : r;                       // row of the tile
+      const bool warp_has_rows = rho - lane < n_rows, has_row = rho < n_rows;
+      const int tok = has_row ? p.toks[it.tok0 + rho / rep] : 0, qpos = has_row ? p.tok_pos[tok] : -1;
+      float m_ref = -INFINITY, l = 0.f;              // reference maximum (raw score units) and sum relative to it
+#pragma unroll 1
+      for (int j = 0; j < n_mine && ok; j++) {
+        const int Jg = J0 + j, a = Jg & 1, bf = Jg % NBUF, u = u0 + j * step, t = it.p0 + u;
+        uint32_t pk[32];                              // 64 weights as bfloat16 pairs: keys 2i, 2i+1
+        ok = mbar_wait(b_sfull + 8 * bf, (Jg / NBUF) & 1, abort);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (warp_has_rows) {
+          uint32_t s[64];
+          ft_ld64(t_lane + bf * 64, s);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          if (NBUF == 1) {                // the one S buffer may take the next page's scores
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(b_sempty + 8 * bf);
+          }
+          if (p.softcap > 0.f) {
+            const float cap_out = p.softcap / p.scale, cap_in = p.scale / p.softcap;
+#pragma unroll
+            for (int k = 0; k < 64; k++) s[k] = ft_cap(s[k], cap_out, cap_in);
+          }
+          if (t * FS_BK + FS_BK - 1 > qpos) {
+#pragma unroll
+            for (int k = 0; k < 64; k++)
+              if (t * FS_BK + k > qpos) s[k] = 0xff800000u;   // -inf
+          }
+          const float mx = ft_rowmax(s);
+          // ---- move the reference maximum only when the row's maximum has outgrown it by 2^8
+          const bool grow = mx > m_ref && (m_ref == -INFINITY || (mx - m_ref) * sc > 8.0f);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float factor = grow ? ((m_ref == -INFINITY) ? 0.f : ft_ex2((m_ref - mx) * sc)) : 1.f;
+            if (j >= 1) {
+              // O holds the products of the pages before: they must be complete before it is rewritten
+              ok = mbar_wait(b_ofull + 8 * (a ^ 1), ((Jg - 1) >> 1) & 1, abort);
+              if (!ok) break;
+              asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+              uint32_t v[32];
+#pragma unroll 1
+              for (int c0 = 0; c0 < VD; c0 += 32) {
+                tmem_ld32(t_lane + 128 + c0, v);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int k = 0; k < 32; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * factor);
+                tmem_st32(t_lane + 128 + c0, v);
+              }
+              asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+              asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            }
+            l *= factor;
+            if (grow) m_ref = mx;
+          }
+          const float msc = (m_ref == -INFINITY) ? 0.f : m_ref * sc;
+          uint64_t rs2 = 0ull;                          // two partial sums side by side
+          const uint64_t sc2 = ft_pack2(sc, sc), nm2 = ft_pack2(-msc, -msc);
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {
+            float x0, x1, x2, x3;
+            ft_unpack2(ft_fma2(ft_pack2(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), sc2, nm2), x0, x1);
+            ft_unpack2(ft_fma2(ft_pack2(__uint_as_float(s[2 * k + 2]), __uint_as_float(s[2 * k + 3])), sc2, nm2), x2, x3);
+            const float e0 = ft_ex2(x0), e1 = ft_ex2(x1), e2 = ft_ex2(x2), e3 = ft_ex2(x3);
+            rs2 = ft_add2(rs2, ft_add2(ft_pack2(e0, e1), ft_pack2(e2, e3)));
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(e0, e1), hi = __floats2bfloat162_rn(e2, e3);
+            pk[k] = *(const uint32_t*)&lo;
+            pk[k + 1] = *(const uint32_t*)&hi;
+          }
+          float ra, rb;
+          ft_unpack2(rs2, ra, rb);
+          l += ra + rb;
+        } else if (NBUF == 1) {
+          if (lane == 0) mbar_arrive(b_sempty + 8 * bf);
+        }
+        if (t * FS_BK + FS_BK - 1 > it.last) {
+          // keys behind the tile's last token hold whatever the page held before, or what this tile does not see: their weights are
+          // zero, but 0 * NaN is NaN, so their value rows are cleared, by either half before its own product
+          const int JUg = JU0 + u, st = JUg % STAGES, n_valid = max(0, it.last + 1 - t * FS_BK);
+          ok = mbar_wait(b_kvfull + 8 * st, (JUg / STAGES) & 1, abort);
+          if (!ok) break;
+          for (int e = q * 32 + lane; e < (FS_BK - n_valid) * 8 * NV; e += 128) {
+            const int blk = e / ((FS_BK - n_valid) * 8), e1 = e % ((FS_BK - n_valid) * 8), vr = n_valid + e1 / 8, c = e1 % 8;
+            *(uint4*)(smem + 2 * Q_BYTES + STAGES * K_BYTES + st * V_BYTES + blk * KA + vr * 128 + ((c ^ (vr & 7)) << 4)) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        }
+        // ---- P into tensor memory. The product that read this buffer's last P, two pages ago, is complete: it was issued before
+        // S(Jg), and the commit that announced S(Jg) covers every product issued before it.
+        if (warp_has_rows) {
+          tmem_st32(t_lane + P_COL0 + a * P_STEP, pk);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(b_pfull + 8 * a);
+      }
+      if (ok && n_mine > 0) ok = mbar_wait(b_ofull + 8 * ((J0 + n_mine - 1) & 1), ((J0 + n_mine - 1) >> 1) & 1, abort);
+      if (ok && warp_has_rows) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const size_t at = (size_t)it.part0 + rho + (pair || x == 0 ? 0 : n_rows);
+        const float m = m_ref * sc;
+        if (n_mine > 0) {
+#pragma unroll 1
+          for (int c0 = 0; c0 < VD; c0 += 32) {
+            uint32_t v[32];
+            tmem_ld32(t_lane + 128 + c0, v);
+            asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+            float any = 0.f;                            // not 0: something is not finite (a sum l that is not has seen a score that is not)
+#pragma unroll
+            for (int k = 0; k < 32; k++) any = fmaf(__uint_as_float(v[k]), 0.f, any);
+            if (has_row) {
+              if (any != 0.f && l < INFINITY) {
+                const bf16* qr = (const bf16*)p.q + (size_t)tok * p.q_ld + (size_t)(it.g * rep + rho % rep) * p.hd;
+#pragma unroll 1
+                for (int c = 0; c < 32 && c0 + c < p.vd; c += 4)
+                  *(float4*)(p.part + at * p.vd + c0 + c) = share_sum_by_key(p, it, qr, qpos, m, c0 + c, it.p0 + u0, step);
+              } else {
+#pragma unroll
+                for (int c = 0; c < 32; c += 4)
+                  if (c0 + c < p.vd)
+                    *(float4*)(p.part + at * p.vd + c0 + c) = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]),
+                                                                          __uint_as_float(v[c + 3]));
+              }
+            }
+            __syncwarp();
+          }
+        }
+        if (has_row) *(float2*)(ml + 2 * at) = make_float2(m, l);
+      }
+      // the rows of O are read (the loads above were waited for) before this thread signals the next item's first P
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      JU0 += max(0, n);
+      J0 += n_mine;
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
+  if (threadIdx.x == 0 && *abort) atomicExch(p.err, 2);
+}
+
+// pages [n_pages][G * 64][width] bfloat16; a box is 64 columns of one head's 64 positions, 128-byte swizzle, zero fill
+static int fs_make_map(CUtensorMap* map, const void* base, long long n_pages, int G, int width) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return SLLM_ERR_ARG - 1;
+  cuuint64_t dims[3] = {(cuuint64_t)width, (cuuint64_t)G * FS_BK, (cuuint64_t)n_pages};
+  cuuint64_t strides[2] = {(cuuint64_t)width * 2, (cuuint64_t)G * FS_BK * width * 2};
+  cuuint32_t box[3] = {64, FS_BK, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? 0 : SLLM_ERR_ARG - 2;
+}
+
+template <int KD, int VD, int STAGES>
+static int fs_launch(const CUtensorMap& mk, const CUtensorMap& mv, const ShareArgs& a, int workers, cudaStream_t stream) {
+  // what the kernel lays out after aligning to 1 KB; one block on an SM
+  constexpr size_t need = 2 * FS_ROWS * KD * 2 + STAGES * FS_BK * (KD + VD) * 2 + 512;
+  constexpr size_t smem = need + 1024;
+  static_assert(smem <= 232448, "the block of this head width does not fit an SM");
+  static SllmPerDevice allowed;
+  const cudaError_t e = sllm_allow_smem(allowed, attn_share_kernel<KD, VD, STAGES>, smem);
+  if (e != cudaSuccess) return (int)e;
+  return (int)sllm_launch(attn_share_kernel<KD, VD, STAGES>, dim3(workers), dim3(FS_THREADS), smem, stream, mk, mv, a, (uint32_t)smem);
+}
+
+// first [workers + 1], items [.][8], toks [T]: a plan's for tiles of 256 rows in halves; part: part_rows * (vd + 2) floats.
+SLLM_EXPORT int sllm_share_attn_tc_bf16(const void* q, int q_ld, const int* tok_pos, const int* block_table, int max_pages, const void* kpages,
+                                        const void* vpages, long long n_pages, const int* first, const int* items, const int* toks,
+                                        int workers, float* part, long long part_rows, int H, int G, int hd, int vd, float scale, float softcap,
+                                        int* err, cudaStream_t stream) {
+  if (workers <= 0) return 0;
+  if (hd < 8 || hd > 128 || hd % 8 || vd < 8 || vd > 128 || vd % 8 || G < 1 || H < 1 || H % G != 0 || H / G > 2 * FS_ROWS || q_ld < H * hd || (q_ld & 7) ||
+      n_pages < 1 || n_pages > 0x7fffffffLL || (long long)G * FS_BK > 0x7fffffffLL || part_rows < 1 || max_pages < 1 ||
+      ((uintptr_t)q & 15) || ((uintptr_t)kpages & 15) || ((uintptr_t)vpages & 15) || ((uintptr_t)part & 15) || ((uintptr_t)items & 15))
+    return SLLM_ERR_ARG;
+  ShareArgs a{q, q_ld, tok_pos, block_table, max_pages, kpages, vpages, (int)n_pages, first, items, toks, part, part_rows, H, G, hd, vd, scale,
+              softcap, err};
+  CUtensorMap mk, mv;
+  int rc = fs_make_map(&mk, kpages, n_pages, G, hd);
+  if (rc) return rc;
+  rc = fs_make_map(&mv, vpages, n_pages, G, vd);
+  if (rc) return rc;
+  if (vd <= 64) {
+    if (hd <= 64) return fs_launch<64, 64, 10>(mk, mv, a, workers, stream);
+    return fs_launch<128, 64, 6>(mk, mv, a, workers, stream);
+  }
+  if (hd <= 64) return fs_launch<64, 128, 7>(mk, mv, a, workers, stream);
+  return fs_launch<128, 128, 5>(mk, mv, a, workers, stream);
+}

@@ -1725,8 +1725,11 @@ class SharedAttention:
             raise KernelError(f"no kernels for {dtype}; supported: float32, bfloat16")
         self.dtype, self.suffix = dtype, _SUFFIX[dtype]
         self.lib = load_library(f"share_{self.suffix}")
-        for n in ("share_attn", "share_merge"):
-            getattr(self.lib, f"sllm_{n}_{self.suffix}").restype = c_int
+        self._attn, self._merge = (getattr(self.lib, f"sllm_share_{n}_{self.suffix}") for n in ("attn", "merge"))
+        self._attn_tc = load_library("attn_share_tcgen05").sllm_share_attn_tc_bf16 if dtype == torch.bfloat16 else None
+        for fn in (self._attn, self._merge, self._attn_tc):
+            if fn is not None:
+                fn.restype = c_int
 
     @staticmethod
     def takes(head_dim: int, v_dim: int, rep: int = 1) -> bool:
@@ -1739,6 +1742,8 @@ class SharedAttention:
             raise KernelError(f"shared attention takes widths in multiples of 4 up to 256, not keys of {head_dim} and values of {v_dim}")
         if sm_count is None:
             sm_count = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+        if self.dtype == torch.bfloat16 and all(w % 8 == 0 and w <= 128 for w in (head_dim, v_dim)):
+            return TileShape(rows=256, workers=sm_count, halves=True, item_pages=1.0, half_cost=0.7)       # tcgen05
         return TileShape(rows=64, workers=2 * sm_count)
 
     def attn(self, q, out, tok_pos, block_table, kpages, vpages, plan, part, scale, err_flag, softcap=None, sink=None):
@@ -1769,13 +1774,13 @@ class SharedAttention:
         if T == 0:
             return
         rows = plan.capacity.rows
-        _check(getattr(self.lib, f"sllm_share_attn_{self.suffix}")(
+        _check((self._attn_tc if shape.halves else self._attn)(
             c_void_p(q.data_ptr()), q.stride(0), _ptr(tok_pos, torch.int32, "tok_pos"), _ptr(block_table, torch.int32, "block_table"),
             block_table.shape[1], _ptr(kpages, self.dtype, "kpages"), _ptr(vpages, self.dtype, "vpages"), c_longlong(kpages.shape[0]),
             _ptr(plan.first, torch.int32, "plan"), _ptr(plan.items, torch.int32, "plan"), _ptr(plan.toks, torch.int32, "plan"),
             as_int(shape.workers), _ptr(part, torch.float32, "part"), c_longlong(rows), as_int(H), as_int(G), hd, vd, c_float(scale),
             c_float(softcap or 0.0), _ptr(err_flag, torch.int32, "err_flag"), _stream()), "share_attn")
-        _check(getattr(self.lib, f"sllm_share_merge_{self.suffix}")(
+        _check(self._merge(
             _ptr(part, torch.float32, "part"), c_longlong(rows), _ptr(plan.list_first, torch.int32, "plan"), _ptr(plan.list, torch.int32, "plan"),
             _ptr(out, self.dtype, "out"), _ptr(sink, torch.float32, "sink"), as_int(T), as_int(H), as_int(G), vd, _stream()), "share_merge")
 

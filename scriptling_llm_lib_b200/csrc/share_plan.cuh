@@ -1,0 +1,84 @@
+// The plan of an attention over shared pages (cache/share.py) as its kernels read it.
+#pragma once
+#include "common.cuh"
+
+#define SHARE_LOG2E 1.4426950408889634f
+#define SHARE_ERR_PAGE 5          // what *err says: a page id outside the storage, or a position outside the block table
+
+struct ShareArgs {
+  const void* q;             // [T, q_ld] queries that have their positions; head h at columns h * hd
+  int q_ld;
+  const int* tok_pos;        // [T]
+  const int* block_table;    // [n_seqs, max_pages]
+  int max_pages;
+  const void *kpages, *vpages;   // [n_pages][G][PAGE][hd], [n_pages][G][PAGE][vd]
+  int n_pages;
+  const int *first, *items, *toks;   // of the plan: where a block's items begin, items of eight words, rows of the step in the tree's order
+  float* part;               // [part_rows][vd], then [part_rows][2]: m and l
+  long long part_rows;
+  int H, G, hd, vd;
+  float scale, softcap;
+  int* err;
+};
+
+// An item as a block works on it: pages [p0, p1) of row `seq` of the table; keys up to `last`, the position of its last token
+struct ShareItem {
+  int tok0, n_tok, g, p0, p1, last, part0, seq;
+};
+__device__ __forceinline__ ShareItem share_item(const ShareArgs& p, int i) {
+  const int4 a = *(const int4*)(p.items + 8 * (size_t)i), b = *(const int4*)(p.items + 8 * (size_t)i + 4);
+  ShareItem it;
+  it.tok0 = a.x;
+  it.n_tok = a.y;
+  it.last = p.tok_pos[a.z];
+  it.g = a.w;
+  it.p0 = b.x;
+  const int end = it.last / SLLM_PAGE + 1;         // (a plan may be older than the step, and the sequences shorter or longer)
+  it.p1 = b.y < 0 || b.y > end ? end : b.y;
+  it.part0 = b.z;
+  it.seq = b.w;
+  return it;
+}
+// the page at place `i` of a row of the table; -1 (and *err) where there is none
+__device__ __forceinline__ int share_page(const ShareArgs& p, const int* row, int i) {
+  const int page = i < p.max_pages ? row[i] : -1;
+  if (page >= 0 && page < p.n_pages) return page;
+  atomicExch(p.err, SHARE_ERR_PAGE);
+  return -1;
+}
+
+// Four elements of a row's weighted sum of values, key by key and over those alone that it sees: for a row whose sum came out not
+// finite. In a tile's product a page's values all enter it, with weights of zero, and 0 times what is not finite is NaN. Pages t0,
+// t0 + step, ... of the item's.
+template <typename A>
+__device__ __noinline__ float4 share_sum_by_key(const ShareArgs& p, const ShareItem& it, const A* q, int qpos, float m, int d0, int t0, int step) {
+  const int* row = p.block_table + (size_t)it.seq * p.max_pages;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int key = t0 * SLLM_PAGE; key <= qpos && key < it.p1 * SLLM_PAGE; key++) {
+    if (key % SLLM_PAGE == 0 && (key / SLLM_PAGE - t0) % step) {        // a page of the other half's
+      key += SLLM_PAGE - 1;
+      continue;
+    }
+    const int page = share_page(p, row, key / SLLM_PAGE);
+    if (page < 0) continue;
+    const size_t at = ((size_t)page * p.G + it.g) * SLLM_PAGE + key % SLLM_PAGE;
+    const A *k = (const A*)p.kpages + at * p.hd, *v = (const A*)p.vpages + at * p.vd + d0;
+    float s = 0.f;
+    for (int d = 0; d < p.hd; d += 4) {
+      const float4 a = ld4(q + d), b = ld4(k + d);
+      s = fmaf(a.x, b.x, s);
+      s = fmaf(a.y, b.y, s);
+      s = fmaf(a.z, b.z, s);
+      s = fmaf(a.w, b.w, s);
+    }
+    s *= p.scale;
+    if (p.softcap > 0.f) s = p.softcap * tanhf(s / p.softcap);
+    const float w = exp2f(fmaf(s, SHARE_LOG2E, m == -INFINITY ? 0.f : -m));
+    const float4 x = ld4(v);
+    acc.x = fmaf(w, x.x, acc.x);
+    acc.y = fmaf(w, x.y, acc.y);
+    acc.z = fmaf(w, x.z, acc.z);
+    acc.w = fmaf(w, x.w, acc.w);
+  }
+  return acc;
+}
