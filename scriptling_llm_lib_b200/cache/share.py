@@ -73,9 +73,12 @@ def share_tree(table: np.ndarray, whole: np.ndarray):
     return order, nodes, np.asarray(own, dtype=np.int64)
 
 
-def saved_pages(nodes) -> int:
-    """Pages that a step need not read again."""
-    return sum((hi - lo - 1) * (b - a) for lo, hi, a, b in nodes)
+def share_pays(tree, held, new) -> bool:
+    """Whether a step of these sequences is faster by the tree than each sequence for itself."""
+    if tree is None:
+        return False
+    saved = sum((hi - lo - 1) * (b - a) for lo, hi, a, b in tree[1])
+    return saved > 0
 
 
 class SharePlan:
@@ -97,6 +100,14 @@ class SharePlan:
             host = self.host()
             self.dev = torch.from_numpy(host).to(device)
             self._views()
+
+    def again(self, other: "SharePlan") -> np.ndarray:
+        """Take the layout of another plan of the same rows, heads, shape and capacity; the words for the device's buffer."""
+        same = lambda p: (p.n_seqs, p.n_rows, p.n_heads, p.n_kv, p.shape, p.capacity)        # noqa: E731
+        if same(other) != same(self):
+            raise ValueError(f"a plan of {same(other)} cannot stand where one of {same(self)} does")
+        self.parts, self.n_items, self.n_list, self.part_rows = other.parts, other.n_items, other.n_list, other.part_rows
+        return self.host()
 
     def fits(self, cap: "PlanCapacity") -> bool:
         return self.n_items <= cap.items and self.n_list <= cap.entries and self.part_rows <= cap.rows

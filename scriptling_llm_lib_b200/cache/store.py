@@ -10,6 +10,11 @@ a list of pages, position p living in page p // PAGE. One page id serves all uni
 Pages come from the group's pool as the sequence grows and go back when it is closed, or, in a
 window group, as soon as no later query can see them. Nothing relies on cleared memory: every read
 is bounded by the sequence's length.
+
+A sequence can be forked: the new slots hold the same pages (a page's id then has several holders in its pool) and copies of the
+fixed-size states. A page that several hold is never written: the step that would write its free positions first gives the
+writer a page of its own with the positions held so far (`reserve`). Pages can be moved to the front of their storage, or into a
+storage of another size, while sequences hold them (`compact`).
 """
 from __future__ import annotations
 
@@ -19,6 +24,7 @@ import numpy as np
 import torch
 
 from .needs import PAGE, CacheNeed, StateNeed
+from .share import share_tree
 
 SEQ_STATE_WORDS = 8      # int32 words of a sequence's record (lib_sampling.cu has the same layout)
 SEQ_POS, SEQ_GENERATED, SEQ_LAST_TOKEN, SEQ_FLAGS, SEQ_KEY, SEQ_COUNTER = 0, 1, 2, 3, 4, 6
@@ -76,6 +82,49 @@ class KVGroup:
             i += 1
         self.behind[slot] = i
 
+    def fork(self, slot: int, new: int, length: int) -> None:
+        """The new slot holds what `slot` holds of its first `length` positions: the same pages."""
+        lst = self.pages[slot][:pages_for(length)]
+        for pg in lst:
+            if pg >= 0:
+                self.pool.share(pg)
+        self.pages[new] = lst
+        self.table[new, :len(lst)] = lst
+        self.behind[new] = self.behind[slot]
+
+    def shared_written(self, slot: int, length: int, n: int) -> list[int]:
+        """Places of the slot's pages that `n` tokens behind `length` would be written to and that others hold too."""
+        lst = self.pages[slot]
+        return [i for i in range(length // PAGE, min(len(lst), pages_for(length + n))) if lst[i] >= 0 and self.pool.holders(lst[i]) > 1]
+
+    def copies_needed(self, growth, length) -> int:
+        """Pages that a step which adds to these slots has to make its own first: every writer of a shared page needs one, but where all
+        its holders write the last of them keeps it."""
+        if not self.pool.n_shared:
+            return 0
+        writers: dict[int, int] = {}
+        for slot, n in growth:
+            for i in self.shared_written(slot, length[slot], n):
+                page = self.pages[slot][i]
+                writers[page] = writers.get(page, 0) + 1
+        return sum(min(k, self.pool.holders(page) - 1) for page, k in writers.items())
+
+    def own_written(self, slot: int, length: int, n: int) -> list[tuple[int, int, int]]:
+        """Give the slot pages of its own where it would write shared ones: (from, to, positions held) of each."""
+        out = []
+        for i in self.shared_written(slot, length, n):
+            page, mine = self.pages[slot][i], self.pool.alloc()
+            self.pool.free(page)
+            self.pages[slot][i] = self.table[slot, i] = mine
+            out.append((page, mine, max(0, length - i * PAGE)))
+        return out
+
+    def renumber(self, to: dict[int, int], n: int | None = None) -> None:
+        self.pool.renumber(to, n)
+        for slot, lst in self.pages.items():
+            lst[:] = [to[pg] if pg >= 0 else -1 for pg in lst]
+            self.table[slot, :len(lst)] = lst
+
     def release_all(self, slot: int) -> None:
         lst = self.pages.pop(slot)
         for pg in lst:
@@ -92,9 +141,13 @@ class SequenceCache:
                  n_slots: int, n_pages: int, dtype: torch.dtype, device):
         if n_slots < 1 or n_pages < 1:
             raise ValueError("the cache needs at least one slot and one page")
-        self.n_slots, self.n_pages, self.dtype, self.device = n_slots, n_pages, dtype, device
+        self.n_slots, self.n_pages, self.dtype, self.device = n_slots, n_pages, dtype, torch.device(device)
         self.slots = FreeList(n_slots, "cache slot")
         self.length = [0] * n_slots
+        self.version = 0          # changes whenever slots come to hold other pages than they did, but for pages added at their end
+        self._trees: dict = {}
+        self._kernels = None
+        self.err_flag = None      # where the copying kernels report (an engine's; made on first use else)
         by_need: dict[CacheNeed, list[int]] = {}
         for unit, need in cache_needs.items():
             if need is not None:
@@ -126,6 +179,7 @@ class SequenceCache:
     def open(self) -> int:
         slot = self.slots.alloc()
         self.length[slot] = 0
+        self.version += 1
         for g in self.groups:
             g.open(slot)
         def zero(st):
@@ -154,17 +208,136 @@ class SequenceCache:
             g.release_all(slot)
         self.slots.free(slot)
         self.length[slot] = 0
+        self.version += 1
+
+    # ------------------------------------------------------------------ copies
+    def _ids(self, *lists):
+        """Lists of numbers as int32 tensors on the cache's device, in one copy."""
+        host = torch.tensor(list(lists), dtype=torch.int32)
+        if self.device.type == "cuda":
+            host = host.pin_memory()
+        return host.to(self.device, non_blocking=True)
+
+    def _copy(self, pairs, src, dst, rows=None, slots=False) -> None:
+        """Copies of pages (the first `rows` positions of each, None: all) or of slots, from one tensor to another or within one. A cache
+        that is not on a CUDA device does bookkeeping alone (its tests); its few bytes go by indexing."""
+        if not src or not pairs:
+            return
+        if self.device.type != "cuda":
+            for a, b in pairs:
+                for i, (s, d) in enumerate(zip(src, dst)):
+                    if slots:
+                        b[d] = a[s]
+                    else:
+                        n = PAGE if rows is None else rows[i]
+                        b[:, d, :, :n] = a[:, s, :, :n]
+            return
+        if self._kernels is None:
+            from ..csrc.bindings import PageKernels
+            self._kernels = PageKernels()
+        if self.err_flag is None:
+            self.err_flag = torch.zeros(1, dtype=torch.int32, device=self.device)
+        ids = self._ids(src, dst, *([rows] if rows is not None else []))
+        if slots:
+            self._kernels.copy_slots(pairs, ids[0], ids[1], self.err_flag)
+        else:
+            self._kernels.copy_pages(pairs, ids[0], ids[1], ids[2] if rows is not None else None, self.err_flag)
+
+    def _states(self) -> list[torch.Tensor]:
+        out, todo = [self.seq_state], list(self.state.values())
+        while todo:
+            st = todo.pop()
+            if isinstance(st, dict):
+                todo.extend(st.values())
+            else:
+                out.append(st)
+        return out
+
+    def fork(self, slot: int, n: int = 1) -> list[int]:
+        """`n` new slots that hold what `slot` holds: the same pages, copies of its states and of its record (its sampling stream goes on
+        in each: `seed` starts others). All or CacheFull."""
+        if not self.slots.is_held(slot):
+            raise ValueError(f"cache slot {slot} is not held; it cannot be forked")
+        if n < 0:
+            raise ValueError(f"{n} forks of a sequence")
+        if n > self.slots.n_free:
+            raise CacheFull(f"{n} forks of a sequence; {self.slots.n_free} of {self.slots.n} cache slots are free")
+        new = [self.slots.alloc() for _ in range(n)]
+        for s in new:
+            self.length[s] = self.length[slot]
+            for g in self.groups:
+                g.fork(slot, s, self.length[slot])
+        self._copy([(t, t) for t in self._states()], [slot] * n, new, slots=True)
+        self.version += 1
+        return new
+
+    def compact(self, n_pages: int | None = None) -> int:
+        """Move the held pages of every group to the front of its storage; with `n_pages`, into a new storage of that many (fewer give
+        memory back, more make room). Returns the number of pages that were copied; CacheFull, with nothing changed, where more are
+        held. Kernels that were captured with the old storage's addresses are the caller's to drop."""
+        if n_pages is not None:
+            if n_pages < 1:
+                raise ValueError("the cache needs at least one page")
+            for g in self.groups:
+                if g.pool.n_held > n_pages:
+                    raise CacheFull(f"{g.pool.n_held} pages of the {g.need.kind} group are held; {n_pages} are to be kept")
+        moved = 0
+        for g in self.groups:
+            held = [i for i in range(g.pool.n) if g.pool.is_held(i)]
+            if n_pages is None:
+                k = len(held)
+                to = {i: i for i in held if i < k}
+                room = [i for i in range(k) if i not in to]
+                to.update(zip((i for i in held if i >= k), room))
+                src = [i for i in held if i >= k]
+                self._copy([(g.k, g.k), (g.v, g.v)], src, [to[i] for i in src])
+            else:
+                to, src = {i: j for j, i in enumerate(held)}, held
+                for name in ("k", "v"):        # (one after the other: both old and new are held meanwhile)
+                    old = getattr(g, name)
+                    new = torch.empty((old.shape[0], n_pages + 1, *old.shape[2:]), dtype=old.dtype, device=old.device)
+                    self._copy([(old, new)], src, [to[i] for i in src])
+                    setattr(g, name, new)
+                    del old
+            g.renumber(to, n_pages)
+            moved += len(src)
+        if n_pages is not None:
+            self.n_pages = n_pages
+        self.version += 1
+        return moved
+
+    # ------------------------------------------------------------------ what sequences share
+    @property
+    def shares_pages(self) -> bool:
+        return any(g.pool.n_shared for g in self.groups)
+
+    def share_tree(self, group: int, slots: list[int]):
+        """`share_tree` of these slots' pages, kept until slots come to hold other pages."""
+        if not self.groups[group].pool.n_shared:
+            return None
+        if self._trees.get("version") != self.version or len(self._trees) > 64:
+            self._trees = {"version": self.version}
+        key = (group, tuple(slots))
+        if key not in self._trees:
+            whole = np.asarray([self.length[s] // PAGE for s in slots], dtype=np.int64)
+            self._trees[key] = share_tree(np.ascontiguousarray(self.block_table(group, slots)), whole)
+        return self._trees[key]
 
     # ------------------------------------------------------------------ growth
     def reserve(self, growth: list[tuple[int, int]]) -> None:
         """Pages for `n_new` more tokens of each (slot, n_new); either all are had or CacheFull is
-        raised and nothing has changed."""
+        raised and nothing has changed. A slot that would write a page that others hold too gets a copy of its own."""
         for g in self.groups:
-            want = sum(g.pages_needed(slot, self.length[slot] + n) for slot, n in growth)
+            want = sum(g.pages_needed(slot, self.length[slot] + n) for slot, n in growth) + g.copies_needed(growth, self.length)
             if want > g.pool.n_free:
                 raise CacheFull(f"the step needs {want} more cache pages of {PAGE} tokens in the {g.need.kind} group; "
                                 f"{g.pool.n_free} of {g.pool.n} are free")
         for g in self.groups:
+            if g.pool.n_shared:
+                own = [c for slot, n in growth for c in g.own_written(slot, self.length[slot], n)]
+                if own:
+                    self.version += 1
+                    self._copy([(g.k, g.k), (g.v, g.v)], *(list(c) for c in zip(*own)))
             for slot, n in growth:
                 g.grow(slot, self.length[slot] + n)
 

@@ -3,7 +3,8 @@ option names and defaults (-model, -prompt, -tokens 200, -strategy greedy, -temp
 -top-k 50, -top-p 0.9, -repeat-penalty 1.1, -repeat-last-n 64, -kernel-info), generated ids on
 standard output, the two timing lines on standard error. The prompt is a list of token ids
 ("1,2,3" or "1 2 3"; several prompts separated by ';' form a batch), since tokenizer and chat
-template are not part of this library. Added: -dtype, -seed, -stop, and `-random CONFIG.json
+template are not part of this library. Added: -dtype, -seed, -stop, -n (continuations of every prompt, a line each),
+-share-prefix (what the prompts begin with in common goes through the model once), and `-random CONFIG.json
 -seed-weights S` which first writes a random-weights model folder to -model.
 """
 from __future__ import annotations
@@ -45,6 +46,9 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("-dtype", "--dtype", default="bfloat16", choices=["bfloat16", "float32"])
     ap.add_argument("-seed", "--seed", type=int, default=0, help="Seed of the sampling streams")
     ap.add_argument("-stop", "--stop", default=None, help="Stop token ids (default: config.json's eos ids; '' for none)")
+    ap.add_argument("-n", "--n", type=int, default=1, help="Continuations of every prompt, one line of ids each")
+    ap.add_argument("-share-prefix", "--share-prefix", dest="share_prefix", action="store_true",
+                    help="Run what the prompts begin with in common through the model once")
     ap.add_argument("-random", "--random", default=None, metavar="CONFIG.json",
                     help="Write a random-weights model for this config.json into -model first")
     ap.add_argument("-seed-weights", "--seed-weights", dest="seed_weights", type=int, default=0)
@@ -90,7 +94,9 @@ def main(argv=None) -> int:
         ids, st = llm.generate(args.model, prompts, args.tokens, args.strategy, temperature=args.temperature,
                                top_k=args.top_k, top_p=args.top_p, repeat_penalty=args.repeat_penalty,
                                repeat_last_n=args.repeat_last_n, seed=args.seed, stop_ids=stop, dtype=args.dtype,
-                               stats=True)
+                               stats=True, n=args.n, share_prefix=args.share_prefix)
+        if args.n > 1:
+            ids, st = [o for outs in ids for o in outs], {k: [x for some in v for x in some] for k, v in st.items()}
     except Exception as e:  # the reference prints "error: ..." and exits 1 (examples/infer/main.go:99-102)
         print(f"error: {e}", file=sys.stderr)
         return 1

@@ -8,6 +8,10 @@ in the output and counted, and ends its sequence; the last sampled token is not 
 (model_f32.go:598-602). Sequences of a batch end independently; requests beyond what fits at once
 run as further batches on the slots the earlier ones gave back.
 
+Prompts that begin alike can share what they begin with (`share_prefix`, and `n` continuations of each prompt): the common run of
+tokens goes through the model once, its sequence is forked for the others, and later steps read its pages once for all. The sampled
+tokens are those that the requests would give alone, but for rounding.
+
 The loop's decisions (who is live, who stops and why, how requests are split into batches) are
 plain Python over token ids, so they can be tested with a scripted step function.
 """
@@ -16,6 +20,7 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 from typing import Callable, Sequence as Seq
 
+import numpy as np
 import torch
 
 from ..cache.needs import PAGE
@@ -36,23 +41,62 @@ class GenerationResult:
 
 
 def plan_batches(prompt_lens: Seq[int], max_tokens: int, max_seqs: int, page_capacity: int,
-                 max_positions: int) -> list[list[int]]:
+                 max_positions: int, n: int = 1) -> list[list[int]]:
     """Split request indices, in order, into batches that fit `max_seqs` slots and `page_capacity`
-    cache pages when every request runs to its longest (prompt + max_tokens - 1 tokens held)."""
+    cache pages when every request runs to its longest (prompt + max_tokens - 1 tokens held). With `n` > 1 requests n k to
+    n k + n - 1 are one prompt: within a batch those behind the first need no pages for what they share."""
     batches, cur, cur_pages = [], [], 0
-    for i, n in enumerate(prompt_lens):
-        held = min(max_positions, min(n, max_positions) + max_tokens - 1)
-        pages = (max(held, 1) + PAGE - 1) // PAGE
-        if pages > page_capacity:
-            raise ValueError(f"request {i} needs {pages} cache pages ({held} tokens); the cache has {page_capacity}")
-        if cur and (len(cur) >= max_seqs or cur_pages + pages > page_capacity):
+    for i, length in enumerate(prompt_lens):
+        own, shared = request_pages(length, max_tokens, max_positions)
+        if own + shared > page_capacity:
+            raise ValueError(f"request {i} needs {own + shared} cache pages; the cache has {page_capacity}")
+        again = bool(cur) and i % n != 0
+        if cur and (len(cur) >= max_seqs or cur_pages + own + (0 if again else shared) > page_capacity):
             batches.append(cur)
-            cur, cur_pages = [], 0
+            cur, cur_pages, again = [], 0, False
         cur.append(i)
-        cur_pages += pages
+        cur_pages += own + (0 if again else shared)
     if cur:
         batches.append(cur)
     return batches
+
+
+def request_pages(length: int, max_tokens: int, max_positions: int) -> tuple[int, int]:
+    """Pages that a request needs when it runs to its longest: its own, and those that it shares with others of the same prompt (all
+    of the prompt but its last token is shared, in whole pages)."""
+    prompt = min(length, max_positions)
+    held = min(max_positions, prompt + max_tokens - 1)
+    shared = (prompt - 1) // PAGE
+    return (max(held, 1) + PAGE - 1) // PAGE - shared, shared
+
+
+def shared_runs(prompts: Seq[Seq[int]], alike: Seq | None = None) -> list[tuple[int, list[int], int, int]]:
+    """What prompts begin with in common, as a tree: (depth, members, start, end) says that these prompts are the same up to `end`, and
+    up to `start`, where their parent ends (0: they have none), with others too. Parents stand before their children. Every prompt keeps
+    its last token for itself. With `alike`, only prompts with the same entry there are compared."""
+    key = (lambda i: (alike[i], prompts[i])) if alike is not None else (lambda i: prompts[i])
+    order = sorted(range(len(prompts)), key=key)
+    arrays = [np.asarray(prompts[i], dtype=np.int64) for i in order]
+    lcp = []
+    for (i, a), (j, b) in zip(zip(order, arrays), zip(order[1:], arrays[1:])):
+        n = min(len(a), len(b)) - 1
+        same = a[:n] == b[:n]
+        lcp.append(0 if alike is not None and alike[i] != alike[j] else n if same.all() else int(same.argmin()))
+    runs, stack = [], [(0, len(order), 0, 0)]
+    while stack:
+        lo, hi, start, depth = stack.pop()
+        if hi - lo < 2:
+            continue
+        m = min(lcp[lo:hi - 1])
+        if m // PAGE > start // PAGE:          # a whole page more that is held once
+            runs.append((depth, [order[k] for k in range(lo, hi)], start, m))
+            start, depth = m, depth + 1
+        at = lo
+        for k in range(lo, hi):
+            if k == hi - 1 or lcp[k] == m:
+                stack.append((at, k + 1, start, depth))
+                at = k + 1
+    return sorted(runs, key=lambda r: r[0])
 
 
 @dataclass
@@ -115,15 +159,45 @@ class Generator:
     def __init__(self, engine, sampler):
         self.engine, self.sampler = engine, sampler
 
+    def _open(self, seqs: dict, n: int, state: BatchState, runs) -> list[int]:
+        """Open a batch's sequences into `seqs`, the runs of tokens that they share run once, level by level of the tree, and their
+        sequences forked for the members. Returns the prompt tokens that each holds already."""
+        from .step import StepEntry
+        done = [0] * n
+        for depth in range(1 + max((r[0] for r in runs), default=-1)):
+            level = [r for r in runs if r[0] == depth]
+            for _, members, start, _ in level:
+                if members[0] not in seqs:               # (a deeper run's members were forked with their parent's)
+                    seqs[members[0]] = self.engine.open()
+            self.engine.prompt_step([StepEntry(seqs[m[0]], state.seqs[m[0]].prompt[a:b]) for _, m, a, b in level])
+            # a run's first member goes on with its sequence; the others, but for those that share a deeper run with one before, fork it
+            deeper = {i: r[1][0] for r in runs if r[0] == depth + 1 for i in r[1]}
+            for _, members, _, end in level:
+                heads = [i for i in members[1:] if deeper.get(i, i) == i]
+                seqs.update(zip(heads, self.engine.fork(seqs[members[0]], len(heads))))
+                for i in members:
+                    done[i] = end
+        for i in range(n):
+            if i not in seqs:
+                seqs[i] = self.engine.open()
+        return done
+
     def generate(self, prompts: list[list[int]], max_tokens: int = 100, options: SamplingOptions | None = None,
                  stop_ids=None, seed: int = 0, max_batch: int | None = None,
-                 on_step: Callable[[int, dict[int, int]], bool | None] | None = None) -> list[GenerationResult]:
+                 on_step: Callable[[int, dict[int, int]], bool | None] | None = None, n: int = 1,
+                 share_prefix: bool = False) -> list[GenerationResult]:
+        """`n` continuations of every prompt, side by side in the results (request n k + j is continuation j of prompt k, with the
+        sampling stream of that number); their prompt goes through the model once. `share_prefix`: so does whatever else the prompts of a
+        batch begin with in common."""
         from .step import StepEntry
+        if n < 1:
+            raise ValueError(f"{n} continuations of a prompt")
+        prompts = [p for p in prompts for _ in range(n)]
         options = options or SamplingOptions()
         eng = self.engine
         stop = eng.layout.stop_ids if stop_ids is None else stop_ids
         max_seqs = min(eng.cache.n_slots, max_batch or eng.cache.n_slots)
-        batches = plan_batches([len(p) for p in prompts], max_tokens, max_seqs, eng.cache.n_pages, eng.max_positions)
+        batches = plan_batches([len(p) for p in prompts], max_tokens, max_seqs, eng.cache.n_pages, eng.max_positions, n)
         results: list[GenerationResult | None] = [None] * len(prompts)
         # With an engine that keeps per-sequence state records on the device and a sampler that reads
         # them, a step's sampling takes nothing from the host: options and stop set go up once per call,
@@ -133,18 +207,23 @@ class Generator:
             self.sampler.begin(options, stop)
         for batch in batches:
             state = BatchState(batch, [prompts[i] for i in batch], max_tokens, stop, eng.max_positions)
-            seqs = {i: eng.open() for i in range(len(batch))}
             seeds = [seed + r for r in batch]               # one sampling stream per request
-            if on_device_state:
-                eng.cache.seed([seqs[i].slot for i in range(len(batch))], seeds)
             t_ev = [eng.new_event() for _ in range(3)]
+            seqs: dict = {}
             try:
                 t_ev[0].record()
                 live = state.live()
+                runs = []
+                if n > 1 or share_prefix:
+                    runs = shared_runs([s.prompt for s in state.seqs], None if share_prefix else [r // n for r in batch])
+                done = self._open(seqs, len(batch), state, runs)
+                if on_device_state:
+                    eng.cache.seed([seqs[i].slot for i in range(len(batch))], seeds)
+                entries = [StepEntry(seqs[i], state.seqs[i].prompt[done[i]:] if done[i] else state.seqs[i].prompt) for i in live]
                 if hasattr(eng, "prompt_step"):          # long batches of prompts go through in portions
-                    logits, index = eng.prompt_step([StepEntry(seqs[i], state.seqs[i].prompt) for i in live])
+                    logits, index = eng.prompt_step(entries)
                 else:
-                    logits = eng.step([StepEntry(seqs[i], state.seqs[i].prompt) for i in live])
+                    logits = eng.step(entries)
                     index = eng.last_step if on_device_state else None
                 fed = [len(state.seqs[i].prompt) for i in live]
                 step_no = 0

@@ -1,7 +1,7 @@
 """CUDA graphs of the decode step.
 
 A decode step launches a few hundred small kernels whose sizes depend only on the batch size, so
-it is captured once per (padded batch size, block-table width) and replayed: the step's index
+it is captured once per (padded batch size, block-table width, whether its sequences share pages) and replayed: the step's index
 arrays live in one static device buffer that is refreshed from pinned host memory before each
 replay. Rows added to fill the batch up to its padded size read and write a spare cache page and a
 spare state slot of their own, so they change nothing a real row sees.
@@ -24,8 +24,8 @@ def _next_pow2(n: int) -> int:
 
 
 class DecodeGraph:
-    def __init__(self, engine, batch: int, width: int):
-        from .step import StepContext
+    def __init__(self, engine, batch: int, width: int, shared: bool = False):
+        from .step import SharedStep, StepContext
         self.engine, self.batch, self.width = engine, batch, width
         n_groups = len(engine.cache.groups)
         B = batch
@@ -46,6 +46,8 @@ class DecodeGraph:
         ctx.block_tables = [v.view(B, width) for v in views[8:]]
         ctx.is_decode = True
         ctx.max_pages = width
+        if shared:                  # plans with room for any batch; the warm-up's is of spare rows alone
+            ctx.share = SharedStep(engine, [], [], [], padded=B)
         self.ctx = ctx
         self._fill_host([], [], [], [])
         self.dev.copy_(self.host)
@@ -123,6 +125,8 @@ class DecodeGraph:
                 self.dev[n:B].zero_()
         else:
             self.dev.copy_(self.host, non_blocking=True)
+        if self.ctx.share is not None:
+            self.ctx.share.refresh(slots, pos0)
         self.copied.record()
         self.graph.replay()
         from ..csrc import bindings
@@ -148,7 +152,7 @@ class DecodeGraphs:
 
     def __init__(self, engine):
         self.engine = engine
-        self.graphs: dict[tuple[int, int], DecodeGraph] = {}
+        self.graphs: dict[tuple[int, int, bool], DecodeGraph] = {}
         self.pool = torch.cuda.graph_pool_handle() if torch.cuda.is_available() else None
         self.last_index = None
         self.last_graph: DecodeGraph | None = None
@@ -156,17 +160,18 @@ class DecodeGraphs:
     def clear(self):
         self.graphs.clear()
 
-    def run(self, ids, pos0, slots, tables) -> torch.Tensor:
+    def run(self, ids, pos0, slots, tables, shared: bool = False) -> torch.Tensor:
+        """`shared`: the sequences share pages; the step is captured a second time, with attention that reads those once."""
         need = max(1, max(t.shape[1] for t in tables)) if tables else 1
         cap = -(-self.engine.max_positions // PAGE)
         width = min(max(8, _next_pow2(need)), max(cap, need))
         batch = _next_pow2(ids.shape[0] if isinstance(ids, torch.Tensor) else len(ids))
-        key = (batch, width)
+        key = (batch, width, shared)
         g = self.graphs.pop(key, None)
         if g is None:
             while len(self.graphs) >= self.MAX_GRAPHS:
                 self.graphs.pop(next(iter(self.graphs)))          # the dict is kept in order of last use
-            g = DecodeGraph(self.engine, batch, width)
+            g = DecodeGraph(self.engine, batch, width, shared)
         self.graphs[key] = g
         out = g.run(ids, pos0, slots, tables)
         self.last_graph, self.last_index = g, g.index(out.shape[0])

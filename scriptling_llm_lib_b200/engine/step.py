@@ -16,10 +16,10 @@ from itertools import chain
 import numpy as np
 import torch
 
-from ..cache import PAGE, SequenceCache, pages_for
+from ..cache import PAGE, PlanCapacity, SequenceCache, SharePlan, pages_for, share_pays
 from ..config.registry import architecture_for, architecture_name, load_config
 from ..csrc.bindings import CastKernels, KernelSet, SplitGemm
-from ..parts.base import Part
+from ..parts.base import Mixer, Part
 from ..parts.linear import linears
 from ..weights.loader import load_weights, stored_to_kept
 from .graphs import DecodeGraphs
@@ -56,6 +56,10 @@ class Sequence:
         if not self.closed:
             self.engine.cache.close(self.slot)
             self.closed = True
+
+    def fork(self, n: int = 1) -> list["Sequence"]:
+        """`n` sequences that go on from here, see `Engine.fork`."""
+        return self.engine.fork(self, n)
 
 
 def _token_ids(runs, total: int) -> np.ndarray:
@@ -105,6 +109,7 @@ class StepContext:
         self.seq_lens_host: list[int] | None = None     # rows of every sequence, known on the host (None in a replayed step)
         self.from_start = False                         # every sequence of the step starts at its position 0
         self.scratch: dict = {}                         # what parts of one kind share within a step (made by the first to ask)
+        self.share = None                               # SharedStep: the step's sequences share pages worth reading once
 
     @property
     def kernels_f32(self):
@@ -130,9 +135,66 @@ class StepContext:
         k, v = self.cache.groups[g].unit_storage(unit)
         return k, v, self.block_tables[g]
 
+    def share_plan(self, unit: int, n_heads: int, head_dim: int, v_dim: int):
+        """The plan for attention of `n_heads` query heads over the unit's pages where the step's sequences share some of them and the
+        kernel takes the widths; None: every sequence for itself."""
+        return None if self.share is None else self.share.plan(self.cache.group_of_unit[unit], n_heads, head_dim, v_dim)
+
     def unit_state(self, unit: int):
         """State tensor [n_slots, ...] of the unit; index it with `self.slots`."""
         return self.cache.state[unit]
+
+
+class SharedStep:
+    """What a step whose sequences share pages keeps for its attention layers: a plan for every cache group and head layout that asks,
+    made when the first layer does. A captured decode step's plans have room for any of its batches and are laid out again
+    (`refresh`) when slots come to hold other pages or the sequences have grown by a sixteenth."""
+
+    def __init__(self, engine: "Engine", slots, held, new, padded: int | None = None):
+        self.engine, self.padded = engine, padded
+        self.plans: dict[tuple, SharePlan | None] = {}
+        self.laid_out: dict[tuple, tuple] = {}
+        self.staging: dict[tuple, torch.Tensor] = {}
+        self.slots, self.held, self.new = slots, held, new
+
+    def plan(self, group: int, n_heads: int, head_dim: int, v_dim: int):
+        key = (group, n_heads, head_dim, v_dim)
+        if key not in self.plans:
+            need, ops = self.engine.cache.groups[group].need, self.engine.kernels.shared
+            takes = need.kind == "full" and ops.takes(head_dim, v_dim, n_heads // need.kv_heads)
+            self.plans[key] = self._build(key) if takes else None
+        return self.plans[key]
+
+    def _build(self, key, device=True):
+        group, n_heads, head_dim, v_dim = key
+        cache, B = self.engine.cache, self.padded
+        n_kv, shape = cache.groups[group].need.kv_heads, self.engine.kernels.shared.shape(head_dim, v_dim)
+        held, new, tree, n = list(self.held), list(self.new), None, 0 if B is None else B - len(self.slots)
+        table = cache.block_table(group, self.slots) if self.slots else np.zeros((0, 1), dtype=np.int32)
+        if n == 0:
+            tree = cache.share_tree(group, self.slots)
+        else:               # rows that fill the batch up: one token each on the spare page, which no one shares with them
+            table = np.concatenate([table, np.full((n, table.shape[1]), cache.n_pages, dtype=np.int32)])
+            held, new = held + [0] * n, new + [1] * n
+        capacity = None if B is None else PlanCapacity.of_decode(B, n_heads, n_kv, shape)
+        return SharePlan.build(table, held, new, n_heads, n_kv, shape, self.engine.device if device else None, capacity, tree)
+
+    def refresh(self, slots, held) -> None:
+        """Lay the plans out for these sequences, at the addresses that they have (the stream's order keeps steps apart)."""
+        self.slots, self.held, self.new = list(slots), list(held), [1] * len(slots)
+        pages = sum(h // PAGE + 1 for h in held)
+        for key, plan in self.plans.items():
+            if plan is None:
+                continue
+            was = self.laid_out.get(key)
+            if was is not None and was[:2] == (self.engine.cache.version, self.slots) and was[2] <= pages <= was[2] + max(1, was[2] // 16):
+                continue
+            host = torch.from_numpy(plan.again(self._build(key, device=False)))
+            if key not in self.staging:
+                self.staging[key] = torch.empty_like(host).pin_memory()
+            self.staging[key].copy_(host)
+            plan.dev.copy_(self.staging[key], non_blocking=True)
+            self.laid_out[key] = (self.engine.cache.version, self.slots, pages)
 
 
 class Engine:
@@ -171,6 +233,8 @@ class Engine:
         n_slots = max_seqs if max_seqs is not None else min(n_pages, 1024)
         self.cache = SequenceCache(self.model.cache_needs(), self.model.state_needs(), n_slots, n_pages, self.dtype,
                                    self.device)
+        self.cache.err_flag = self.err_flag
+        self._sharing: list[int] | None = None
         self.max_positions = min(self.layout.max_positions, n_pages * PAGE)
         self.model.prepare(self.max_positions, self.device)
         padded = 1
@@ -233,6 +297,53 @@ class Engine:
     def open(self) -> Sequence:
         return Sequence(self, self.cache.open())
 
+    def fork(self, sequence: Sequence, n: int = 1) -> list[Sequence]:
+        """`n` more sequences that hold what `sequence` holds and go on from there, each on its own. Their whole pages are the same ones, so
+        that later steps read them once for all; the last, partly filled page is copied by the step that writes to it. States of
+        fixed size are copied. CacheFull, with nothing changed, where slots are missing."""
+        if sequence.closed or sequence.engine is not self:
+            raise StepError("the sequence to fork is closed or belongs to another engine")
+        return [Sequence(self, slot) for slot in self.cache.fork(sequence.slot, n)]
+
+    def compact(self, max_tokens: int | None = None) -> int:
+        """Move the pages that sequences hold to the front of the cache, while the sequences are open; with `max_tokens`, into a cache for
+        that many tokens held at once, as `resize_cache` would make it: smaller (memory back) or larger (room for more). Returns the
+        pages copied. CacheFull or StepError, with nothing changed, where what is held does not fit."""
+        if max_tokens is None:
+            return self.cache.compact()
+        n_pages = max(1, pages_for(max_tokens))
+        longest = max((self.cache.length[s] for s in range(self.cache.n_slots) if self.cache.slots.is_held(s)), default=0)
+        if longest > n_pages * PAGE:
+            raise StepError(f"a sequence holds {longest} tokens; a cache for {max_tokens} holds at most {n_pages * PAGE} of one")
+        moved = self.cache.compact(n_pages)
+        self.decode_graphs.clear()              # they hold the old storage's addresses
+        self.max_positions = min(self.layout.max_positions, n_pages * PAGE)
+        self.model.prepare(self.max_positions, self.device)
+        return moved
+
+    def _shares(self, slots, held, new) -> bool:
+        """Whether a step of these sequences is to go by the plans of `SharedStep`: pages that it need not read again are worth the
+        partial results that reading them once leaves."""
+        cache = self.cache
+        if not cache.shares_pages or len(slots) < 2:
+            return False
+        return any(cache.groups[g].pool.n_shared and share_pays(cache.share_tree(g, slots), held, new) for g in self._share_groups())
+
+    def _share_groups(self) -> list[int]:
+        """Cache groups with layers whose attention can read shared pages once."""
+        if self._sharing is None:
+            groups, ops = set(), self.kernels.shared
+            for e in self.layout.schedule:
+                g = self.cache.group_of_unit.get(e.cache_unit)
+                if g is None or self.cache.groups[g].need.kind != "full":
+                    continue
+                for part in self.model.blocks[e.layer].parts():
+                    heads = part.shares_pages() if isinstance(part, Mixer) else None
+                    if heads is not None and ops.takes(heads[1], heads[2], heads[0] // self.cache.groups[g].need.kv_heads):
+                        groups.add(g)
+            self._sharing = sorted(groups)
+        return self._sharing
+
     def tickets(self, n: int) -> torch.Tensor:
         """Zeroed int32 counters that kernels of one stream draw tickets from and leave zero (which
         of several blocks finishes last). One buffer for the engine: its kernels run one after another.
@@ -293,7 +404,7 @@ class Engine:
         if self.use_graphs and T == B:
             slots = [e.sequence.slot for e in entries]
             tables = [self.cache.block_table(g, slots) for g in range(len(self.cache.groups))]
-            logits = self.decode_graphs.run(ids, pos0, slots, tables)
+            logits = self.decode_graphs.run(ids, pos0, slots, tables, self._shares(slots, pos0, lens))
             self.last_step = self.decode_graphs.last_index
             # the captured step's own buffer is overwritten by the next replay: the caller gets a copy
             if want_rows != list(range(B)):
@@ -393,7 +504,8 @@ class Engine:
         self.cache.reserve(growth)
         slots = [s.slot for s in sequences]
         tables = [self.cache.block_table(g, slots) for g in range(len(self.cache.groups))]
-        logits = self.decode_graphs.run(ids.contiguous(), [s.length for s in sequences], slots, tables)
+        held = [s.length for s in sequences]
+        logits = self.decode_graphs.run(ids.contiguous(), held, slots, tables, self._shares(slots, held, [1] * len(slots)))
         self.last_step = self.decode_graphs.last_index
         self.cache.advance(growth)
         return logits
@@ -445,6 +557,8 @@ class Engine:
         ctx.token_ids, ctx.tok_pos, ctx.tok_seq, ctx.seq_start, ctx.seq_pos0, ctx.slots, ctx.want_rows, ctx.seq_pos_after = views[:8]
         ctx.block_tables = [v.view(B, t.shape[1]) for v, t in zip(views[8:], tables)]
         ctx.is_decode = bool((lens_a == 1).all())
+        if self._shares(slots, pos0, lens):
+            ctx.share = SharedStep(self, slots, pos0, lens)
         ctx.seq_lens_host = [int(n) for n in lens]
         ctx.from_start = not pos0_a.any()
         ctx.max_pages = int(-(-(int((pos0_a + lens_a).max())) // PAGE))

@@ -12,9 +12,10 @@ from __future__ import annotations
 
 import os
 import threading
+from operator import index as as_int
 
 from .cache.needs import PAGE
-from .engine.generate import GenerationResult, Generator
+from .engine.generate import GenerationResult, Generator, request_pages
 from .engine.step import DTYPES, Engine
 from .sampling.sampler import Sampler, SamplingOptions
 
@@ -48,10 +49,13 @@ def unload(model_dir=None) -> None:
             del _models[key]
 
 
-def _fit_cache(eng: Engine, prompts, max_tokens, max_batch):
-    """Grow the engine's cache so the requests run in as few batches as memory allows."""
+def _fit_cache(eng: Engine, prompts, max_tokens, max_batch, n: int = 1):
+    """Grow the engine's cache so the requests run in as few batches as memory allows. `n` continuations of a prompt hold its pages once."""
     import torch
     pages = [(min(eng.layout.max_positions, len(p) + max_tokens - 1) + PAGE - 1) // PAGE for p in prompts]
+    if n > 1:
+        need = [request_pages(len(p), max_tokens, eng.layout.max_positions) for p in prompts]
+        pages = [own + (0 if j else shared) for own, shared in need for j in range(n)]
     if max_batch:
         pages = sorted(pages, reverse=True)[:max_batch]
     want_pages, want_seqs = sum(pages), len(pages)
@@ -68,7 +72,7 @@ def _fit_cache(eng: Engine, prompts, max_tokens, max_batch):
 def generate(model_dir, prompt_ids, max_tokens: int = 100, strategy: str = "greedy", *, temperature: float = 1.0,
              top_k: int = 50, top_p: float = 0.9, repeat_penalty: float = 1.15, repeat_last_n: int = 64,
              seed: int = 0, stop_ids=None, dtype: str = "bfloat16", device: str = "cuda:0", max_batch: int | None = None,
-             stats: bool = False, on_step=None):
+             stats: bool = False, on_step=None, n: int = 1, share_prefix: bool = False):
     """Generate from token ids.
 
     prompt_ids: a list of ids -> returns the list of generated ids; a list of lists (unequal
@@ -77,6 +81,11 @@ def generate(model_dir, prompt_ids, max_tokens: int = 100, strategy: str = "gree
     empty list for none) is kept in the output. `strategy` "greedy" ignores temperature and
     penalty; `temperature=0.0` means greedy. With `stats=True` returns (ids, stats) where stats
     holds prompt_tokens, generated_tokens, prefill_ms, decode_ms (lists when given a batch).
+
+    `n` > 1: that many continuations of every prompt, each with a sampling stream of its own (seed + n * prompt + continuation);
+    every prompt's list of ids becomes a list of `n` such lists, and its entries of `stats` lists of `n`. The prompt goes through the
+    model once and its pages are held and read once. `share_prefix`: the same for whatever the prompts of a batch begin with in
+    common (a system prompt, a document). Both leave the numbers as they are but for rounding.
     """
     single = len(prompt_ids) > 0 and not isinstance(prompt_ids[0], (list, tuple))
     prompts = [list(prompt_ids)] if single else [list(p) for p in prompt_ids]
@@ -86,12 +95,17 @@ def generate(model_dir, prompt_ids, max_tokens: int = 100, strategy: str = "gree
     with _models_lock:
         run_lock = _run_locks.setdefault(id(eng), threading.Lock())
     with run_lock:      # concurrent callers of one model take turns (the reference gives each a clone; here they share a cache)
-        _fit_cache(eng, prompts, max_tokens, max_batch)
-        results = Generator(eng, sampler).generate(prompts, max_tokens, options, stop_ids, seed, max_batch, on_step)
-    ids = [r.tokens for r in results]
+        n = as_int(n)
+        if n < 1:
+            raise ValueError(f"{n} continuations of a prompt")
+        _fit_cache(eng, prompts, max_tokens, max_batch, n)
+        results = Generator(eng, sampler).generate(prompts, max_tokens, options, stop_ids, seed, max_batch, on_step, n, bool(share_prefix))
+    ids, st = [r.tokens for r in results], _stats(results)
+    if n > 1:
+        by_prompt = lambda v: [v[i:i + n] for i in range(0, len(v), n)]      # noqa: E731
+        ids, st = by_prompt(ids), {k: by_prompt(v) for k, v in st.items()}
     if not stats:
         return ids[0] if single else ids
-    st = _stats(results)
     return (ids[0], {k: v[0] for k, v in st.items()}) if single else (ids, st)
 
 

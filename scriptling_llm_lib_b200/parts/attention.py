@@ -47,6 +47,8 @@ weight multiplies it, and `after_rotation` (which takes none) norms a head once 
 same sink logit for every head as a constant instead of a stored one (0: one is added to the denominator). `value_mix`:
 layers that share a `group` mix their values with those the group's first layer projected for the same token, v <- (1 - lam)
 v + lam v_first with lam a stored number, before they are cached; the first layer's values stay at hand for the step.
+Where a step's sequences share pages (they were forked from one another), a layer that sees every earlier key reads those once
+for all of them (`_attend_shared`), whatever its widths, caps and sinks, as far as that kernel takes the widths.
 With any of these, attention runs on the kernels that know keys and values of different widths, the window with kept
 positions and the sink: in bfloat16 the tcgen05 prompt kernels (widths up to 128 in multiples of 8), the mma.sync prompt and
 decode kernels (keys up to 256, values up to 128, multiples of 8), else and in 32-bit the generic ones.
@@ -304,8 +306,27 @@ class Attention(Mixer):
         path = self.out.fold_path(ctx, rows, ctx.dtype, finishing=True)
         return path is not None and (ctx.is_decode or path == "tiles")
 
+    def shares_pages(self):
+        return None if self.span else (self.n_heads, self.head_dim, self.v_dim)
+
+    def _share_plan(self, ctx, unit):
+        """The step's plan where its sequences share pages and this layer sees all of them."""
+        plan = getattr(ctx, "share_plan", None)
+        return None if self.span or plan is None else plan(unit, self.n_heads, self.head_dim, self.v_dim)
+
+    def _attend_shared(self, plan, q, ctx, kpages, vpages, block_table):
+        """The step's queries (the leading columns of `q`) over pages that are read once for all sequences that share them."""
+        attn = torch.empty((q.shape[0], self.n_heads * self.v_dim), dtype=q.dtype, device=q.device)
+        part = torch.empty((plan.part_floats(self.v_dim),), dtype=torch.float32, device=q.device)
+        ctx.kernels.shared.attn(q, attn, ctx.tok_pos, block_table, kpages, vpages, plan, part, self.scale, ctx.err_flag, softcap=self.softcap,
+                                sink=self.sink)
+        return attn
+
     def _attend(self, qkv, x, ctx, kpages, vpages, block_table, fast_decode, fusion, writes, unit=None):
         """The step's queries (the leading columns of `qkv`) over the cache -> [T, n_heads * v_dim]."""
+        plan = self._share_plan(ctx, unit)
+        if plan is not None:
+            return self._attend_shared(plan, qkv, ctx, kpages, vpages, block_table)
         attn = torch.empty((x.shape[0], self.n_heads * self.v_dim), dtype=x.dtype, device=x.device)
         plain_widths = not self.other_widths and self.head_dim in PrefillAttentionTC.HEAD_DIMS
         if not plain_widths and exact_prompt_kernel(ctx, x.dtype, self.head_dim, self.v_dim, kpages.numel()):
@@ -364,7 +385,10 @@ class Attention(Mixer):
         options = dict(softcap=self.softcap, sink=self.sink, keep=self.keep_first)
         pages = ctx.pages_seen(unit) if ctx.is_decode else 0
         gated = False
-        if ctx.is_decode and bf16 and DecodeKernels.general_takes(hd, vd):
+        plan = self._share_plan(ctx, unit)
+        if plan is not None:
+            attn = self._attend_shared(plan, q, ctx, kpages, vpages, block_table)
+        elif ctx.is_decode and bf16 and DecodeKernels.general_takes(hd, vd):
             attn = torch.empty((T, H * vd), dtype=q.dtype, device=q.device)
             fused_gate = gate if gate is not None and gate_aligned(gate) else None
             gated = fused_gate is not None
@@ -454,7 +478,7 @@ class Attention(Mixer):
         tc = ctx.kernels.tensor_core if x.dtype == torch.bfloat16 else None
         # a rotation can ride in the decode attention kernel, or in the q|k|v product of a long prompt step
         fast_decode = fast_decode and not self.other_widths
-        fusion = rotation if (fast_decode and rotation is not None and not self.own_store
+        fusion = rotation if (fast_decode and rotation is not None and not self.own_store and self._share_plan(ctx, unit) is None
                               and DecodeKernels.rotation_fusable(*rotation[1:])) else None
         fused_product = None
         if (tc is not None and writes and not fast_decode and not self.own_store and rotation is not None and x.shape[0] > tc.SKINNY_MAX_M

@@ -111,6 +111,11 @@ class Mixer(Part):
     def state_need(self) -> StateNeed | None:
         return None
 
+    def shares_pages(self) -> tuple[int, int, int] | None:
+        """(query heads, key width, value width) of a mixer that reads the pages of a step's sequences once where they share them
+        (`ctx.share_plan`); None: each sequence is read for itself."""
+        return None
+
     def forward(self, x, ctx, unit: int, writes: bool):
         raise NotImplementedError
 
