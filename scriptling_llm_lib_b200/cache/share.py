@@ -22,20 +22,26 @@ from .needs import PAGE
 
 MAX_DEPTH = 4       # levels of shared runs; what lies deeper is read by each sequence for itself
 MIN_SAVED = 4       # pages that a node must save its members to be worth another partial result for each row
-ITEM_WORDS = 8      # int32 words of an item: first token in the list, tokens, last token, kv head, first page, page end (-1: to the
-                    # last token), first row of the scratch, row of the block table
+ITEM_WORDS = 8      # int32 words of an item: first token in the list, tokens, last token (-1: of a node, all of whose keys all its tokens
+                    # see), kv head, first page, page end (-1: to the last token), first row of the scratch, row of the block table
 
 
 @dataclass(frozen=True)
 class TileShape:
     """What a kernel works on: rows (tokens x query heads of a key/value head) of a tile, blocks that stay and walk their lists.
-    `halves`: a tile of at most half the rows is worked on twice, by pages of either parity, and leaves two partial results."""
+    `halves`: a tile of at most half the rows is worked on twice, by pages of either parity, and leaves two partial results.
+    `thin_rows`: tiles of at most so many rows are thin: they stand behind the others in a block's list, each with one of its
+    `thin_warps` warps."""
     rows: int
     workers: int
     halves: bool = False
     item_pages: float = 1.0      # what an item costs beside its pages, in pages
     half_cost: float = 1.0       # what a page of a tile of at most half the rows costs, a full tile's page being 1
     min_pages: int = 2           # an item is not cut to fewer
+    thin_rows: int = 0
+    thin_warps: int = 0
+    thin_cost: float = 0.0       # what a page of a thin tile costs the block
+    thin_item: float = 0.0       # and an item
 
 
 def share_tree(table: np.ndarray, whole: np.ndarray):
@@ -115,14 +121,15 @@ class SharePlan:
     def _sizes(self):
         s, c = self.shape, self.capacity
         # (items start at a multiple of four words: they are read sixteen bytes at a time)
-        return [-(-(s.workers + 1) // 4) * 4, ITEM_WORDS * c.items, self.n_rows, self.n_rows * self.n_kv + 1, c.entries]
+        return [-(-(s.workers + 1) // 4) * 4, -(-(s.workers * s.thin_warps + 1) // 4) * 4, ITEM_WORDS * c.items, self.n_rows,
+                self.n_rows * self.n_kv + 1, c.entries]
 
     def host(self) -> np.ndarray:
-        """The buffer's words: where each block's items begin, the items, the tokens in the tree's order, where each token and
+        """The buffer's words: where each block's items begin, where each of its warps' thin items do, the items, the tokens in the tree's order, where each token and
         key/value head's entries begin, the entries (rows of the scratch)."""
         sizes, p = self._sizes(), self.parts
         out, off = np.zeros(sum(sizes), dtype=np.int32), 0
-        for n, part in zip(sizes, (p["first"], p["items"].ravel(), p["toks"], p["list_first"], p["list"])):
+        for n, part in zip(sizes, (p["first"], p["thin_first"], p["items"].ravel(), p["toks"], p["list_first"], p["list"])):
             out[off:off + len(part)] = part
             off += n
         return out
@@ -132,11 +139,15 @@ class SharePlan:
         for n in self._sizes():
             views.append(self.dev[at:at + n])
             at += n
-        self.first, self.items, self.toks, self.list_first, self.list = views
+        self.first, self.thin_first, self.items, self.toks, self.list_first, self.list = views
 
     def part_floats(self, v_dim: int) -> int:
-        """float32 elements of the scratch for values `v_dim` wide: a row's sums over the values, then its maximum and sum."""
-        return self.capacity.rows * (v_dim + 2)
+        """float32 elements of the scratch for values `v_dim` wide: the rows' sums over the values, then their maxima and sums."""
+        return self.scratch_rows * (v_dim + 2)
+
+    @property
+    def scratch_rows(self) -> int:
+        return -(-max(1, self.capacity.rows) // 32) * 32
 
     @classmethod
     def build(cls, table, held, new, n_heads: int, n_kv: int, shape: TileShape, device, capacity=None, tree=None) -> "SharePlan":
@@ -157,7 +168,9 @@ class SharePlan:
             raise ValueError(f"{rep} query heads on one key/value head; a tile has {shape.rows} rows")
         if np.any(-(-(held + new) // PAGE) > width):
             raise ValueError(f"a sequence of {int((held + new).max())} tokens does not fit {width} pages")
-        order, nodes, own = tree if tree is not None else share_tree(table, held // PAGE)
+        if tree is None or any(held[tree[0][lo:hi]].min() < PAGE * end for lo, hi, _, end in tree[1]):     # (or one that was taken back)
+            tree = share_tree(table, held // PAGE)
+        order, nodes, own = tree
         parts = _lay_out(order, nodes, own, held, new, rep, n_kv, shape)
         return cls(n_seqs, int(new.sum()), n_heads, n_kv, shape, width, parts, device, capacity)
 
@@ -172,14 +185,38 @@ class PlanCapacity:
     @classmethod
     def of_decode(cls, n_seqs: int, n_heads: int, n_kv: int, shape: TileShape) -> "PlanCapacity":
         """What any plan of one token for each of `n_seqs` sequences needs at most: every level of the tree has each token once, in
-        at most one tile more than its nodes need, and every block cuts one tile at most."""
+        at most one tile more than its nodes need, and every block, and every warp with thin tiles, cuts one tile at most."""
         rep = n_heads // n_kv
         per = max(1, shape.rows // rep)
         tiles = n_seqs + MAX_DEPTH * (n_seqs // 2 + -(-n_seqs // per))
         twice = 2 if shape.halves else 1
-        cuts = shape.workers * min(per, n_seqs)
-        entries = twice * (n_kv * n_seqs * (1 + MAX_DEPTH) + cuts)
-        return cls(n_kv * tiles + shape.workers, entries, entries * rep)
+        thin = shape.workers * shape.thin_warps
+        cuts = twice * shape.workers * min(per, n_seqs) + thin * min(shape.thin_rows // rep, n_seqs)
+        entries = twice * n_kv * n_seqs * (1 + MAX_DEPTH) + cuts
+        return cls(n_kv * tiles + shape.workers + thin, entries, entries * rep)
+
+
+def _cut(cost, pages, marks, least: int):
+    """Units that stand in a line, each as long as its cost, cut where the line is marked, but into no pieces of fewer than `least` pages:
+    (unit, first page, page end, the number of marks in front of its middle) of every piece, in the line's order."""
+    ends = np.cumsum(cost)
+    at = ends - cost
+    k0, k1 = np.searchsorted(marks, at, "right"), np.searchsorted(marks, ends - 1e-6, "left")
+    n = np.maximum(0, k1 - k0)
+    cu = np.repeat(np.arange(len(cost)), n)
+    k = np.arange(len(cu)) - np.repeat(np.cumsum(n) - n, n) + k0[cu]
+    cut = np.rint((marks[k] - at[cu]) / cost[cu] * pages[cu]).astype(np.int64) if len(cu) else cu
+    fine = (cut >= least) & (pages[cu] - cut >= least)
+    fine[1:] &= (cu[1:] != cu[:-1]) | (cut[1:] >= cut[:-1] + least)
+    cu, cut = cu[fine], cut[fine]
+    iu, begin = np.concatenate([np.arange(len(cost)), cu]), np.concatenate([np.zeros(len(cost), dtype=np.int64), cut])
+    by = np.lexsort((begin, iu))
+    iu, begin = iu[by], begin[by]
+    stop = np.append(begin[1:], 0)
+    last = np.append(iu[1:] != iu[:-1], np.ones(min(1, len(iu)), dtype=bool))
+    stop = np.where(last, pages[iu], stop[:len(iu)])
+    middle = at[iu] + cost[iu] * (begin + stop) / (2.0 * np.maximum(1, pages[iu]))
+    return iu, begin, stop, np.searchsorted(marks, middle, "right")
 
 
 def _lay_out(order, nodes, own, held, new, rep: int, n_kv: int, shape: TileShape) -> dict:
@@ -209,42 +246,39 @@ def _lay_out(order, nodes, own, held, new, rep: int, n_kv: int, shape: TileShape
     last_pos = held[seq_of_row[t_last]] + t_last - starts[seq_of_row[t_last]] if len(s) else t_last
     t_end = np.where(end[s] < 0, last_pos // PAGE + 1, end[s])
     t_pages = t_end - page[s]
-    half = (t_n * rep <= shape.rows // 2) if shape.halves else np.zeros(len(s), dtype=bool)
+    thin = t_n * rep <= shape.thin_rows
+    half = (t_n * rep <= shape.rows // 2) & ~thin if shape.halves else np.zeros(len(s), dtype=bool)
     cost = t_pages * np.where(half, shape.half_cost, 1.0) + shape.item_pages
-    # ---- a tile for every key/value head; the line of all their costs is cut into equal lengths, one for each block
-    u = np.repeat(np.arange(len(s)), n_kv)
+    cost[thin] = t_pages[thin] * shape.thin_cost + shape.thin_item
+    # ---- a tile for every key/value head, the thin ones behind the others
+    by = np.argsort(thin, kind="stable")
+    u = np.repeat(by, n_kv)
     g = np.tile(np.arange(n_kv), len(s))
-    c = cost[u]
-    at = np.cumsum(c) - c
-    total = float(c.sum())
-    per_block = max(total / shape.workers, shape.min_pages + shape.item_pages)
-    k0 = np.floor(at / per_block).astype(np.int64)
-    k1 = np.floor((at + c - 1e-6) / per_block).astype(np.int64)
-    n_cut = k1 - k0
-    cu = np.repeat(np.arange(len(u)), n_cut)
-    k = np.arange(len(cu)) - np.repeat(np.cumsum(n_cut) - n_cut, n_cut) + k0[cu] + 1
-    pages_u = t_pages[u]
-    cut = np.rint((k * per_block - at[cu]) / c[cu] * pages_u[cu]).astype(np.int64)
-    fine = (cut >= shape.min_pages) & (pages_u[cu] - cut >= shape.min_pages)
-    cu, cut = cu[fine], cut[fine]
-    # items: every unit from its start and from each of its cuts on
-    iu = np.concatenate([np.arange(len(u)), cu])
-    begin = np.concatenate([np.zeros(len(u), dtype=np.int64), cut])
-    by = np.lexsort((begin, iu))
-    iu, begin = iu[by], begin[by]
-    last = np.append(iu[1:] != iu[:-1], True) if len(iu) else np.zeros(0, dtype=bool)
-    stop = np.where(last, pages_u[iu], np.append(begin[1:], 0))
-    middle = at[iu] + c[iu] * (begin + stop) / (2.0 * np.maximum(1, pages_u[iu]))
-    worker = np.minimum(shape.workers - 1, (middle / per_block).astype(np.int64))
+    c, pages_u = cost[u], t_pages[u]
+    n_thick = n_kv * int((~thin).sum())
+    share = max(float(c.sum()) / shape.workers, shape.min_pages + shape.item_pages)      # of a block
+    # the line of the tiles' costs is cut into equal lengths, one for each block; what is left of each block's share is the warps'
+    i1, b1, e1, w1 = _cut(c[:n_thick], pages_u[:n_thick], share * np.arange(1, shape.workers), shape.min_pages)
+    if n_thick < len(u):
+        load = np.bincount(w1, weights=c[i1] * (e1 - b1) / np.maximum(1, pages_u[i1]), minlength=shape.workers)
+        left = np.repeat(np.maximum(share - load, 0.02 * share) / shape.thin_warps, shape.thin_warps)
+        line = np.cumsum(left)
+        i2, b2, e2, w2 = _cut(c[n_thick:], pages_u[n_thick:], line[:-1] * (float(c[n_thick:].sum()) / line[-1]), 1)
+    else:
+        i2 = b2 = e2 = w2 = np.zeros(0, dtype=np.int64)
+    iu, begin, stop = np.concatenate([i1, i2 + n_thick]), np.concatenate([b1, b2]), np.concatenate([e1, e2])
+    last = stop == pages_u[iu]
     tile = u[iu]
     rows = t_n[tile] * rep * np.where(half[tile], 2, 1)
     part0 = np.cumsum(rows) - rows
     items = np.empty((len(iu), ITEM_WORDS), dtype=np.int32)
-    items[:, 0], items[:, 1], items[:, 2], items[:, 3] = t_off[tile], t_n[tile], t_last[tile], g[iu]
+    leaf = end[s[tile]] < 0
+    items[:, 0], items[:, 1], items[:, 2], items[:, 3] = t_off[tile], t_n[tile], np.where(leaf, t_last[tile], -1), g[iu]
     items[:, 4] = page[s[tile]] + begin
-    items[:, 5] = np.where(last & (end[s[tile]] < 0), -1, page[s[tile]] + stop)
+    items[:, 5] = np.where(last & leaf, -1, page[s[tile]] + stop)
     items[:, 6], items[:, 7] = part0, seq[s[tile]]
-    first = np.searchsorted(worker, np.arange(shape.workers + 1))
+    first = np.searchsorted(w1, np.arange(shape.workers + 1))
+    thin_first = len(i1) + np.searchsorted(w2, np.arange(shape.workers * shape.thin_warps + 1))
     # ---- which rows of the scratch belong to a token and key/value head
     n_i = t_n[tile]
     it = np.repeat(np.arange(len(iu)), n_i)
@@ -258,4 +292,4 @@ def _lay_out(order, nodes, own, held, new, rep: int, n_kv: int, shape: TileShape
     by = np.argsort(key, kind="stable")
     list_first = np.zeros(T * n_kv + 1, dtype=np.int64)
     np.cumsum(np.bincount(key, minlength=T * n_kv), out=list_first[1:])
-    return {"first": first, "items": items, "toks": toks, "list_first": list_first, "list": entry[by], "part_rows": int(rows.sum())}
+    return {"first": first, "thin_first": thin_first, "items": items, "toks": toks, "list_first": list_first, "list": entry[by], "part_rows": int(rows.sum())}

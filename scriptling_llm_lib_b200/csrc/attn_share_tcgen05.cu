@@ -9,6 +9,11 @@
 // in turn and leave two partial results: the chain of a page (scores, maximum, weights, product with the values), which bounds a tile of
 // few rows, then runs twice at a time. Both halves go through the one ring; a half that does not use a page gives it back as it passes.
 //
+// Tiles of at most 16 rows (one token of a sequence's own pages, as a rule) are thin: 128 rows of tensor memory would be filled for a few.
+// They come behind the others, when the ring and its roles are done: each warp has its own list, fetches keys and values by TMA into
+// two or three buffers of its own and computes with mma.sync (16 rows fill one tile), so that six or eight chains run side by side and
+// memory is what bounds them. A plan gives every block its share of either kind.
+//
 // Rows of a tile belong to several sequences and stand anywhere in the step, so a warp gathers them (16 bytes a lane, asynchronously,
 // into the 128-byte swizzle) where keys and values come by TMA, a page and head at a time. S = Q K^T (128 x 64) and O += P V as
 // in attn_prefill_tcgen05.cu: thread = row = tensor-memory lane, P back into tensor memory as bfloat16 pairs (the weights' only
@@ -20,6 +25,8 @@
 #define FS_THREADS 384       // warp 0: TMA, warps 1-2: the products of either half, warp 3: queries, warps 4-7 and 8-11: softmax of either half
 #define FS_ROWS 128          // rows of a half
 #define FS_BK SLLM_PAGE
+#define FS_CACHED 64         // items that a block keeps decoded in shared memory
+#define FS_THIN 16           // rows of a thin tile
 
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
@@ -28,6 +35,242 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
 // 16 bytes from global to shared memory, or 16 zero bytes
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool copy) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(copy ? 16 : 0) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// warps with thin tiles, and the buffers (a page of keys or of values) that each has
+template <int KD, int VD>
+__host__ __device__ constexpr int fs_thin_warps() { return KD <= 64 && VD <= 64 ? 8 : 6; }
+template <int KD, int VD>
+__host__ __device__ constexpr int fs_thin_bufs() { return KD <= 64 && VD <= 64 ? 3 : 2; }
+
+// One warp's thin items [i0, i1): a page's keys, then its values, into the buffer that comes round, fetched as far ahead as there are
+// buffers (across items: a cursor walks the list in front of the work). Lane (r = lane / 4, c = lane % 4) has rows r and r + 8 of the
+// tile; of the scores keys 8 n + 2 c and + 1, of the output dims 8 n + 2 c and + 1.
+template <int KD, int VD>
+__device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensorMap* map_v, const ShareArgs& p, int i0, int i1, uint8_t* buf,
+                                        uint32_t bar, volatile int* abort) {
+  constexpr uint32_t K_BYTES = FS_BK * KD * 2, V_BYTES = FS_BK * VD * 2, BUF = K_BYTES > V_BYTES ? K_BYTES : V_BYTES, KA = FS_BK * 128;
+  constexpr int NK = KD / 64, NV = VD / 64, BUFS = fs_thin_bufs<KD, VD>();
+  const int lane = threadIdx.x & 31, rep = p.H / p.G, r0 = lane >> 2, c2 = 2 * (lane & 3);
+  const uint32_t sB = smem_u32(buf);
+  const float sc = p.scale * FT_LOG2E;
+  if (i0 >= i1) return;
+
+  // ---- the cursor: what is fetched next
+  int fi = i0, ft = 0, fbase = 0, ids = 0, fetched = 0, taken = 0;
+  ShareItem f = share_item(p, fi);
+  ft = f.p0;
+  auto settle = [&]() {               // to an item that has pages left; its next 32 page ids, one a lane
+    while (ft >= f.p1 && ++fi < i1) {
+      f = share_item(p, fi);
+      ft = f.p0;
+    }
+    if (fi < i1) {
+      fbase = ft;
+      ids = ft + lane < f.p1 ? share_page(p, p.block_table + (size_t)f.seq * p.max_pages, ft + lane) : 0;
+    }
+  };
+  settle();
+  auto fetch = [&]() {                // one buffer: a page's keys if `fetched` is even, else its values
+    if (fi >= i1) return;
+    const int page = __shfl_sync(0xffffffffu, ids, ft - fbase), b = fetched % BUFS;
+    if (lane == 0) {
+      const int at = page < 0 ? p.n_pages : page;
+      const uint32_t to = sB + b * BUF, on = bar + 8 * b;
+      if (fetched & 1) {
+        mbar_expect_tx(on, V_BYTES);
+#pragma unroll
+        for (int a = 0; a < NV; a++) tma_load_3d(to + a * KA, map_v, 64 * a, f.g * FS_BK, at, on);
+      } else {
+        mbar_expect_tx(on, K_BYTES);
+#pragma unroll
+        for (int a = 0; a < NK; a++) tma_load_3d(to + a * KA, map_k, 64 * a, f.g * FS_BK, at, on);
+      }
+    }
+    if ((fetched & 1) && (++ft >= f.p1 || ft - fbase == 32)) settle();
+    fetched++;
+  };
+  for (int b = 0; b < BUFS; b++) fetch();
+
+  bool ok = true;
+  for (int i = i0; ok && i < i1; i++) {
+    const ShareItem it = share_item(p, i);
+    const int n_rows = it.n_tok * rep, see0 = share_sees(it, r0, rep), see1 = share_sees(it, r0 + 8, rep);
+    const bf16* q0 = (const bf16*)p.q + (see0 < 0 ? 0 : (size_t)p.toks[it.tok0 + r0 / rep] * p.q_ld + (size_t)(it.g * rep + r0 % rep) * p.hd);
+    const bf16* q1 = (const bf16*)p.q + (see1 < 0 ? 0 : (size_t)p.toks[it.tok0 + (r0 + 8) / rep] * p.q_ld + (size_t)(it.g * rep + (r0 + 8) % rep) * p.hd);
+    uint32_t q[KD / 16][4];
+#pragma unroll
+    for (int k = 0; k < KD / 16; k++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int d = 16 * k + c2 + (e >> 1) * 8;
+        q[k][e] = d < p.hd && ((e & 1) ? see1 : see0) >= 0 ? *(const uint32_t*)(((e & 1) ? q1 : q0) + d) : 0u;
+      }
+    float o[VD / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+#pragma unroll
+    for (int n = 0; n < VD / 8; n++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[n][e] = 0.f;
+    for (int t = it.p0; t < it.p1; t++) {
+      float s[8][4];
+#pragma unroll
+      for (int n = 0; n < 8; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[n][e] = 0.f;
+      {
+        const int b = taken % BUFS;
+        ok = mbar_wait(bar + 8 * b, (taken / BUFS) & 1, abort);
+        if (!ok) break;
+        const uint32_t from = sB + b * BUF, key = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
+#pragma unroll
+        for (int k = 0; k < KD / 16; k++) {
+          if (16 * k >= p.hd) break;
+#pragma unroll
+          for (int n = 0; n < 4; n++) {
+            uint32_t r[4];
+            const uint32_t row = 16 * n + key, c = (2 * k + ch) & 7;
+            ldmatrix4(from + (k >> 2) * KA + row * 128 + ((c ^ (row & 7)) << 4), r);
+            mma16816(s[2 * n], q[k], r[0], r[1]);
+            mma16816(s[2 * n + 1], q[k], r[2], r[3]);
+          }
+        }
+        taken++;
+        __syncwarp();
+        fetch();
+      }
+      if (p.softcap > 0.f) {
+        const float cap_out = p.softcap / p.scale, cap_in = p.scale / p.softcap;
+#pragma unroll
+        for (int n = 0; n < 8; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[n][e] = __uint_as_float(ft_cap(__float_as_uint(s[n][e]), cap_out, cap_in));
+      }
+      if (t * FS_BK + FS_BK - 1 > it.last - (it.n_tok - 1)) {      // (rows past the tile's end see nothing here, zeros elsewhere)
+#pragma unroll
+        for (int n = 0; n < 8; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (t * FS_BK + 8 * n + c2 + (e & 1) > ((e >> 1) ? see1 : see0)) s[n][e] = -INFINITY;
+      }
+      float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+      for (int n = 0; n < 8; n++) {
+        x0 = ft_max3(x0, s[n][0], s[n][1]);
+        x1 = ft_max3(x1, s[n][2], s[n][3]);
+      }
+#pragma unroll
+      for (int d = 1; d < 4; d <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
+      }
+      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
+        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1), f0 = m0 == -INFINITY ? 0.f : ft_ex2((m0 - n0) * sc), f1 = m1 == -INFINITY ? 0.f : ft_ex2((m1 - n1) * sc);
+        m0 = n0;
+        m1 = n1;
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int n = 0; n < VD / 8; n++) {
+          o[n][0] *= f0;
+          o[n][1] *= f0;
+          o[n][2] *= f1;
+          o[n][3] *= f1;
+        }
+      }
+      const float a0 = m0 == -INFINITY ? 0.f : -m0 * sc, a1 = m1 == -INFINITY ? 0.f : -m1 * sc;
+      uint32_t w[4][4];                // weights of 16 keys: the first operand of the product with their values
+#pragma unroll
+      for (int n = 0; n < 8; n++) {
+        const float e0 = ft_ex2(fmaf(s[n][0], sc, a0)), e1 = ft_ex2(fmaf(s[n][1], sc, a0)), e2 = ft_ex2(fmaf(s[n][2], sc, a1)), e3 = ft_ex2(fmaf(s[n][3], sc, a1));
+        l0 += e0 + e1;
+        l1 += e2 + e3;
+        const __nv_bfloat162 u = __floats2bfloat162_rn(e0, e1), v = __floats2bfloat162_rn(e2, e3);
+        w[n >> 1][2 * (n & 1)] = *(const uint32_t*)&u;
+        w[n >> 1][2 * (n & 1) + 1] = *(const uint32_t*)&v;
+      }
+      {
+        const int b = taken % BUFS;
+        ok = mbar_wait(bar + 8 * b, (taken / BUFS) & 1, abort);
+        if (!ok) break;
+        const uint32_t from = sB + b * BUF;
+        const int n_valid = it.last + 1 - t * FS_BK;
+        if (n_valid < FS_BK) {           // behind the last token: weights are zero, but 0 * NaN is NaN
+          for (int e = lane; e < (FS_BK - n_valid) * 8 * NV; e += 32) {
+            const int blk = e / ((FS_BK - n_valid) * 8), e1 = e % ((FS_BK - n_valid) * 8);
+            *(uint4*)(buf + b * BUF + blk * KA + (n_valid + e1 / 8) * 128 + (e1 % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        const uint32_t key = (lane & 7) + (((lane >> 3) & 1) << 3), ch = lane >> 4;
+#pragma unroll
+        for (int n = 0; n < VD / 16; n++) {
+          if (16 * n >= p.vd) break;
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            uint32_t r[4];
+            const uint32_t row = 16 * k + key, c = (2 * n + ch) & 7;
+            ldmatrix4_trans(from + (n >> 2) * KA + row * 128 + ((c ^ (row & 7)) << 4), r);
+            mma16816(o[2 * n], w[k], r[0], r[1]);
+            mma16816(o[2 * n + 1], w[k], r[2], r[3]);
+          }
+        }
+        taken++;
+        __syncwarp();
+        fetch();
+      }
+    }
+    if (!ok) break;
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, d);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, d);
+    }
+    float any0 = 0.f, any1 = 0.f;                   // not 0: something is not finite
+#pragma unroll
+    for (int n = 0; n < VD / 8; n++) {
+      any0 = fmaf(o[n][0], 0.f, fmaf(o[n][1], 0.f, any0));
+      any1 = fmaf(o[n][2], 0.f, fmaf(o[n][3], 0.f, any1));
+    }
+    const bool bad0 = any0 != 0.f && l0 < INFINITY, bad1 = any1 != 0.f && l1 < INFINITY;
+    float* ml = p.part + (size_t)p.part_rows * p.vd;
+#pragma unroll
+    for (int half = 0; half < 2; half++) {
+      const int r = r0 + 8 * half;
+      if (r >= n_rows) continue;
+      const size_t at = (size_t)it.part0 + r;
+      if (half ? bad1 : bad0) {
+#pragma unroll 1
+        for (int d = c2; d < p.vd; d += 8) {
+          const float4 v = share_sum_by_key(p, it, half ? q1 : q0, half ? see1 : see0, (half ? m1 : m0) * sc, d & ~3, it.p0, 1);
+          *(float2*)(p.part + share_at(at, d & ~3, p.vd) + (d & 2)) = (d & 2) ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < VD / 8; n++)
+          if (8 * n < p.vd)
+            *(float2*)(p.part + share_at(at, (8 * n + c2) & ~3, p.vd) + (c2 & 2)) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+      }
+      if ((lane & 3) == 0) *(float2*)(ml + 2 * at) = make_float2((half ? m1 : m0) * sc, half ? l1 : l0);
+    }
+    __syncwarp();
+  }
+  if (!ok || *abort) {                // let the copies that are under way land before the block leaves
+    volatile int never = 0;
+    for (int j = taken; j < fetched; j++) mbar_wait(bar + 8 * (j % BUFS), (j / BUFS) & 1, &never);
+  }
 }
 
 // Keys of up to KD and values of up to VD dims (64 or 128 either): narrower ones are filled up with zeros on the chip.
@@ -42,6 +285,8 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   // whose O takes 128-255, have one S 0-63 and P0 64-95, P1 96-127
   constexpr int NBUF = VD > 64 ? 1 : 2;
   constexpr uint32_t P_COL0 = VD > 64 ? 64 : 192, P_STEP = 32, SUB_COLS = 256;
+  constexpr int THIN_BUF = K_BYTES > V_BYTES ? K_BYTES : V_BYTES, THIN_BUFS = fs_thin_bufs<KD, VD>(), THIN_WARPS = fs_thin_warps<KD, VD>();
+  static_assert(THIN_WARPS * THIN_BUFS * THIN_BUF <= 2 * Q_BYTES + STAGES * (K_BYTES + V_BYTES), "the thin tiles' buffers take the ring's place");
   static_assert(STAGES >= 4, "a half that takes every other page has its next page's scores issued ahead");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -54,7 +299,9 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   constexpr uint32_t SUB_BARS = 64, B_SEMPTY = 16, B_PFULL = 32, B_OFULL = 48;
   uint32_t* tmem_slot = (uint32_t*)(bars + 4 + 2 * STAGES + 16);
   volatile int* abort = (volatile int*)(tmem_slot + 1);
-  if ((uint8_t*)(abort + 1) > smem_raw + smem_bytes) {      // the 1 KB alignment took more than the launch left room for
+  ShareItem* cached = (ShareItem*)(bars + 4 + 2 * STAGES + 16 + 2 + THIN_WARPS * THIN_BUFS);
+  const uint32_t b_thin = smem_u32(bars + 4 + 2 * STAGES + 16 + 2);     // a barrier for every thin buffer
+  if ((uint8_t*)(cached + FS_CACHED) > smem_raw + smem_bytes) {      // the 1 KB alignment took more than the launch left room for
     if (threadIdx.x == 0) atomicExch(p.err, 3);
     return;
   }
@@ -76,6 +323,7 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         mbar_init(b_sub + SUB_BARS * x + B_PFULL + 8 * a, 4);
         mbar_init(b_sub + SUB_BARS * x + B_OFULL + 8 * a, 1);
       }
+    for (int a = 0; a < THIN_WARPS * THIN_BUFS; a++) mbar_init(b_thin + 8 * a, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -94,30 +342,34 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   // Every role walks the same items and counts by itself the pages fetched (JU), the pages its half has taken (J) and the query
   // buffers used (Q: one by a tile of at most 128 rows, two by a larger one); a barrier's phase follows from those counts.
   const int rep = p.H / p.G, i0 = p.first[blockIdx.x], i1 = p.first[blockIdx.x + 1];
+  if (i1 > i0) {
+    if (threadIdx.x < min(FS_CACHED, i1 - i0)) cached[threadIdx.x] = share_item(p, i0 + threadIdx.x);
+    __syncthreads();
+  }
+  auto item = [&](int i) -> ShareItem { return i - i0 < FS_CACHED ? cached[i - i0] : share_item(p, i); };
   if (warp == 0) {
+    const bool one = elect_one();
     int JU = 0;
     bool ok = true;
     for (int i = i0; ok && i < i1; i++) {
-      const ShareItem it = share_item(p, i);
+      const ShareItem it = item(i);
       const int* row = p.block_table + (size_t)it.seq * p.max_pages;
       for (int t0 = it.p0; ok && t0 < it.p1; t0 += 32) {
         // (a page that is none is fetched past the storage's end: zeros)
         const int mine = t0 + lane < it.p1 ? share_page(p, row, t0 + lane) : 0, n = min(32, it.p1 - t0);
         for (int j = 0; j < n; j++) {
           const int page = __shfl_sync(0xffffffffu, mine, j), s = JU % STAGES;
-          if (lane == 0) {
-            ok = mbar_wait(b_kvempty + 8 * s, ((JU / STAGES) & 1) ^ 1, abort);
-            if (ok) {
-              const int at = page < 0 ? p.n_pages : page;
-              mbar_expect_tx(b_kvfull + 8 * s, K_BYTES + V_BYTES);
-#pragma unroll
-              for (int a = 0; a < NK; a++) tma_load_3d(sK + s * K_BYTES + a * KA, &map_k, 64 * a, it.g * FS_BK, at, b_kvfull + 8 * s);
-#pragma unroll
-              for (int a = 0; a < NV; a++) tma_load_3d(sV + s * V_BYTES + a * KA, &map_v, 64 * a, it.g * FS_BK, at, b_kvfull + 8 * s);
-            }
-          }
-          ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+          ok = mbar_wait(b_kvempty + 8 * s, ((JU / STAGES) & 1) ^ 1, abort);      // (the whole warp: lanes that part here stay apart)
           if (!ok) break;
+          if (one) {
+            const int at = page < 0 ? p.n_pages : page;
+            mbar_expect_tx(b_kvfull + 8 * s, K_BYTES + V_BYTES);
+#pragma unroll
+            for (int a = 0; a < NK; a++) tma_load_3d(sK + s * K_BYTES + a * KA, &map_k, 64 * a, it.g * FS_BK, at, b_kvfull + 8 * s);
+#pragma unroll
+            for (int a = 0; a < NV; a++) tma_load_3d(sV + s * V_BYTES + a * KA, &map_v, 64 * a, it.g * FS_BK, at, b_kvfull + 8 * s);
+          }
+          __syncwarp();
           JU++;
         }
       }
@@ -132,21 +384,31 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     int Q = 0;
     bool ok = true;
     for (int i = i0; ok && i < i1; i++) {
-      const ShareItem it = share_item(p, i);
+      const ShareItem it = item(i);
       const int n_rows = it.n_tok * rep;
       for (int b0 = 0; ok && b0 < n_rows; b0 += FS_ROWS, Q++) {
         const int b = Q & 1;
         // the products that read what the buffer held are done
-        if (lane == 0) ok = mbar_wait(b_qempty + 8 * b, ((Q >> 1) & 1) ^ 1, abort);
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        ok = mbar_wait(b_qempty + 8 * b, ((Q >> 1) & 1) ^ 1, abort);
         if (!ok) break;
-        const int c = lane % VECS;
-        if (c < k_used) {
-#pragma unroll 4
-          for (int r = lane / VECS; r < min(FS_ROWS, n_rows - b0); r += 32 / VECS) {
-            const int rho = b0 + r, tok = p.toks[it.tok0 + rho / rep];
-            cp_async16(sQ + b * Q_BYTES + (c >> 3) * QA + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                       (const bf16*)p.q + (size_t)tok * p.q_ld + (size_t)(it.g * rep + rho % rep) * p.hd + (c < k_vecs ? 8 * c : 0), c < k_vecs);
+        __syncwarp();
+        // a lane finds four rows; then 32 / VECS rows go together, a lane to a vector
+        const int c = lane % VECS, n = min(FS_ROWS, n_rows - b0);
+        unsigned long long row[FS_ROWS / 32];
+#pragma unroll
+        for (int k = 0; k < FS_ROWS / 32; k++) {
+          const int rho = min(b0 + 32 * k + lane, n_rows - 1);
+          row[k] = (unsigned long long)((const bf16*)p.q + (size_t)p.toks[it.tok0 + rho / rep] * p.q_ld + (size_t)(it.g * rep + rho % rep) * p.hd);
+        }
+#pragma unroll
+        for (int k = 0; k < FS_ROWS / 32; k++) {
+          if (32 * k >= n) break;
+#pragma unroll
+          for (int e = 0; e < VECS; e++) {
+            const int r = 32 * k + e * (32 / VECS) + lane / VECS;
+            const char* from = (const char*)__shfl_sync(0xffffffffu, row[k], r & 31);
+            if (r < n && c < k_used)
+              cp_async16(sQ + b * Q_BYTES + (c >> 3) * QA + r * 128 + (((c & 7) ^ (r & 7)) << 4), from + (c < k_vecs ? 16 * c : 0), c < k_vecs);
           }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -165,18 +427,12 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     int JU0 = 0, J0 = 0, Q = 0;
     bool ok = true;
     for (int i = i0; ok && i < i1; i++) {
-      const ShareItem it = share_item(p, i);
+      const ShareItem it = item(i);
       const bool pair = it.n_tok * rep > FS_ROWS;
       const int n = it.p1 - it.p0, step = pair ? 1 : 2, u0 = pair ? 0 : x, n_mine = n > u0 ? (n - u0 + step - 1) / step : 0;
       const int mine = pair ? Q + x : Q, b = mine & 1;
       ok = mbar_wait(b_qfull + 8 * b, (mine >> 1) & 1, abort);
-      if (ok && pair) {                     // the other half's buffer: not read, given back
-        const int other = Q + 1 - x;
-        ok = mbar_wait(b_qfull + 8 * (other & 1), (other >> 1) & 1, abort);
-        if (ok && one) mbar_arrive(b_qempty + 8 * (other & 1));
-      }
       if (!ok) break;
-      Q += pair ? 2 : 1;
       if (n_mine <= 0 && one) mbar_arrive(b_qempty + 8 * b);
       auto issue_s = [&](int j) -> bool {
         const int JUg = JU0 + u0 + j * step, s = JUg % STAGES, Jg = J0 + j, sb = Jg % NBUF;
@@ -223,6 +479,12 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         }
         j++;
       }
+      if (ok && pair) {                     // the other half's buffer: not read, given back
+        const int other = Q + 1 - x;
+        ok = mbar_wait(b_qfull + 8 * (other & 1), (other >> 1) & 1, abort);
+        if (ok && one) mbar_arrive(b_qempty + 8 * (other & 1));
+      }
+      Q += pair ? 2 : 1;
       JU0 += max(0, n);
       J0 += n_mine;
     }
@@ -237,13 +499,13 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     int JU0 = 0, J0 = 0;
     bool ok = true;
     for (int i = i0; ok && i < i1; i++) {
-      const ShareItem it = share_item(p, i);
+      const ShareItem it = item(i);
       const int n_rows = it.n_tok * rep;
       const bool pair = n_rows > FS_ROWS;
       const int n = it.p1 - it.p0, step = pair ? 1 : 2, u0 = pair ? 0 : x, n_mine = n > u0 ? (n - u0 + step - 1) / step : 0;
       const int rho = pair ? x * FS_ROWS + r : r;                       // row of the tile
       const bool warp_has_rows = rho - lane < n_rows, has_row = rho < n_rows;
-      const int tok = has_row ? p.toks[it.tok0 + rho / rep] : 0, qpos = has_row ? p.tok_pos[tok] : -1;
+      const int qpos = share_sees(it, rho, rep);
       float m_ref = -INFINITY, l = 0.f;              // reference maximum (raw score units) and sum relative to it
 #pragma unroll 1
       for (int j = 0; j < n_mine && ok; j++) {
@@ -354,16 +616,16 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             for (int k = 0; k < 32; k++) any = fmaf(__uint_as_float(v[k]), 0.f, any);
             if (has_row) {
               if (any != 0.f && l < INFINITY) {
-                const bf16* qr = (const bf16*)p.q + (size_t)tok * p.q_ld + (size_t)(it.g * rep + rho % rep) * p.hd;
+                const bf16* qr = (const bf16*)p.q + (size_t)p.toks[it.tok0 + rho / rep] * p.q_ld + (size_t)(it.g * rep + rho % rep) * p.hd;
 #pragma unroll 1
                 for (int c = 0; c < 32 && c0 + c < p.vd; c += 4)
-                  *(float4*)(p.part + at * p.vd + c0 + c) = share_sum_by_key(p, it, qr, qpos, m, c0 + c, it.p0 + u0, step);
+                  *(float4*)(p.part + share_at(at, c0 + c, p.vd)) = share_sum_by_key(p, it, qr, qpos, m, c0 + c, it.p0 + u0, step);
               } else {
 #pragma unroll
                 for (int c = 0; c < 32; c += 4)
                   if (c0 + c < p.vd)
-                    *(float4*)(p.part + at * p.vd + c0 + c) = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]), __uint_as_float(v[c + 2]),
-                                                                          __uint_as_float(v[c + 3]));
+                    *(float4*)(p.part + share_at(at, c0 + c, p.vd)) = make_float4(__uint_as_float(v[c]), __uint_as_float(v[c + 1]),
+                                                                                  __uint_as_float(v[c + 2]), __uint_as_float(v[c + 3]));
               }
             }
             __syncwarp();
@@ -379,8 +641,12 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (warp < THIN_WARPS && !*abort) {
+    const int w = blockIdx.x * THIN_WARPS + warp;
+    fs_thin<KD, VD>(&map_k, &map_v, p, p.thin_first[w], p.thin_first[w + 1], smem + warp * THIN_BUFS * THIN_BUF, b_thin + 8 * warp * THIN_BUFS, abort);
+  }
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
-  if (threadIdx.x == 0 && *abort) atomicExch(p.err, 2);
+  if (lane == 0 && *abort) atomicExch(p.err, 2);
 }
 
 // pages [n_pages][G * 64][width] bfloat16; a box is 64 columns of one head's 64 positions, 128-byte swizzle, zero fill
@@ -399,32 +665,36 @@ static int fs_make_map(CUtensorMap* map, const void* base, long long n_pages, in
 template <int KD, int VD, int STAGES>
 static int fs_launch(const CUtensorMap& mk, const CUtensorMap& mv, const ShareArgs& a, int workers, cudaStream_t stream) {
   // what the kernel lays out after aligning to 1 KB; one block on an SM
-  constexpr size_t need = 2 * FS_ROWS * KD * 2 + STAGES * FS_BK * (KD + VD) * 2 + 512;
-  constexpr size_t smem = need + 1024;
-  static_assert(smem <= 232448, "the block of this head width does not fit an SM");
+  constexpr size_t need = 2 * FS_ROWS * KD * 2 + STAGES * FS_BK * (KD + VD) * 2 + (4 + 2 * STAGES + 16 + 2 + fs_thin_warps<KD, VD>() * fs_thin_bufs<KD, VD>()) * 8 +
+                          FS_CACHED * sizeof(ShareItem);
+  constexpr size_t room = 232448;
+  constexpr size_t smem = need + 1024 <= room ? need + 1024 : room;     // the slack for the alignment, as far as it fits
+  static_assert(need + 512 <= smem, "the block of this head width does not fit an SM");
   static SllmPerDevice allowed;
   const cudaError_t e = sllm_allow_smem(allowed, attn_share_kernel<KD, VD, STAGES>, smem);
   if (e != cudaSuccess) return (int)e;
   return (int)sllm_launch(attn_share_kernel<KD, VD, STAGES>, dim3(workers), dim3(FS_THREADS), smem, stream, mk, mv, a, (uint32_t)smem);
 }
 
-// first [workers + 1], items [.][8], toks [T]: a plan's for tiles of 256 rows in halves; part: part_rows * (vd + 2) floats.
+// first [workers + 1], thin_first [workers * thin_warps + 1], items [.][8], toks [T]: a plan's for tiles of 256 rows in halves, with thin
+// ones of at most FS_THIN rows; part: part_rows * (vd + 2) floats.
 SLLM_EXPORT int sllm_share_attn_tc_bf16(const void* q, int q_ld, const int* tok_pos, const int* block_table, int max_pages, const void* kpages,
-                                        const void* vpages, long long n_pages, const int* first, const int* items, const int* toks,
-                                        int workers, float* part, long long part_rows, int H, int G, int hd, int vd, float scale, float softcap,
+                                        const void* vpages, long long n_pages, const int* first, const int* thin_first, const int* items,
+                                        const int* toks, int workers, int thin_warps, float* part, long long part_rows, int H, int G, int hd, int vd, float scale, float softcap,
                                         int* err, cudaStream_t stream) {
   if (workers <= 0) return 0;
   if (hd < 8 || hd > 128 || hd % 8 || vd < 8 || vd > 128 || vd % 8 || G < 1 || H < 1 || H % G != 0 || H / G > 2 * FS_ROWS || q_ld < H * hd || (q_ld & 7) ||
-      n_pages < 1 || n_pages > 0x7fffffffLL || (long long)G * FS_BK > 0x7fffffffLL || part_rows < 1 || max_pages < 1 ||
+      n_pages < 1 || n_pages > 0x7fffffffLL || (long long)G * FS_BK > 0x7fffffffLL || part_rows < 1 || part_rows % 32 || max_pages < 1 ||
       ((uintptr_t)q & 15) || ((uintptr_t)kpages & 15) || ((uintptr_t)vpages & 15) || ((uintptr_t)part & 15) || ((uintptr_t)items & 15))
     return SLLM_ERR_ARG;
-  ShareArgs a{q, q_ld, tok_pos, block_table, max_pages, kpages, vpages, (int)n_pages, first, items, toks, part, part_rows, H, G, hd, vd, scale,
+  ShareArgs a{q, q_ld, tok_pos, block_table, max_pages, kpages, vpages, (int)n_pages, first, thin_first, items, toks, part, part_rows, H, G, hd, vd, scale,
               softcap, err};
   CUtensorMap mk, mv;
   int rc = fs_make_map(&mk, kpages, n_pages, G, hd);
   if (rc) return rc;
   rc = fs_make_map(&mv, vpages, n_pages, G, vd);
   if (rc) return rc;
+  if (thin_warps != (hd <= 64 && vd <= 64 ? fs_thin_warps<64, 64>() : fs_thin_warps<128, 128>())) return SLLM_ERR_ARG;
   if (vd <= 64) {
     if (hd <= 64) return fs_launch<64, 64, 10>(mk, mv, a, workers, stream);
     return fs_launch<128, 64, 6>(mk, mv, a, workers, stream);

@@ -1743,7 +1743,9 @@ class SharedAttention:
         if sm_count is None:
             sm_count = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
         if self.dtype == torch.bfloat16 and all(w % 8 == 0 and w <= 128 for w in (head_dim, v_dim)):
-            return TileShape(rows=256, workers=sm_count, halves=True, item_pages=1.0, half_cost=0.7)       # tcgen05
+            narrow = max(head_dim, v_dim) <= 64
+            return TileShape(rows=256, workers=sm_count, halves=True, item_pages=3.0, half_cost=0.7, thin_rows=16, thin_warps=8 if narrow else 6,
+                             thin_cost=0.4, thin_item=0.2)                                                   # tcgen05, and mma.sync for thin tiles
         return TileShape(rows=64, workers=2 * sm_count)
 
     def attn(self, q, out, tok_pos, block_table, kpages, vpages, plan, part, scale, err_flag, softcap=None, sink=None):
@@ -1773,12 +1775,13 @@ class SharedAttention:
             raise KernelError(f"shared attention: the plan is laid out for {plan.shape}, these widths want {shape}")
         if T == 0:
             return
-        rows = plan.capacity.rows
+        rows = plan.scratch_rows
+        thin = ((_ptr(plan.thin_first, torch.int32, "plan"),), (as_int(shape.thin_warps),)) if shape.halves else ((), ())
         _check((self._attn_tc if shape.halves else self._attn)(
             c_void_p(q.data_ptr()), q.stride(0), _ptr(tok_pos, torch.int32, "tok_pos"), _ptr(block_table, torch.int32, "block_table"),
             block_table.shape[1], _ptr(kpages, self.dtype, "kpages"), _ptr(vpages, self.dtype, "vpages"), c_longlong(kpages.shape[0]),
-            _ptr(plan.first, torch.int32, "plan"), _ptr(plan.items, torch.int32, "plan"), _ptr(plan.toks, torch.int32, "plan"),
-            as_int(shape.workers), _ptr(part, torch.float32, "part"), c_longlong(rows), as_int(H), as_int(G), hd, vd, c_float(scale),
+            _ptr(plan.first, torch.int32, "plan"), *thin[0], _ptr(plan.items, torch.int32, "plan"), _ptr(plan.toks, torch.int32, "plan"),
+            as_int(shape.workers), *thin[1], _ptr(part, torch.float32, "part"), c_longlong(rows), as_int(H), as_int(G), hd, vd, c_float(scale),
             c_float(softcap or 0.0), _ptr(err_flag, torch.int32, "err_flag"), _stream()), "share_attn")
         _check(self._merge(
             _ptr(part, torch.float32, "part"), c_longlong(rows), _ptr(plan.list_first, torch.int32, "plan"), _ptr(plan.list, torch.int32, "plan"),

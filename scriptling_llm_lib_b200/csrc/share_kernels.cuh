@@ -45,7 +45,7 @@ __device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareIt
 #pragma unroll
   for (int i = 0; i < QPT; i++) {
     const int r = ty * QPT + i;
-    qpos[i] = r < n_rows ? p.tok_pos[p.toks[it.tok0 + r / rep]] : -1;
+    qpos[i] = share_sees(it, r, rep);
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
@@ -163,7 +163,7 @@ __device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareIt
       float4 v = make_float4(o[i][gg][0], o[i][gg][1], o[i][gg][2], o[i][gg][3]);
       if (!(fabsf(v.x) + fabsf(v.y) + fabsf(v.z) + fabsf(v.w) < INFINITY) && ls < INFINITY)
         v = share_sum_by_key(p, it, (const A*)p.q + (size_t)p.toks[it.tok0 + r / rep] * p.q_ld + (size_t)(it.g * rep + r % rep) * hd, qpos[i], m[i], d0, it.p0, 1);
-      *(float4*)(p.part + at * vd + d0) = v;
+      *(float4*)(p.part + share_at(at, d0, vd)) = v;
     }
     if (tx == 0) *(float2*)(ml + 2 * at) = make_float2(m[i], ls);
   }
@@ -184,7 +184,9 @@ __global__ void __launch_bounds__(256) share_fma_kernel(ShareArgs p) {
 }
 
 // ------------------------------------------------------------------ joining partial results
-// A warp for a token and query head: the list's entries are read once for M, then every lane adds four values' sums over them.
+// A warp for a token and RB query heads that stand side by side in the scratch (a power of two that divides the heads of a key/value
+// head, so that their 16-byte pieces fill whole sectors). Lane j RB + r has head r of them: first entry base + j of the list (row of the
+// scratch, m, l), then the dims 4 (j + k 32 / RB) .. + 3 of the sum, of which NQ fit. Loads of four entries are under way at once.
 struct ShareMergeArgs {
   const float* part;
   long long part_rows;
@@ -193,41 +195,73 @@ struct ShareMergeArgs {
   const float* sink;         // [H] or null
   int T, H, G, vd;
 };
-template <typename A>
+template <typename A, int RB, int NQ>
 __global__ void __launch_bounds__(128) share_merge_kernel(ShareMergeArgs p) {
   pdl_launch_dependents();
   pdl_wait();
+  constexpr int J = 32 / RB;                        // entries held at a time
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (w >= (long long)p.T * p.H) return;
-  const int lane = threadIdx.x & 31, t = (int)(w / p.H), h = (int)(w % p.H), rep = p.H / p.G, g = h / rep, r = h % rep;
+  const int per = p.H / RB;
+  if (w >= (long long)p.T * per) return;
+  const int lane = threadIdx.x & 31, j = lane / RB, t = (int)(w / per), h = (int)(w % per) * RB + lane % RB, rep = p.H / p.G, g = h / rep, r = h % rep;
   const int i0 = p.list_first[(size_t)t * p.G + g], n = p.list_first[(size_t)t * p.G + g + 1] - i0;
   const float2* ml = (const float2*)(p.part + (size_t)p.part_rows * p.vd);
   const float sink = p.sink ? p.sink[h] * SHARE_LOG2E : -INFINITY;
-  float M = -INFINITY;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, ml[p.list[i0 + i] + r].x);
-  M = fmaxf(warp_max(M), sink);
+  int at = j < n ? p.list[i0 + j] + r : 0;
+  float2 v = j < n ? ml[at] : make_float2(-INFINITY, 0.f);
+  float M = v.x;
+  for (int i = j + J; i < n; i += J) M = fmaxf(M, ml[p.list[i0 + i] + r].x);
+#pragma unroll
+  for (int d = RB; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  M = fmaxf(M, sink);
   const float M0 = M == -INFINITY ? 0.f : M;                    // (nothing seen: every weight below is 2^-inf = 0)
   float den = 0.f;
-  for (int i = lane; i < n; i += 32) {
-    const float2 v = ml[p.list[i0 + i] + r];
-    den = fmaf(exp2f(v.x - M0), v.y, den);
+  float4 a[NQ];
+#pragma unroll
+  for (int k = 0; k < NQ; k++) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int base = 0; base < n; base += J) {
+    if (base) {
+      at = base + j < n ? p.list[i0 + base + j] + r : 0;
+      v = base + j < n ? ml[at] : make_float2(-INFINITY, 0.f);
+    }
+    // an entry none of whose keys this row sees, or none at all, weighs 0 and its values are not read; a sum that is NaN spoils the row
+    const float wgt = v.y != v.y ? v.y : exp2f(v.x - M0);
+    if (wgt != 0.f) den = fmaf(wgt, v.y, den);
+    const int m = min(J, n - base);
+    for (int e0 = 0; e0 < m; e0 += 4) {
+      float c[4];
+      float4 x[4][NQ];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int from = ((e0 + e) * RB + lane % RB) & 31;
+        c[e] = __shfl_sync(0xffffffffu, wgt, from);
+        const size_t row = __shfl_sync(0xffffffffu, at, from);
+        if (e0 + e >= m) c[e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < NQ; k++) {
+          const int d = 4 * (j + k * J);
+          x[e][k] = c[e] != 0.f && d < p.vd ? *(const float4*)(p.part + share_at(row, d, p.vd)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int k = 0; k < NQ; k++) {
+          a[k].x = fmaf(c[e], x[e][k].x, a[k].x);
+          a[k].y = fmaf(c[e], x[e][k].y, a[k].y);
+          a[k].z = fmaf(c[e], x[e][k].z, a[k].z);
+          a[k].w = fmaf(c[e], x[e][k].w, a[k].w);
+        }
+    }
   }
-  den = warp_sum(den);
+#pragma unroll
+  for (int d = RB; d < 32; d <<= 1) den += __shfl_xor_sync(0xffffffffu, den, d);
   if (p.sink) den += exp2f(sink - M0);
   const float inv = den > 0.f || den != den ? 1.0f / den : 0.f;
-  for (int d0 = 4 * lane; d0 < p.vd; d0 += 128) {
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = 0; i < n; i++) {
-      const size_t at = (size_t)p.list[i0 + i] + r;
-      const float m = ml[at].x;
-      if (m == -INFINITY) continue;                             // an item none of whose keys this row sees
-      const float c = exp2f(m - M0);
-      const float4 v = *(const float4*)(p.part + at * p.vd + d0);
-      a.x = fmaf(c, v.x, a.x);
-      a.y = fmaf(c, v.y, a.y);
-      a.z = fmaf(c, v.z, a.z);
-      a.w = fmaf(c, v.w, a.w);
-    }
-    st4((A*)p.out + (size_t)w * p.vd + d0, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
+  A* out = (A*)p.out + ((size_t)t * p.H + h) * p.vd;
+#pragma unroll
+  for (int k = 0; k < NQ; k++) {
+    const int d = 4 * (j + k * J);
+    if (d < p.vd) st4(out + d, make_float4(a[k].x * inv, a[k].y * inv, a[k].z * inv, a[k].w * inv));
   }
 }

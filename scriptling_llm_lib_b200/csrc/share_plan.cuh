@@ -13,15 +13,24 @@ struct ShareArgs {
   int max_pages;
   const void *kpages, *vpages;   // [n_pages][G][PAGE][hd], [n_pages][G][PAGE][vd]
   int n_pages;
-  const int *first, *items, *toks;   // of the plan: where a block's items begin, items of eight words, rows of the step in the tree's order
-  float* part;               // [part_rows][vd], then [part_rows][2]: m and l
-  long long part_rows;
+  // of the plan: where a block's items begin and where each of its warps' thin items do, items of eight words, rows of the step in the
+  // tree's order
+  const int *first, *thin_first, *items, *toks;
+  float* part;               // the rows' sums over the values (share_at), then [part_rows][2]: m and l
+  long long part_rows;       // a multiple of 32
   int H, G, hd, vd;
   float scale, softcap;
   int* err;
 };
 
-// An item as a block works on it: pages [p0, p1) of row `seq` of the table; keys up to `last`, the position of its last token
+// Where dims d .. d + 3 (d a multiple of 4) of a row of the scratch stand: 32 rows together, four dims of a row side by side. Threads that
+// have a row each then write 512 bytes in a row to memory with 16 bytes a thread (in rows of vd floats the same stores took 5 us of a block's
+// 256 x 128 sums, one line a thread).
+__device__ __forceinline__ size_t share_at(size_t row, int d, int vd) { return (row >> 5) * 32 * (size_t)vd + (size_t)d * 32 + (row & 31) * 4; }
+
+// An item as a block works on it: pages [p0, p1) of row `seq` of the table; keys up to `last`, the position of its last token. A leaf's
+// tokens are of one sequence and follow one another; a node's see all of its keys, whatever their positions (last: SHARE_NODE).
+#define SHARE_NODE 0x3fffffff
 struct ShareItem {
   int tok0, n_tok, g, p0, p1, last, part0, seq;
 };
@@ -30,14 +39,19 @@ __device__ __forceinline__ ShareItem share_item(const ShareArgs& p, int i) {
   ShareItem it;
   it.tok0 = a.x;
   it.n_tok = a.y;
-  it.last = p.tok_pos[a.z];
+  it.last = a.z < 0 ? SHARE_NODE : min(p.tok_pos[a.z], SHARE_NODE - 1);
   it.g = a.w;
   it.p0 = b.x;
-  const int end = it.last / SLLM_PAGE + 1;         // (a plan may be older than the step, and the sequences shorter or longer)
+  const int end = it.last / SLLM_PAGE + 1;         // (a plan may be older than the step, and its sequences longer now)
   it.p1 = b.y < 0 || b.y > end ? end : b.y;
   it.part0 = b.z;
   it.seq = b.w;
   return it;
+}
+// the position up to which row `rho` of an item's tile sees keys; -1 for a row past the tile's end
+__device__ __forceinline__ int share_sees(const ShareItem& it, int rho, int rep) {
+  const int i = rho / rep;
+  return i >= it.n_tok ? -1 : it.last == SHARE_NODE ? SHARE_NODE : it.last - (it.n_tok - 1 - i);
 }
 // the page at place `i` of a row of the table; -1 (and *err) where there is none
 __device__ __forceinline__ int share_page(const ShareArgs& p, const int* row, int i) {
@@ -51,7 +65,7 @@ __device__ __forceinline__ int share_page(const ShareArgs& p, const int* row, in
 // finite. In a tile's product a page's values all enter it, with weights of zero, and 0 times what is not finite is NaN. Pages t0,
 // t0 + step, ... of the item's.
 template <typename A>
-__device__ __noinline__ float4 share_sum_by_key(const ShareArgs& p, const ShareItem& it, const A* q, int qpos, float m, int d0, int t0, int step) {
+__device__ __noinline__ float4 share_sum_by_key(const ShareArgs& p, const ShareItem it, const A* q, int qpos, float m, int d0, int t0, int step) {
   const int* row = p.block_table + (size_t)it.seq * p.max_pages;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int key = t0 * SLLM_PAGE; key <= qpos && key < it.p1 * SLLM_PAGE; key++) {

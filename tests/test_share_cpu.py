@@ -204,7 +204,8 @@ def _batch(rng, n, rep, runs):
     return table, held, new
 
 
-@pytest.mark.parametrize("shape", [TileShape(256, 148, True, 1.0, 0.7), TileShape(64, 296), TileShape(64, 7, min_pages=1), TileShape(16, 40, True)], ids=str)
+@pytest.mark.parametrize("shape", [TileShape(256, 148, True, 1.0, 0.7), TileShape(64, 296), TileShape(64, 7, min_pages=1), TileShape(16, 40, True),
+                                   TileShape(256, 148, True, 2.0, 0.7, 2, 16, 8, 0.4, 0.2)], ids=str)
 @pytest.mark.parametrize("runs", [False, True])
 def test_a_plan_covers_every_key_of_every_row_once(shape, runs):
     rng = random.Random(11)
@@ -218,13 +219,17 @@ def test_a_plan_covers_every_key_of_every_row_once(shape, runs):
         assert plan.n_rows == T and sorted(p["toks"].tolist()) == list(range(T))
         pages, owner, rows_of = {}, {}, {}
         for tok0, n_tok, last, g, a, b, part0, row in p["items"].tolist():
-            end = pos[last] // PAGE + 1
+            end = pos[last] // PAGE + 1 if last >= 0 else b
             b = end if b < 0 else min(b, end)
-            assert 1 <= n_tok * rep <= shape.rows and p["toks"][tok0 + n_tok - 1] == last and a <= b
+            assert 1 <= n_tok * rep <= shape.rows and a < b and (last < 0 or p["toks"][tok0 + n_tok - 1] == last)
+            if last >= 0:                                   # of one sequence, one behind the other
+                assert [pos[int(p["toks"][tok0 + i])] for i in range(n_tok)] == list(range(pos[last] - n_tok + 1, pos[last] + 1))
+            else:                                           # a node: every one of its keys is in front of all its tokens
+                assert all(pos[int(p["toks"][tok0 + i])] >= b * PAGE for i in range(n_tok))
             for i in range(n_tok):
                 t = int(p["toks"][tok0 + i])
                 pages.setdefault((t, g), []).extend((j, int(table[row, j])) for j in range(a, b))
-                for half in range(2 if shape.halves and n_tok * rep <= shape.rows // 2 else 1):
+                for half in range(2 if shape.halves and shape.thin_rows < n_tok * rep <= shape.rows // 2 else 1):
                     at = part0 + half * n_tok * rep + i * rep
                     assert at not in owner
                     owner[at] = (t, g)
@@ -237,8 +242,10 @@ def test_a_plan_covers_every_key_of_every_row_once(shape, runs):
                 assert all(seen[j] == table[seq[t], j] for j in range(pos[t] // PAGE + 1))     # every page that it sees, as its own table has it
                 mine = p["list"][p["list_first"][t * G + g]:p["list_first"][t * G + g + 1]]
                 assert len(mine) and sorted(int(e) for e in mine) == sorted(rows_of[t, g])
-        first = p["first"]
-        assert first[0] == 0 and first[-1] == len(p["items"]) and (np.diff(first) >= 0).all()
+        first, thin = p["first"], p["thin_first"]
+        assert first[0] == 0 and first[-1] == thin[0] and thin[-1] == len(p["items"]) and (np.diff(first) >= 0).all() and (np.diff(thin) >= 0).all()
+        rows = p["items"][:, 1] * rep
+        assert (rows[:thin[0]] > shape.thin_rows).all() and (rows[thin[0]:] <= shape.thin_rows).all()
         if not runs:
             cap = PlanCapacity.of_decode(n, G * rep, G, shape)
             assert plan.fits(cap)
@@ -253,14 +260,18 @@ def plan_with(roomy, plan):
 def test_plans_share_the_work_evenly_among_blocks():
     table = np.arange(64 * 200, dtype=np.int32).reshape(64, 200)
     table[:, :128] = np.arange(128)
-    shape = TileShape(256, 148, True, 1.0, 0.7)
-    plan = SharePlan.build(table, [8192 + 40 * i for i in range(64)], [1] * 64, 32, 8, shape, None)
-    items, first = plan.parts["items"], plan.parts["first"]
-    pos = np.asarray([8192 + 40 * i for i in range(64)])
-    end = np.where(items[:, 5] < 0, pos[items[:, 2]] // PAGE + 1, items[:, 5])
-    cost = (end - items[:, 4]) * np.where(items[:, 1] * 4 <= 128, 0.7, 1.0) + 1.0
-    load = [cost[a:b].sum() for a, b in zip(first, first[1:])]
-    assert max(load) < 1.5 * sum(load) / 148
+    held = np.asarray([8192 + 40 * i for i in range(64)])
+    for thin in (0, 16):
+        shape = TileShape(256, 148, True, 1.0, 0.7, 2, thin, 8 if thin else 0, 0.5, 0.25)
+        plan = SharePlan.build(table, held, [1] * 64, 32, 8, shape, None)
+        items, first, warps = plan.parts["items"], plan.parts["first"], plan.parts["thin_first"]
+        end = np.where(items[:, 5] < 0, held[items[:, 2]] // PAGE + 1, items[:, 5])
+        cost = (end - items[:, 4]) * np.where(items[:, 1] * 4 <= 128, 0.7, 1.0) + 1.0
+        load = np.asarray([cost[a:b].sum() for a, b in zip(first, first[1:])])
+        if thin:
+            cost = (end - items[:, 4]) * 0.5 + 0.25
+            load += np.asarray([max(cost[a:b].sum() * 8 for a, b in zip(w, w[1:])) for w in (warps[8 * k:8 * k + 9] for k in range(148))])
+        assert max(load) < 1.7 * sum(load) / 148
 
 
 def test_plans_refuse_what_does_not_fit_together():
