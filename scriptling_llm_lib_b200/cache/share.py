@@ -42,6 +42,7 @@ class TileShape:
     thin_warps: int = 0
     thin_cost: float = 0.0       # what a page of a thin tile costs the block
     thin_item: float = 0.0       # and an item
+    thin_start: float = 0.0      # and having any behind others
 
 
 def share_tree(table: np.ndarray, whole: np.ndarray):
@@ -261,7 +262,8 @@ def _lay_out(order, nodes, own, held, new, rep: int, n_kv: int, shape: TileShape
     i1, b1, e1, w1 = _cut(c[:n_thick], pages_u[:n_thick], share * np.arange(1, shape.workers), shape.min_pages)
     if n_thick < len(u):
         load = np.bincount(w1, weights=c[i1] * (e1 - b1) / np.maximum(1, pages_u[i1]), minlength=shape.workers)
-        left = np.repeat(np.maximum(share - load, 0.02 * share) / shape.thin_warps, shape.thin_warps)
+        left = np.maximum(share - load - np.where(load > 0, shape.thin_start, 0.0), 0.0)
+        left = np.repeat((left if left.any() else np.ones_like(left)) / shape.thin_warps, shape.thin_warps)
         line = np.cumsum(left)
         i2, b2, e2, w2 = _cut(c[n_thick:], pages_u[n_thick:], line[:-1] * (float(c[n_thick:].sum()) / line[-1]), 1)
     else:

@@ -21,6 +21,7 @@
 // compute nothing. Waits are bounded (2 s), after which the kernel raises *err, lets its copies land, frees its tensor memory and returns.
 #include "attn_tcgen05.cuh"
 #include "share_plan.cuh"
+#include <type_traits>
 
 #define FS_THREADS 384       // warp 0: TMA, warps 1-2: the products of either half, warp 3: queries, warps 4-7 and 8-11: softmax of either half
 #define FS_ROWS 128          // rows of a half
@@ -49,6 +50,13 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// an 8 x 8 matrix of 16-bit elements, two of a row in each lane, turned over
+__device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
 // warps with thin tiles, and the buffers (a page of keys or of values) that each has
 template <int KD, int VD>
 __host__ __device__ constexpr int fs_thin_warps() { return KD <= 64 && VD <= 64 ? 8 : 6; }
@@ -56,8 +64,10 @@ template <int KD, int VD>
 __host__ __device__ constexpr int fs_thin_bufs() { return KD <= 64 && VD <= 64 ? 3 : 2; }
 
 // One warp's thin items [i0, i1): a page's keys, then its values, into the buffer that comes round, fetched as far ahead as there are
-// buffers (across items: a cursor walks the list in front of the work). Lane (r = lane / 4, c = lane % 4) has rows r and r + 8 of the
-// tile; of the scores keys 8 n + 2 c and + 1, of the output dims 8 n + 2 c and + 1.
+// buffers (across items: a cursor walks the list in front of the work). Keys, and dims of the values, are the 16 rows of mma.m16n8k16 and
+// the tile's rows its 8 columns, twice where it has more than 8: half the products of the other way round for the usual tile, whose few
+// rows would leave most of 16 empty. Lane (r = lane / 4, c = lane % 4) has of the scores keys 16 n + r and + 8 of rows 2 c and 2 c + 1,
+// of the output their dims 16 d + r and + 8.
 template <int KD, int VD>
 __device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensorMap* map_v, const ShareArgs& p, int i0, int i1, uint8_t* buf,
                                         uint32_t bar, volatile int* abort) {
@@ -68,163 +78,239 @@ __device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensor
   const float sc = p.scale * FT_LOG2E;
   if (i0 >= i1) return;
 
-  // ---- the cursor: what is fetched next
-  int fi = i0, ft = 0, fbase = 0, ids = 0, fetched = 0, taken = 0;
-  ShareItem f = share_item(p, fi);
-  ft = f.p0;
-  auto settle = [&]() {               // to an item that has pages left; its next 32 page ids, one a lane
-    while (ft >= f.p1 && ++fi < i1) {
-      f = share_item(p, fi);
-      ft = f.p0;
-    }
-    if (fi < i1) {
-      fbase = ft;
-      ids = ft + lane < f.p1 ? share_page(p, p.block_table + (size_t)f.seq * p.max_pages, ft + lane) : 0;
+  // ---- 32 items at a time are held one a lane, with their first token and the ids of their first four pages: what an item needs before
+  // its first product is then on the way together (one by one, each item was three loads deep: 4 us)
+  int hbase = i0;
+  ShareItem held;
+  int tok_first = 0, page4[4];
+  auto hold = [&](int base) {
+    hbase = base;
+    if (base + lane < i1) {
+      held = share_item(p, base + lane);
+      tok_first = p.toks[held.tok0];
+      const int* row = p.block_table + (size_t)held.seq * p.max_pages;
+#pragma unroll
+      for (int k = 0; k < 4; k++) page4[k] = held.p0 + k < held.p1 ? share_page(p, row, held.p0 + k) : -1;
     }
   };
-  settle();
+  auto held_item = [&](int i) -> ShareItem {
+    const int from = i - hbase;
+    ShareItem it;
+    it.tok0 = __shfl_sync(0xffffffffu, held.tok0, from);
+    it.n_tok = __shfl_sync(0xffffffffu, held.n_tok, from);
+    it.g = __shfl_sync(0xffffffffu, held.g, from);
+    it.p0 = __shfl_sync(0xffffffffu, held.p0, from);
+    it.p1 = __shfl_sync(0xffffffffu, held.p1, from);
+    it.last = __shfl_sync(0xffffffffu, held.last, from);
+    it.part0 = __shfl_sync(0xffffffffu, held.part0, from);
+    it.seq = __shfl_sync(0xffffffffu, held.seq, from);
+    return it;
+  };
+  // ---- the cursor: what is fetched next, among the items held
+  int fi = i0, ft = 0, fp0 = 0, fp1 = 0, fg = 0, fseq = 0, fetched = 0, taken = 0;
+  auto settle = [&]() {               // to an item that has pages left
+    while (ft >= fp1 && ++fi < min(i1, hbase + 32)) {
+      const ShareItem f = held_item(fi);
+      ft = fp0 = f.p0;
+      fp1 = f.p1;
+      fg = f.g;
+      fseq = f.seq;
+    }
+  };
   auto fetch = [&]() {                // one buffer: a page's keys if `fetched` is even, else its values
-    if (fi >= i1) return;
-    const int page = __shfl_sync(0xffffffffu, ids, ft - fbase), b = fetched % BUFS;
+    if (fi >= min(i1, hbase + 32)) return;
+    const int b = fetched % BUFS, k = ft - fp0;
+    int page;
+    if (k < 4) {
+      const int mine = k == 0 ? page4[0] : k == 1 ? page4[1] : k == 2 ? page4[2] : page4[3];
+      page = __shfl_sync(0xffffffffu, mine, fi - hbase);
+    } else {
+      page = share_page(p, p.block_table + (size_t)fseq * p.max_pages, ft);
+    }
     if (lane == 0) {
       const int at = page < 0 ? p.n_pages : page;
       const uint32_t to = sB + b * BUF, on = bar + 8 * b;
       if (fetched & 1) {
         mbar_expect_tx(on, V_BYTES);
 #pragma unroll
-        for (int a = 0; a < NV; a++) tma_load_3d(to + a * KA, map_v, 64 * a, f.g * FS_BK, at, on);
+        for (int a = 0; a < NV; a++) tma_load_3d(to + a * KA, map_v, 64 * a, fg * FS_BK, at, on);
       } else {
         mbar_expect_tx(on, K_BYTES);
 #pragma unroll
-        for (int a = 0; a < NK; a++) tma_load_3d(to + a * KA, map_k, 64 * a, f.g * FS_BK, at, on);
+        for (int a = 0; a < NK; a++) tma_load_3d(to + a * KA, map_k, 64 * a, fg * FS_BK, at, on);
       }
     }
-    if ((fetched & 1) && (++ft >= f.p1 || ft - fbase == 32)) settle();
+    __syncwarp();
+    if ((fetched & 1) && ++ft >= fp1) settle();
     fetched++;
   };
-  for (int b = 0; b < BUFS; b++) fetch();
+  auto begin = [&](int base) {        // the buffers are empty: hold the next items and fill them
+    hold(base);
+    fi = base - 1;
+    ft = fp1 = 0;
+    settle();
+    for (int b = 0; b < BUFS; b++) fetch();
+  };
+  begin(i0);
 
   bool ok = true;
   for (int i = i0; ok && i < i1; i++) {
-    const ShareItem it = share_item(p, i);
+    if (i == hbase + 32) begin(i);
+    const ShareItem it = held_item(i);
     const int n_rows = it.n_tok * rep, see0 = share_sees(it, r0, rep), see1 = share_sees(it, r0 + 8, rep);
-    const bf16* q0 = (const bf16*)p.q + (see0 < 0 ? 0 : (size_t)p.toks[it.tok0 + r0 / rep] * p.q_ld + (size_t)(it.g * rep + r0 % rep) * p.hd);
-    const bf16* q1 = (const bf16*)p.q + (see1 < 0 ? 0 : (size_t)p.toks[it.tok0 + (r0 + 8) / rep] * p.q_ld + (size_t)(it.g * rep + (r0 + 8) % rep) * p.hd);
-    uint32_t q[KD / 16][4];
+    const int first = __shfl_sync(0xffffffffu, tok_first, i - hbase);       // (a leaf's tokens follow one another)
+    const int t0 = see0 < 0 ? 0 : it.last != SHARE_NODE ? first + r0 / rep : p.toks[it.tok0 + r0 / rep];
+    const int t1 = see1 < 0 ? 0 : it.last != SHARE_NODE ? first + (r0 + 8) / rep : p.toks[it.tok0 + (r0 + 8) / rep];
+    const bf16* q0 = (const bf16*)p.q + (see0 < 0 ? 0 : (size_t)t0 * p.q_ld + (size_t)(it.g * rep + r0 % rep) * p.hd);
+    const bf16* q1 = (const bf16*)p.q + (see1 < 0 ? 0 : (size_t)t1 * p.q_ld + (size_t)(it.g * rep + (r0 + 8) % rep) * p.hd);
+    auto work = [&](auto groups) {                    // 1: up to 8 rows, 2: up to 16
+    constexpr int GROUPS = decltype(groups)::value;
+    uint32_t q[GROUPS][KD / 16][2];                      // queries of rows r0 and r0 + 8: the second operand of the scores' products
 #pragma unroll
     for (int k = 0; k < KD / 16; k++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int d = 16 * k + c2 + (e >> 1) * 8;
-        q[k][e] = d < p.hd && ((e & 1) ? see1 : see0) >= 0 ? *(const uint32_t*)(((e & 1) ? q1 : q0) + d) : 0u;
+      for (int e = 0; e < 2; e++) {
+        const int d = 16 * k + c2 + 8 * e;
+        q[0][k][e] = d < p.hd && see0 >= 0 ? *(const uint32_t*)(q0 + d) : 0u;
+        if (GROUPS == 2) q[GROUPS - 1][k][e] = d < p.hd && see1 >= 0 ? *(const uint32_t*)(q1 + d) : 0u;
       }
-    float o[VD / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    int see[GROUPS][2];                                  // of rows c2, c2 + 1 and of those 8 on
+    float o[GROUPS][VD / 16][4], m[GROUPS][2], l[GROUPS][2];
 #pragma unroll
-    for (int n = 0; n < VD / 8; n++)
+    for (int x = 0; x < GROUPS; x++) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) o[n][e] = 0.f;
+      for (int e = 0; e < 2; e++) {
+        see[x][e] = share_sees(it, 8 * x + c2 + e, rep);
+        m[x][e] = -INFINITY;
+        l[x][e] = 0.f;
+      }
+#pragma unroll
+      for (int d = 0; d < VD / 16; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[x][d][e] = 0.f;
+    }
+    const bool masked = it.last != SHARE_NODE;
     for (int t = it.p0; t < it.p1; t++) {
-      float s[8][4];
+      float s[GROUPS][4][4];
 #pragma unroll
-      for (int n = 0; n < 8; n++)
+      for (int x = 0; x < GROUPS; x++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[n][e] = 0.f;
+        for (int n = 0; n < 4; n++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) s[x][n][e] = 0.f;
       {
         const int b = taken % BUFS;
         ok = mbar_wait(bar + 8 * b, (taken / BUFS) & 1, abort);
-        if (!ok) break;
-        const uint32_t from = sB + b * BUF, key = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
-#pragma unroll
-        for (int k = 0; k < KD / 16; k++) {
-          if (16 * k >= p.hd) break;
+        if (!ok) return;
+        const uint32_t from = sB + b * BUF, key = (lane & 7) + (((lane >> 3) & 1) << 3), ch = lane >> 4;
+        // (a step's four matrices are on their way while the products of the step before run: in turn with them each load's 33 clocks show)
+        uint32_t r[2][4][4];
+        auto load = [&](int k) {
 #pragma unroll
           for (int n = 0; n < 4; n++) {
-            uint32_t r[4];
             const uint32_t row = 16 * n + key, c = (2 * k + ch) & 7;
-            ldmatrix4(from + (k >> 2) * KA + row * 128 + ((c ^ (row & 7)) << 4), r);
-            mma16816(s[2 * n], q[k], r[0], r[1]);
-            mma16816(s[2 * n + 1], q[k], r[2], r[3]);
+            ldmatrix4(from + (k >> 2) * KA + row * 128 + ((c ^ (row & 7)) << 4), r[k & 1][n]);
           }
+        };
+        load(0);
+#pragma unroll
+        for (int k = 0; k < KD / 16; k++) {
+          if (k + 1 < KD / 16) load(k + 1);          // (past hd: zeros)
+#pragma unroll
+          for (int x = 0; x < GROUPS; x++)
+#pragma unroll
+            for (int n = 0; n < 4; n++) mma16816(s[x][n], r[k & 1][n], q[x][k][0], q[x][k][1]);
         }
         taken++;
         __syncwarp();
         fetch();
       }
-      if (p.softcap > 0.f) {
-        const float cap_out = p.softcap / p.scale, cap_in = p.scale / p.softcap;
+      uint32_t w[GROUPS][4][2];                  // weights of 16 keys: the second operand of the product with their values
 #pragma unroll
-        for (int n = 0; n < 8; n++)
+      for (int x = 0; x < GROUPS; x++) {
+        if (p.softcap > 0.f) {
+          const float cap_out = p.softcap / p.scale, cap_in = p.scale / p.softcap;
 #pragma unroll
-          for (int e = 0; e < 4; e++) s[n][e] = __uint_as_float(ft_cap(__float_as_uint(s[n][e]), cap_out, cap_in));
-      }
-      if (t * FS_BK + FS_BK - 1 > it.last - (it.n_tok - 1)) {      // (rows past the tile's end see nothing here, zeros elsewhere)
+          for (int n = 0; n < 4; n++)
 #pragma unroll
-        for (int n = 0; n < 8; n++)
-#pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (t * FS_BK + 8 * n + c2 + (e & 1) > ((e >> 1) ? see1 : see0)) s[n][e] = -INFINITY;
-      }
-      float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < 8; n++) {
-        x0 = ft_max3(x0, s[n][0], s[n][1]);
-        x1 = ft_max3(x1, s[n][2], s[n][3]);
-      }
-#pragma unroll
-      for (int d = 1; d < 4; d <<= 1) {
-        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, d));
-        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, d));
-      }
-      if (__any_sync(0xffffffffu, x0 > m0 || x1 > m1)) {
-        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1), f0 = m0 == -INFINITY ? 0.f : ft_ex2((m0 - n0) * sc), f1 = m1 == -INFINITY ? 0.f : ft_ex2((m1 - n1) * sc);
-        m0 = n0;
-        m1 = n1;
-        l0 *= f0;
-        l1 *= f1;
-#pragma unroll
-        for (int n = 0; n < VD / 8; n++) {
-          o[n][0] *= f0;
-          o[n][1] *= f0;
-          o[n][2] *= f1;
-          o[n][3] *= f1;
+            for (int e = 0; e < 4; e++) s[x][n][e] = __uint_as_float(ft_cap(__float_as_uint(s[x][n][e]), cap_out, cap_in));
         }
-      }
-      const float a0 = m0 == -INFINITY ? 0.f : -m0 * sc, a1 = m1 == -INFINITY ? 0.f : -m1 * sc;
-      uint32_t w[4][4];                // weights of 16 keys: the first operand of the product with their values
+        if (masked && t * FS_BK + FS_BK - 1 > it.last - (it.n_tok - 1)) {      // (rows past the tile's end see nothing here, zeros elsewhere)
 #pragma unroll
-      for (int n = 0; n < 8; n++) {
-        const float e0 = ft_ex2(fmaf(s[n][0], sc, a0)), e1 = ft_ex2(fmaf(s[n][1], sc, a0)), e2 = ft_ex2(fmaf(s[n][2], sc, a1)), e3 = ft_ex2(fmaf(s[n][3], sc, a1));
-        l0 += e0 + e1;
-        l1 += e2 + e3;
-        const __nv_bfloat162 u = __floats2bfloat162_rn(e0, e1), v = __floats2bfloat162_rn(e2, e3);
-        w[n >> 1][2 * (n & 1)] = *(const uint32_t*)&u;
-        w[n >> 1][2 * (n & 1) + 1] = *(const uint32_t*)&v;
+          for (int n = 0; n < 4; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (t * FS_BK + 16 * n + r0 + 8 * (e >> 1) > see[x][e & 1]) s[x][n][e] = -INFINITY;
+        }
+        float mx[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          mx[e] = fmaxf(ft_max3(s[x][0][e], s[x][0][e + 2], s[x][1][e]), ft_max3(s[x][1][e + 2], s[x][2][e], s[x][2][e + 2]));
+          mx[e] = ft_max3(mx[e], s[x][3][e], s[x][3][e + 2]);
+        }
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) {
+          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], d));
+          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], d));
+        }
+        if (__any_sync(0xffffffffu, mx[0] > m[x][0] || mx[1] > m[x][1])) {
+          float f[2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float grown = fmaxf(m[x][e], mx[e]);
+            f[e] = m[x][e] == -INFINITY ? 0.f : ft_ex2((m[x][e] - grown) * sc);
+            m[x][e] = grown;
+            l[x][e] *= f[e];
+          }
+#pragma unroll
+          for (int d = 0; d < VD / 16; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[x][d][e] *= f[e & 1];
+        }
+        const float a0 = m[x][0] == -INFINITY ? 0.f : -m[x][0] * sc, a1 = m[x][1] == -INFINITY ? 0.f : -m[x][1] * sc;
+#pragma unroll
+        for (int n = 0; n < 4; n++) {
+          const float e0 = ft_ex2(fmaf(s[x][n][0], sc, a0)), e1 = ft_ex2(fmaf(s[x][n][1], sc, a1)), e2 = ft_ex2(fmaf(s[x][n][2], sc, a0)), e3 = ft_ex2(fmaf(s[x][n][3], sc, a1));
+          l[x][0] += e0 + e2;
+          l[x][1] += e1 + e3;
+          const __nv_bfloat162 u = __floats2bfloat162_rn(e0, e1), v = __floats2bfloat162_rn(e2, e3);
+          w[x][n][0] = transposed8x8(*(const uint32_t*)&u);
+          w[x][n][1] = transposed8x8(*(const uint32_t*)&v);
+        }
       }
       {
         const int b = taken % BUFS;
         ok = mbar_wait(bar + 8 * b, (taken / BUFS) & 1, abort);
-        if (!ok) break;
+        if (!ok) return;
         const uint32_t from = sB + b * BUF;
         const int n_valid = it.last + 1 - t * FS_BK;
         if (n_valid < FS_BK) {           // behind the last token: weights are zero, but 0 * NaN is NaN
           for (int e = lane; e < (FS_BK - n_valid) * 8 * NV; e += 32) {
-            const int blk = e / ((FS_BK - n_valid) * 8), e1 = e % ((FS_BK - n_valid) * 8);
+            const int blk = NV == 1 ? 0 : e & 1, e1 = e / NV;
             *(uint4*)(buf + b * BUF + blk * KA + (n_valid + e1 / 8) * 128 + (e1 % 8) * 16) = make_uint4(0, 0, 0, 0);
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
         }
-        const uint32_t key = (lane & 7) + (((lane >> 3) & 1) << 3), ch = lane >> 4;
+        const uint32_t key = (lane & 7) + ((lane >> 4) << 3), ch = (lane >> 3) & 1;
+        uint32_t r[2][4][4];
+        auto load = [&](int n, int d4) {             // 16 keys of 64 dims
 #pragma unroll
-        for (int n = 0; n < VD / 16; n++) {
-          if (16 * n >= p.vd) break;
+          for (int d = 0; d < 4; d++) {
+            const uint32_t row = 16 * n + key, c = 2 * d + ch;
+            ldmatrix4_trans(from + d4 * KA + row * 128 + ((c ^ (row & 7)) << 4), r[n & 1][d]);
+          }
+        };
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            uint32_t r[4];
-            const uint32_t row = 16 * k + key, c = (2 * n + ch) & 7;
-            ldmatrix4_trans(from + (n >> 2) * KA + row * 128 + ((c ^ (row & 7)) << 4), r);
-            mma16816(o[2 * n], w[k], r[0], r[1]);
-            mma16816(o[2 * n + 1], w[k], r[2], r[3]);
+        for (int d4 = 0; d4 < NV; d4++) {
+          load(0, d4);
+#pragma unroll
+          for (int n = 0; n < 4; n++) {
+            if (n < 3) load(n + 1, d4);
+#pragma unroll
+            for (int x = 0; x < GROUPS; x++)
+#pragma unroll
+              for (int d = 0; d < 4; d++) mma16816(o[x][4 * d4 + d], r[n & 1][d], w[x][n][0], w[x][n][1]);
           }
         }
         taken++;
@@ -232,39 +318,43 @@ __device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensor
         fetch();
       }
     }
-    if (!ok) break;
-#pragma unroll
-    for (int d = 1; d < 4; d <<= 1) {
-      l0 += __shfl_xor_sync(0xffffffffu, l0, d);
-      l1 += __shfl_xor_sync(0xffffffffu, l1, d);
-    }
-    float any0 = 0.f, any1 = 0.f;                   // not 0: something is not finite
-#pragma unroll
-    for (int n = 0; n < VD / 8; n++) {
-      any0 = fmaf(o[n][0], 0.f, fmaf(o[n][1], 0.f, any0));
-      any1 = fmaf(o[n][2], 0.f, fmaf(o[n][3], 0.f, any1));
-    }
-    const bool bad0 = any0 != 0.f && l0 < INFINITY, bad1 = any1 != 0.f && l1 < INFINITY;
+    if (!ok) return;
     float* ml = p.part + (size_t)p.part_rows * p.vd;
 #pragma unroll
-    for (int half = 0; half < 2; half++) {
-      const int r = r0 + 8 * half;
-      if (r >= n_rows) continue;
-      const size_t at = (size_t)it.part0 + r;
-      if (half ? bad1 : bad0) {
-#pragma unroll 1
-        for (int d = c2; d < p.vd; d += 8) {
-          const float4 v = share_sum_by_key(p, it, half ? q1 : q0, half ? see1 : see0, (half ? m1 : m0) * sc, d & ~3, it.p0, 1);
-          *(float2*)(p.part + share_at(at, d & ~3, p.vd) + (d & 2)) = (d & 2) ? make_float2(v.z, v.w) : make_float2(v.x, v.y);
-        }
-      } else {
+    for (int x = 0; x < GROUPS; x++) {
 #pragma unroll
-        for (int n = 0; n < VD / 8; n++)
-          if (8 * n < p.vd)
-            *(float2*)(p.part + share_at(at, (8 * n + c2) & ~3, p.vd) + (c2 & 2)) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+      for (int e = 0; e < 2; e++) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[x][e] += __shfl_xor_sync(0xffffffffu, l[x][e], d);
+        const int r = 8 * x + c2 + e;
+        if (r >= n_rows) continue;
+        const size_t at = (size_t)it.part0 + r;
+        float any = 0.f;                            // not 0: something is not finite
+#pragma unroll
+        for (int d = 0; d < VD / 16; d++) any = fmaf(o[x][d][e], 0.f, fmaf(o[x][d][e + 2], 0.f, any));
+        if (any != 0.f && l[x][e] < INFINITY) {
+          const bf16* qr = (const bf16*)p.q + (size_t)p.toks[it.tok0 + r / rep] * p.q_ld + (size_t)(it.g * rep + r % rep) * p.hd;
+#pragma unroll 1
+          for (int d = r0; d < p.vd; d += 8) {
+            const float4 v = share_sum_by_key(p, it, qr, see[x][e], m[x][e] * sc, d & ~3, it.p0, 1);
+            p.part[share_at(at, d & ~3, p.vd) + (d & 3)] = (d & 3) == 0 ? v.x : (d & 3) == 1 ? v.y : (d & 3) == 2 ? v.z : v.w;
+          }
+        } else {
+#pragma unroll
+          for (int d = 0; d < VD / 16; d++)
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+              const int dim = 16 * d + 8 * k + r0;
+              if (dim < p.vd) p.part[share_at(at, dim & ~3, p.vd) + (dim & 3)] = o[x][d][e + 2 * k];
+            }
+        }
+        if (r0 == 0) *(float2*)(ml + 2 * at) = make_float2(m[x][e] * sc, l[x][e]);
       }
-      if ((lane & 3) == 0) *(float2*)(ml + 2 * at) = make_float2((half ? m1 : m0) * sc, half ? l1 : l0);
     }
+    };
+    if (n_rows <= 8) work(std::integral_constant<int, 1>());
+    else work(std::integral_constant<int, 2>());
+    if (!ok) break;
     __syncwarp();
   }
   if (!ok || *abort) {                // let the copies that are under way land before the block leaves

@@ -1744,8 +1744,8 @@ class SharedAttention:
             sm_count = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
         if self.dtype == torch.bfloat16 and all(w % 8 == 0 and w <= 128 for w in (head_dim, v_dim)):
             narrow = max(head_dim, v_dim) <= 64
-            return TileShape(rows=256, workers=sm_count, halves=True, item_pages=3.0, half_cost=0.7, thin_rows=16, thin_warps=8 if narrow else 6,
-                             thin_cost=0.4, thin_item=0.2)                                                   # tcgen05, and mma.sync for thin tiles
+            return TileShape(rows=256, workers=sm_count, halves=True, item_pages=6.0, half_cost=0.7, thin_rows=16, thin_warps=8 if narrow else 6,
+                             thin_cost=0.35 if narrow else 0.5, thin_item=0.2, thin_start=4.0)                                                   # tcgen05, and mma.sync for thin tiles
         return TileShape(rows=64, workers=2 * sm_count)
 
     def attn(self, q, out, tok_pos, block_table, kpages, vpages, plan, part, scale, err_flag, softcap=None, sink=None):

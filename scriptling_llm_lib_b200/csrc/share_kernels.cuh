@@ -195,15 +195,18 @@ struct ShareMergeArgs {
   const float* sink;         // [H] or null
   int T, H, G, vd;
 };
-template <typename A, int RB, int NQ>
+// With SPLIT the four warps of a block take every fourth run of entries of one output each and meet in shared memory: where outputs are
+// few, the chain of an output's loads (four entries at a time, a microsecond each) is what the kernel lasts.
+template <typename A, int RB, int NQ, bool SPLIT>
 __global__ void __launch_bounds__(128) share_merge_kernel(ShareMergeArgs p) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int J = 32 / RB;                        // entries held at a time
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int per = p.H / RB;
+  __shared__ float4 met[SPLIT ? 3 : 1][NQ][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = p.H / RB;
+  const long long w = SPLIT ? (long long)blockIdx.x : (long long)blockIdx.x * 4 + warp;
   if (w >= (long long)p.T * per) return;
-  const int lane = threadIdx.x & 31, j = lane / RB, t = (int)(w / per), h = (int)(w % per) * RB + lane % RB, rep = p.H / p.G, g = h / rep, r = h % rep;
+  const int j = lane / RB, t = (int)(w / per), h = (int)(w % per) * RB + lane % RB, rep = p.H / p.G, g = h / rep, r = h % rep;
   const int i0 = p.list_first[(size_t)t * p.G + g], n = p.list_first[(size_t)t * p.G + g + 1] - i0;
   const float2* ml = (const float2*)(p.part + (size_t)p.part_rows * p.vd);
   const float sink = p.sink ? p.sink[h] * SHARE_LOG2E : -INFINITY;
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(128) share_merge_kernel(ShareMergeArgs p) {
     const float wgt = v.y != v.y ? v.y : exp2f(v.x - M0);
     if (wgt != 0.f) den = fmaf(wgt, v.y, den);
     const int m = min(J, n - base);
-    for (int e0 = 0; e0 < m; e0 += 4) {
+    for (int e0 = SPLIT ? 4 * warp : 0; e0 < m; e0 += SPLIT ? 16 : 4) {
       float c[4];
       float4 x[4][NQ];
 #pragma unroll
@@ -257,6 +260,23 @@ __global__ void __launch_bounds__(128) share_merge_kernel(ShareMergeArgs p) {
 #pragma unroll
   for (int d = RB; d < 32; d <<= 1) den += __shfl_xor_sync(0xffffffffu, den, d);
   if (p.sink) den += exp2f(sink - M0);
+  if constexpr (SPLIT) {                            // (every warp has the whole of den)
+    if (warp > 0)
+#pragma unroll
+      for (int k = 0; k < NQ; k++) met[warp - 1][k][lane] = a[k];
+    __syncthreads();
+    if (warp > 0) return;
+#pragma unroll
+    for (int o = 0; o < 3; o++)
+#pragma unroll
+      for (int k = 0; k < NQ; k++) {
+        const float4 b = met[o][k][lane];
+        a[k].x += b.x;
+        a[k].y += b.y;
+        a[k].z += b.z;
+        a[k].w += b.w;
+      }
+  }
   const float inv = den > 0.f || den != den ? 1.0f / den : 0.f;
   A* out = (A*)p.out + ((size_t)t * p.H + h) * p.vd;
 #pragma unroll
