@@ -13,6 +13,7 @@ rows' partial results in a scratch buffer; a list says which of them belong to a
 """
 from __future__ import annotations
 
+import ctypes
 from dataclasses import dataclass
 
 import numpy as np
@@ -141,6 +142,11 @@ class SharePlan:
             views.append(self.dev[at:at + n])
             at += n
         self.first, self.thin_first, self.items, self.toks, self.list_first, self.list = views
+        self._pointers = tuple(ctypes.c_void_p(v.data_ptr()) for v in views)
+
+    def pointers(self):
+        """Addresses of the buffer's parts, in their order, for a launch."""
+        return self._pointers
 
     def part_floats(self, v_dim: int) -> int:
         """float32 elements of the scratch for values `v_dim` wide: the rows' sums over the values, then their maxima and sums."""

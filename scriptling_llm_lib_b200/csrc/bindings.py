@@ -1703,16 +1703,13 @@ class GateKernels:
                                    _stream()), "softcap")
 
 
-def _one_device(what: str, **tensors):
-    """All of these on the current CUDA device (a launch goes to the current device's stream)."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise KernelError(f"{what}: {name} is on {t.device}; the kernels run on a CUDA device only")
-        if t.device.index != here:
-            raise KernelError(f"{what}: {name} is on {t.device} while cuda:{here} is the current device")
+def _one_device(what: str, *tensors) -> int:
+    """All of these on the current CUDA device (a launch goes to the current device's stream); its number."""
+    here = torch.cuda.current_device() if _current_device is None else _current_device() if torch.cuda.is_initialized() else -1
+    for t in tensors:
+        if t is not None and (t.get_device() != here or here < 0):
+            raise KernelError(f"{what}: a tensor is on {t.device}; all stand on the current CUDA device")
+    return here
 
 
 class SharedAttention:
@@ -1725,6 +1722,7 @@ class SharedAttention:
             raise KernelError(f"no kernels for {dtype}; supported: float32, bfloat16")
         self.dtype, self.suffix = dtype, _SUFFIX[dtype]
         self.lib = load_library(f"share_{self.suffix}")
+        self._shapes: dict[tuple, TileShape] = {}
         self._attn, self._merge = (getattr(self.lib, f"sllm_share_{n}_{self.suffix}") for n in ("attn", "merge"))
         self._attn_tc = load_library("attn_share_tcgen05").sllm_share_attn_tc_bf16 if dtype == torch.bfloat16 else None
         for fn in (self._attn, self._merge, self._attn_tc):
@@ -1768,24 +1766,22 @@ class SharedAttention:
                               f"{tuple(block_table.shape)} for {T} rows of {plan.n_seqs} sequences")
         if (sink is not None and tuple(sink.shape) != (H,)) or part.numel() < plan.part_floats(vd):
             raise KernelError(f"shared attention: a sink for each of {H} heads and a scratch of {plan.part_floats(vd)} floats")
-        _one_device("shared attention", q=q, out=out, positions=tok_pos, block_table=block_table, keys=kpages, values=vpages, plan=plan.dev,
-                    scratch=part, sink=sink, err_flag=err_flag)
-        shape = self.shape(hd, vd)
+        here = _one_device("shared attention", q, out, tok_pos, block_table, kpages, vpages, plan.dev, part, sink, err_flag)
+        shape = self._shapes.get((here, hd, vd)) or self._shapes.setdefault((here, hd, vd), self.shape(hd, vd))
         if plan.shape != shape:
             raise KernelError(f"shared attention: the plan is laid out for {plan.shape}, these widths want {shape}")
         if T == 0:
             return
         rows = plan.scratch_rows
-        thin = ((_ptr(plan.thin_first, torch.int32, "plan"),), (as_int(shape.thin_warps),)) if shape.halves else ((), ())
+        first, thin_first, items, toks, list_first, entries = plan.pointers()
+        thin = ((thin_first,), (as_int(shape.thin_warps),)) if shape.halves else ((), ())
         _check((self._attn_tc if shape.halves else self._attn)(
             c_void_p(q.data_ptr()), q.stride(0), _ptr(tok_pos, torch.int32, "tok_pos"), _ptr(block_table, torch.int32, "block_table"),
             block_table.shape[1], _ptr(kpages, self.dtype, "kpages"), _ptr(vpages, self.dtype, "vpages"), c_longlong(kpages.shape[0]),
-            _ptr(plan.first, torch.int32, "plan"), *thin[0], _ptr(plan.items, torch.int32, "plan"), _ptr(plan.toks, torch.int32, "plan"),
-            as_int(shape.workers), *thin[1], _ptr(part, torch.float32, "part"), c_longlong(rows), as_int(H), as_int(G), hd, vd, c_float(scale),
+            first, *thin[0], items, toks, as_int(shape.workers), *thin[1], _ptr(part, torch.float32, "part"), c_longlong(rows), as_int(H), as_int(G), hd, vd, c_float(scale),
             c_float(softcap or 0.0), _ptr(err_flag, torch.int32, "err_flag"), _stream()), "share_attn")
         _check(self._merge(
-            _ptr(part, torch.float32, "part"), c_longlong(rows), _ptr(plan.list_first, torch.int32, "plan"), _ptr(plan.list, torch.int32, "plan"),
-            _ptr(out, self.dtype, "out"), _ptr(sink, torch.float32, "sink"), as_int(T), as_int(H), as_int(G), vd, _stream()), "share_merge")
+            _ptr(part, torch.float32, "part"), c_longlong(rows), list_first, entries, _ptr(out, self.dtype, "out"), _ptr(sink, torch.float32, "sink"), as_int(T), as_int(H), as_int(G), vd, _stream()), "share_merge")
 
 
 class PageKernels:
@@ -1801,7 +1797,7 @@ class PageKernels:
         if n < 0 or tuple(dst.shape) != (n,) or (rows is not None and tuple(rows.shape) != (n,)):
             raise KernelError(f"{what}: ids {tuple(src.shape)} and {tuple(dst.shape)}"
                               + (f", rows {tuple(rows.shape)}" if rows is not None else "") + " are one list each, of equal lengths")
-        _one_device(what, src=src, dst=dst, rows=rows, err_flag=err_flag)
+        _one_device(what, src, dst, rows, err_flag)
         if n == 0:
             return
         for i in range(0, len(areas), self.AREAS):
@@ -1821,7 +1817,7 @@ class PageKernels:
         for a, b in pairs:
             if a.dim() != 5 or b.dim() != 5 or a.dtype != b.dtype or a.shape[0] != b.shape[0] or a.shape[2:] != b.shape[2:] or a.shape[3] != PAGE:
                 raise KernelError(f"copy_pages: storages {tuple(a.shape)} {a.dtype} and {tuple(b.shape)} {b.dtype}")
-            _one_device("copy_pages", storage=a, to=b)
+            _one_device("copy_pages", a, b)
             width, units, heads = a.element_size() * a.shape[4], a.shape[0], a.shape[2]
             if a.numel() and b.numel():
                 item = width * PAGE * heads
@@ -1835,7 +1831,7 @@ class PageKernels:
         for a, b in pairs:
             if a.dim() < 1 or a.dtype != b.dtype or a.shape[1:] != b.shape[1:]:
                 raise KernelError(f"copy_slots: tensors {tuple(a.shape)} {a.dtype} and {tuple(b.shape)} {b.dtype}")
-            _one_device("copy_slots", tensor=a, to=b)
+            _one_device("copy_slots", a, b)
             if a.numel() and b.numel():
                 item = a.element_size() * (a.numel() // a.shape[0])
                 areas.append((_ptr(a).value, _ptr(b).value, 0, 0, item, item, item, 1, 1, a.shape[0], b.shape[0]))
