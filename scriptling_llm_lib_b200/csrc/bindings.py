@@ -1744,7 +1744,10 @@ class SharedAttention:
             narrow = max(head_dim, v_dim) <= 64
             return TileShape(rows=256, workers=sm_count, halves=True, item_pages=6.0, half_cost=0.7, thin_rows=16, thin_warps=8 if narrow else 6,
                              thin_cost=0.35 if narrow else 0.5, thin_item=0.2, thin_start=4.0)                                                   # tcgen05, and mma.sync for thin tiles
-        return TileShape(rows=64, workers=2 * sm_count)
+        # FP32 FMA: two blocks on an SM where their rows of queries and weights and two pages fit twice
+        size, smem = (4 if self.dtype == torch.float32 else 2), 4 * 64 * (head_dim + 4 + 68)
+        smem += 2 * PAGE * (head_dim + v_dim + 32 // size) * size
+        return TileShape(rows=64, workers=(2 if smem <= 112 * 1024 else 1) * sm_count, min_pages=1)
 
     def attn(self, q, out, tok_pos, block_table, kpages, vpages, plan, part, scale, err_flag, softcap=None, sink=None):
         """out [T, H * vd] = attention of the step's queries q [T, H * hd or more] (rows may stand apart) at positions tok_pos over the

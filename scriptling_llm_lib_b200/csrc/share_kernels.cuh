@@ -13,39 +13,65 @@
 
 // ------------------------------------------------------------------ FP32 FMA tiles
 // A block of 256 threads: up to 64 rows (16 where a tile has no more: QPT 1) against a page of 64 keys at a time. Thread (ty = tid / 16,
-// tx = tid % 16) has rows QPT ty .. of the tile, keys 4 tx .. + 3 of the page's scores and the dims 4 (tx + 16 g) .. + 3 of the output.
-// Q and K stand in shared memory with their dims outermost, V and the weights by keys; 16-byte accesses. Bound by FMA issue and the
-// shared-memory reads that feed it (a 4 x 4 register tile: 32 bytes for 16 FMAs).
+// tx = tid % 16) has rows QPT ty .. of the tile, keys tx, tx + 16, .. of the page's scores and the dims 4 (tx + 16 g) .. + 3 of the
+// output. Queries, keys and values stand in shared memory as rows (keys and values as they are stored, rows padded by 16 bytes against
+// bank conflicts), the next page on its way by asynchronous copies while one is worked on, where two fit. Bound by FMA issue and the
+// shared-memory reads that feed it (a 4 x 4 register tile: 128 bytes for 64 FMAs); a tile of few rows by those reads alone.
 #define SF_ROWS 64
 #define SF_PS (SLLM_PAGE + 4)
 
+template <typename A>
+__host__ __device__ __forceinline__ int share_row_len(int width) { return width + 16 / (int)sizeof(A); }
+// bytes of shared memory with `stages` pages
+template <typename A>
+static inline size_t share_fma_smem(int hd, int vd, int stages) {
+  return ((size_t)SF_ROWS * (hd + 4) + (size_t)SF_ROWS * SF_PS) * 4 + (size_t)stages * SLLM_PAGE * (share_row_len<A>(hd) + share_row_len<A>(vd)) * sizeof(A);
+}
+// four elements from global to shared memory, or zeros
+template <typename A>
+__device__ __forceinline__ void share_copy4(A* to, const A* from, bool copy) {
+  const uint32_t dst = (uint32_t)__cvta_generic_to_shared(to);
+  if constexpr (sizeof(A) == 4) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(copy ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(from), "r"(copy ? 8 : 0) : "memory");
+}
+
 template <typename A, int NG, int QPT>
-__device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareItem& it, float* sm) {
-  constexpr int BQ = 16 * QPT;
-  const int hd = p.hd, vd = p.vd, rep = p.H / p.G, n_rows = it.n_tok * rep;
-  float* Qs = sm;                              // [hd][BQ]
-  float* Ks = Qs + hd * SF_ROWS;               // [hd][64]
-  float* Vs = Ks + hd * SLLM_PAGE;             // [64][vd]
-  float* Ps = Vs + SLLM_PAGE * vd;             // [BQ][68]
+__device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareItem& it, int stages, float* sm) {
+  const int hd = p.hd, vd = p.vd, rep = p.H / p.G, n_rows = it.n_tok * rep, kq = hd >> 2, vq = vd >> 2;
+  const int ql = hd + 4, kl = share_row_len<A>(hd), vl = share_row_len<A>(vd);
+  float* Qs = sm;                              // [64][ql]
+  float* Ps = Qs + SF_ROWS * ql;               // [64][68]
+  A* Ks = (A*)(Ps + SF_ROWS * SF_PS);          // [stages][64][kl]
+  A* Vs = Ks + stages * SLLM_PAGE * kl;        // [stages][64][vl]
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const A *kp = (const A*)p.kpages, *vp = (const A*)p.vpages;
-  const int kq = hd >> 2, vq = vd >> 2;
+  const int* row = p.block_table + (size_t)it.seq * p.max_pages;
 
-  for (int e = tid; e < BQ * kq; e += 256) {
-    const int r = e % BQ, d = e / BQ;
+  auto fetch = [&](int t) {                    // keys behind the last token, and a page that is none: zeros
+    const int page = share_page(p, row, t), n_keys = page < 0 ? 0 : min(SLLM_PAGE, it.last + 1 - t * SLLM_PAGE), s = (t - it.p0) % stages;
+    const size_t at = ((size_t)max(page, 0) * p.G + it.g) * SLLM_PAGE;
+    for (int e = tid; e < SLLM_PAGE * kq; e += 256) {
+      const int kk = e / kq, d = 4 * (e % kq);
+      share_copy4(Ks + (s * SLLM_PAGE + kk) * kl + d, kp + (at + kk) * hd + d, kk < n_keys);
+    }
+    for (int e = tid; e < SLLM_PAGE * vq; e += 256) {
+      const int kk = e / vq, d = 4 * (e % vq);
+      share_copy4(Vs + (s * SLLM_PAGE + kk) * vl + d, vp + (at + kk) * vd + d, kk < n_keys);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (it.p0 < it.p1) fetch(it.p0);
+  for (int e = tid; e < 16 * QPT * kq; e += 256) {
+    const int r = e / kq, d = 4 * (e % kq);
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < n_rows) v = ld4((const A*)p.q + (size_t)p.toks[it.tok0 + r / rep] * p.q_ld + (size_t)(it.g * rep + r % rep) * hd + 4 * d);
-    Qs[(4 * d + 0) * BQ + r] = v.x;
-    Qs[(4 * d + 1) * BQ + r] = v.y;
-    Qs[(4 * d + 2) * BQ + r] = v.z;
-    Qs[(4 * d + 3) * BQ + r] = v.w;
+    if (r < n_rows) v = ld4((const A*)p.q + (size_t)p.toks[it.tok0 + r / rep] * p.q_ld + (size_t)(it.g * rep + r % rep) * hd + d);
+    *(float4*)(Qs + r * ql + d) = v;
   }
   float m[QPT], l[QPT], o[QPT][NG][4];
   int qpos[QPT];
 #pragma unroll
   for (int i = 0; i < QPT; i++) {
-    const int r = ty * QPT + i;
-    qpos[i] = share_sees(it, r, rep);
+    qpos[i] = share_sees(it, ty * QPT + i, rep);
     m[i] = -INFINITY;
     l[i] = 0.f;
 #pragma unroll
@@ -53,64 +79,56 @@ __device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareIt
 #pragma unroll
       for (int c = 0; c < 4; c++) o[i][gg][c] = 0.f;
   }
-  const int* row = p.block_table + (size_t)it.seq * p.max_pages;
   for (int t = it.p0; t < it.p1; t++) {
-    const int page = share_page(p, row, t), n_keys = page < 0 ? 0 : min(SLLM_PAGE, it.last + 1 - t * SLLM_PAGE);
-    const size_t at = ((size_t)max(page, 0) * p.G + it.g) * SLLM_PAGE;
-    __syncthreads();
-    for (int e = tid; e < SLLM_PAGE * kq; e += 256) {
-      const int kk = e % SLLM_PAGE, d = e / SLLM_PAGE;
-      const float4 v = kk < n_keys ? ld4(kp + (at + kk) * hd + 4 * d) : make_float4(0.f, 0.f, 0.f, 0.f);
-      Ks[(4 * d + 0) * SLLM_PAGE + kk] = v.x;
-      Ks[(4 * d + 1) * SLLM_PAGE + kk] = v.y;
-      Ks[(4 * d + 2) * SLLM_PAGE + kk] = v.z;
-      Ks[(4 * d + 3) * SLLM_PAGE + kk] = v.w;
-    }
-    for (int e = tid; e < SLLM_PAGE * vq; e += 256) {
-      const int kk = e / vq, d = e % vq;
-      *(float4*)(Vs + kk * vd + 4 * d) = kk < n_keys ? ld4(vp + (at + kk) * vd + 4 * d) : make_float4(0.f, 0.f, 0.f, 0.f);
+    if (stages == 2 && t + 1 < it.p1) {
+      fetch(t + 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     __syncthreads();
+    const A *K = Ks + ((t - it.p0) % stages) * SLLM_PAGE * kl, *V = Vs + ((t - it.p0) % stages) * SLLM_PAGE * vl;
     float s[QPT][4];
 #pragma unroll
     for (int i = 0; i < QPT; i++)
 #pragma unroll
       for (int j = 0; j < 4; j++) s[i][j] = 0.f;
 #pragma unroll 4
-    for (int d = 0; d < hd; d++) {
-      float a[QPT];
-      if constexpr (QPT == 4) {
-        const float4 v = *(const float4*)(Qs + d * BQ + ty * 4);
-        a[0] = v.x; a[1] = v.y; a[2] = v.z; a[3] = v.w;
-      } else {
-        a[0] = Qs[d * BQ + ty];
-      }
-      const float4 kb = *(const float4*)(Ks + d * SLLM_PAGE + tx * 4);
-      const float kv[4] = {kb.x, kb.y, kb.z, kb.w};
+    for (int d = 0; d < hd; d += 4) {
+      float4 a[QPT], k[4];
+#pragma unroll
+      for (int i = 0; i < QPT; i++) a[i] = *(const float4*)(Qs + (ty * QPT + i) * ql + d);
+#pragma unroll
+      for (int j = 0; j < 4; j++) k[j] = ld4(K + (tx + 16 * j) * kl + d);
 #pragma unroll
       for (int i = 0; i < QPT; i++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) s[i][j] = fmaf(a[i], kv[j], s[i][j]);
+        for (int j = 0; j < 4; j++) {
+          s[i][j] = fmaf(a[i].x, k[j].x, s[i][j]);
+          s[i][j] = fmaf(a[i].y, k[j].y, s[i][j]);
+          s[i][j] = fmaf(a[i].z, k[j].z, s[i][j]);
+          s[i][j] = fmaf(a[i].w, k[j].w, s[i][j]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < QPT; i++) {
       float mx = -INFINITY;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const int key = 4 * tx + j;
         float v = s[i][j] * p.scale;
         if (p.softcap > 0.f) v = p.softcap * tanhf(v / p.softcap);
-        s[i][j] = key < n_keys && t * SLLM_PAGE + key <= qpos[i] ? v * SHARE_LOG2E : -INFINITY;
+        s[i][j] = t * SLLM_PAGE + tx + 16 * j <= qpos[i] ? v * SHARE_LOG2E : -INFINITY;
         mx = fmaxf(mx, s[i][j]);
       }
 #pragma unroll
       for (int off = 1; off < 16; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
       const float m_new = fmaxf(m[i], mx), corr = m_new == -INFINITY ? 1.f : exp2f(m[i] - m_new);
-      float pr[4], rs = 0.f;
+      float rs = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        pr[j] = s[i][j] == -INFINITY ? 0.f : exp2f(s[i][j] - m_new);
-        rs += pr[j];
+        const float pr = s[i][j] == -INFINITY ? 0.f : exp2f(s[i][j] - m_new);
+        rs += pr;
+        Ps[(ty * QPT + i) * SF_PS + tx + 16 * j] = pr;
       }
       l[i] = fmaf(l[i], corr, rs);                                      // this lane's share of the row's sum
       m[i] = m_new;
@@ -118,9 +136,8 @@ __device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareIt
       for (int gg = 0; gg < NG; gg++)
 #pragma unroll
         for (int c = 0; c < 4; c++) o[i][gg][c] *= corr;
-      *(float4*)(Ps + (ty * QPT + i) * SF_PS + tx * 4) = make_float4(pr[0], pr[1], pr[2], pr[3]);
     }
-    __syncthreads();
+    __syncwarp();                               // (a row's weights are read by the lanes that wrote them)
 #pragma unroll 2
     for (int k4 = 0; k4 < SLLM_PAGE; k4 += 4) {
       float pv[QPT][4];
@@ -135,7 +152,7 @@ __device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareIt
         if (d0 >= vd) continue;
 #pragma unroll
         for (int kk = 0; kk < 4; kk++) {
-          const float4 v = *(const float4*)(Vs + (k4 + kk) * vd + d0);
+          const float4 v = ld4(V + (k4 + kk) * vl + d0);
 #pragma unroll
           for (int i = 0; i < QPT; i++) {
             o[i][gg][0] = fmaf(pv[i][kk], v.x, o[i][gg][0]);
@@ -146,6 +163,8 @@ __device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareIt
         }
       }
     }
+    __syncthreads();                            // this page's place is free
+    if (stages == 1 && t + 1 < it.p1) fetch(t + 1);
   }
   float* ml = p.part + (size_t)p.part_rows * vd;
 #pragma unroll
@@ -171,15 +190,15 @@ __device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareIt
 }
 
 template <typename A, int NG>
-__global__ void __launch_bounds__(256) share_fma_kernel(ShareArgs p) {
+__global__ void __launch_bounds__(256) share_fma_kernel(ShareArgs p, int stages) {
   extern __shared__ __align__(16) float share_sm[];
   pdl_launch_dependents();
   pdl_wait();
   const int i1 = p.first[blockIdx.x + 1];
   for (int i = p.first[blockIdx.x]; i < i1; i++) {
     const ShareItem it = share_item(p, i);
-    if (it.n_tok * (p.H / p.G) <= 16) share_fma_item<A, NG, 1>(p, it, share_sm);
-    else share_fma_item<A, NG, 4>(p, it, share_sm);
+    if (it.n_tok * (p.H / p.G) <= 16) share_fma_item<A, NG, 1>(p, it, stages, share_sm);
+    else share_fma_item<A, NG, 4>(p, it, stages, share_sm);
   }
 }
 
