@@ -47,17 +47,13 @@ __device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareIt
   const A *kp = (const A*)p.kpages, *vp = (const A*)p.vpages;
   const int* row = p.block_table + (size_t)it.seq * p.max_pages;
 
+  // a thread's place in a row of four-element pieces, and its first row, of keys and of values
+  const int kd = 4 * (tid % kq), k0 = tid < 256 / kq * kq ? tid / kq : SLLM_PAGE, vd0 = 4 * (tid % vq), v0 = tid < 256 / vq * vq ? tid / vq : SLLM_PAGE;
   auto fetch = [&](int t) {                    // keys behind the last token, and a page that is none: zeros
     const int page = share_page(p, row, t), n_keys = page < 0 ? 0 : min(SLLM_PAGE, it.last + 1 - t * SLLM_PAGE), s = (t - it.p0) % stages;
     const size_t at = ((size_t)max(page, 0) * p.G + it.g) * SLLM_PAGE;
-    for (int e = tid; e < SLLM_PAGE * kq; e += 256) {
-      const int kk = e / kq, d = 4 * (e % kq);
-      share_copy4(Ks + (s * SLLM_PAGE + kk) * kl + d, kp + (at + kk) * hd + d, kk < n_keys);
-    }
-    for (int e = tid; e < SLLM_PAGE * vq; e += 256) {
-      const int kk = e / vq, d = 4 * (e % vq);
-      share_copy4(Vs + (s * SLLM_PAGE + kk) * vl + d, vp + (at + kk) * vd + d, kk < n_keys);
-    }
+    for (int kk = k0; kk < SLLM_PAGE; kk += 256 / kq) share_copy4(Ks + (s * SLLM_PAGE + kk) * kl + kd, kp + (at + kk) * hd + kd, kk < n_keys);
+    for (int kk = v0; kk < SLLM_PAGE; kk += 256 / vq) share_copy4(Vs + (s * SLLM_PAGE + kk) * vl + vd0, vp + (at + kk) * vd + vd0, kk < n_keys);
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
   if (it.p0 < it.p1) fetch(it.p0);
@@ -214,43 +210,48 @@ struct ShareMergeArgs {
   const float* sink;         // [H] or null
   int T, H, G, vd;
 };
-// With SPLIT the four warps of a block take every fourth run of entries of one output each and meet in shared memory: where outputs are
-// few, the chain of an output's loads (four entries at a time, a microsecond each) is what the kernel lasts.
+// With SPLIT the eight warps of a block share an output's entries and meet in shared memory: where outputs are few, the chain of an output's
+// loads (a microsecond for every four entries) is what the kernel lasts.
+#define SHARE_MERGE_WARPS 8
 template <typename A, int RB, int NQ, bool SPLIT>
-__global__ void __launch_bounds__(128) share_merge_kernel(ShareMergeArgs p) {
+__global__ void __launch_bounds__(32 * SHARE_MERGE_WARPS) share_merge_kernel(ShareMergeArgs p) {
   pdl_launch_dependents();
   pdl_wait();
-  constexpr int J = 32 / RB;                        // entries held at a time
-  __shared__ float4 met[SPLIT ? 3 : 1][NQ][32];
+  constexpr int J = 32 / RB, W = SHARE_MERGE_WARPS, MET = SPLIT ? W : 1;      // J: entries that a warp holds at a time
+  __shared__ float4 met[MET][NQ][32];
+  __shared__ float2 met_ml[MET][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = p.H / RB;
-  const long long w = SPLIT ? (long long)blockIdx.x : (long long)blockIdx.x * 4 + warp;
+  const long long w = SPLIT ? (long long)blockIdx.x : (long long)blockIdx.x * W + warp;
   if (w >= (long long)p.T * per) return;
   const int j = lane / RB, t = (int)(w / per), h = (int)(w % per) * RB + lane % RB, rep = p.H / p.G, g = h / rep, r = h % rep;
   const int i0 = p.list_first[(size_t)t * p.G + g], n = p.list_first[(size_t)t * p.G + g + 1] - i0;
+  // lane (j, .) holds entry base + j * apart: the warps of an output take its entries in turn
+  constexpr int apart = SPLIT ? W : 1, step = apart * J;
+  const int first = SPLIT ? warp : 0;
   const float2* ml = (const float2*)(p.part + (size_t)p.part_rows * p.vd);
-  const float sink = p.sink ? p.sink[h] * SHARE_LOG2E : -INFINITY;
-  int at = j < n ? p.list[i0 + j] + r : 0;
-  float2 v = j < n ? ml[at] : make_float2(-INFINITY, 0.f);
+  // ---- the largest score of this warp's entries; the first of them stay at hand
+  int at = first + j * apart < n ? p.list[i0 + first + j * apart] + r : 0;
+  float2 v = first + j * apart < n ? ml[at] : make_float2(-INFINITY, 0.f);
   float M = v.x;
-  for (int i = j + J; i < n; i += J) M = fmaxf(M, ml[p.list[i0 + i] + r].x);
+#pragma unroll 4
+  for (int i = first + step + j * apart; i < n; i += step) M = fmaxf(M, ml[p.list[i0 + i] + r].x);
 #pragma unroll
   for (int d = RB; d < 32; d <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-  M = fmaxf(M, sink);
   const float M0 = M == -INFINITY ? 0.f : M;                    // (nothing seen: every weight below is 2^-inf = 0)
   float den = 0.f;
   float4 a[NQ];
 #pragma unroll
   for (int k = 0; k < NQ; k++) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int base = 0; base < n; base += J) {
-    if (base) {
-      at = base + j < n ? p.list[i0 + base + j] + r : 0;
-      v = base + j < n ? ml[at] : make_float2(-INFINITY, 0.f);
+  for (int base = first; base < n; base += step) {
+    if (base != first) {
+      at = base + j * apart < n ? p.list[i0 + base + j * apart] + r : 0;
+      v = base + j * apart < n ? ml[at] : make_float2(-INFINITY, 0.f);
     }
     // an entry none of whose keys this row sees, or none at all, weighs 0 and its values are not read; a sum that is NaN spoils the row
     const float wgt = v.y != v.y ? v.y : exp2f(v.x - M0);
     if (wgt != 0.f) den = fmaf(wgt, v.y, den);
-    const int m = min(J, n - base);
-    for (int e0 = SPLIT ? 4 * warp : 0; e0 < m; e0 += SPLIT ? 16 : 4) {
+    const int m = min(J, (n - base + apart - 1) / apart);
+    for (int e0 = 0; e0 < m; e0 += 4) {
       float c[4];
       float4 x[4][NQ];
 #pragma unroll
@@ -278,29 +279,45 @@ __global__ void __launch_bounds__(128) share_merge_kernel(ShareMergeArgs p) {
   }
 #pragma unroll
   for (int d = RB; d < 32; d <<= 1) den += __shfl_xor_sync(0xffffffffu, den, d);
-  if (p.sink) den += exp2f(sink - M0);
-  if constexpr (SPLIT) {                            // (every warp has the whole of den)
-    if (warp > 0)
+  // ---- the warps' sums, and the sink's share
+  const float sink = p.sink ? p.sink[h] * SHARE_LOG2E : -INFINITY;
+  float top = fmaxf(M, sink);
+  if constexpr (SPLIT) {
+    met_ml[warp][lane] = make_float2(M, den);
 #pragma unroll
-      for (int k = 0; k < NQ; k++) met[warp - 1][k][lane] = a[k];
+    for (int k = 0; k < NQ; k++) met[warp][k][lane] = a[k];
     __syncthreads();
-    if (warp > 0) return;
+    if (warp >= NQ) return;                         // warp k adds the dims that the lanes hold under k
 #pragma unroll
-    for (int o = 0; o < 3; o++)
-#pragma unroll
-      for (int k = 0; k < NQ; k++) {
-        const float4 b = met[o][k][lane];
-        a[k].x += b.x;
-        a[k].y += b.y;
-        a[k].z += b.z;
-        a[k].w += b.w;
-      }
+    for (int o = 0; o < W; o++) top = fmaxf(top, met_ml[o][lane].x);
   }
-  const float inv = den > 0.f || den != den ? 1.0f / den : 0.f;
+  const float top0 = top == -INFINITY ? 0.f : top;
+  float all = p.sink ? exp2f(sink - top0) : 0.f;
   A* out = (A*)p.out + ((size_t)t * p.H + h) * p.vd;
+  if constexpr (SPLIT) {
+    float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int k = 0; k < NQ; k++) {
-    const int d = 4 * (j + k * J);
-    if (d < p.vd) st4(out + d, make_float4(a[k].x * inv, a[k].y * inv, a[k].z * inv, a[k].w * inv));
+    for (int o = 0; o < W; o++) {
+      const float2 e = met_ml[o][lane];
+      const float c = e.x == -INFINITY && e.y == 0.f ? 0.f : exp2f((e.x == -INFINITY ? 0.f : e.x) - top0);
+      const float4 x = met[o][warp][lane];
+      all = fmaf(c, e.y, all);
+      b.x = fmaf(c, x.x, b.x);
+      b.y = fmaf(c, x.y, b.y);
+      b.z = fmaf(c, x.z, b.z);
+      b.w = fmaf(c, x.w, b.w);
+    }
+    const float inv = all > 0.f || all != all ? 1.0f / all : 0.f;
+    const int d = 4 * (j + warp * J);
+    if (d < p.vd) st4(out + d, make_float4(b.x * inv, b.y * inv, b.z * inv, b.w * inv));
+  } else {
+    const float c = exp2f(M0 - top0);
+    all = fmaf(c, den, all);
+    const float inv = all > 0.f || all != all ? c / all : 0.f;
+#pragma unroll
+    for (int k = 0; k < NQ; k++) {
+      const int d = 4 * (j + k * J);
+      if (d < p.vd) st4(out + d, make_float4(a[k].x * inv, a[k].y * inv, a[k].z * inv, a[k].w * inv));
+    }
   }
 }
