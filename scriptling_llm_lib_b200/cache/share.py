@@ -14,6 +14,7 @@ rows' partial results in a scratch buffer; a list says which of them belong to a
 from __future__ import annotations
 
 import ctypes
+import struct
 from dataclasses import dataclass
 
 import numpy as np
@@ -128,8 +129,8 @@ class SharePlan:
                 self.n_rows * self.n_kv + 1, c.entries]
 
     def host(self) -> np.ndarray:
-        """The buffer's words: where each block's items begin, where each of its warps' thin items do, the items, the tokens in the tree's order, where each token and
-        key/value head's entries begin, the entries (rows of the scratch)."""
+        """The buffer's words: where each block's items begin, where each of its warps' thin items do, the items, the tokens in the tree's
+        order, where each token and key/value head's entries begin, the entries (rows of the scratch)."""
         sizes, p = self._sizes(), self.parts
         out, off = np.zeros(sum(sizes), dtype=np.int32), 0
         for n, part in zip(sizes, (p["first"], p["thin_first"], p["items"].ravel(), p["toks"], p["list_first"], p["list"])):
@@ -143,11 +144,11 @@ class SharePlan:
             views.append(self.dev[at:at + n])
             at += n
         self.first, self.thin_first, self.items, self.toks, self.list_first, self.list = views
-        self._pointers = tuple(ctypes.c_void_p(v.data_ptr()) for v in views)
-
-    def pointers(self):
-        """Addresses of the buffer's parts, in their order, for a launch."""
-        return self._pointers
+        # what the kernels' launchers read (SharePlanDev): six addresses, then the scratch's rows and the sizes
+        s = self.shape
+        self._struct = ctypes.create_string_buffer(struct.pack("6q q 5i 4x", *(v.data_ptr() for v in views), self.scratch_rows, self.n_rows, self.n_heads,
+                                                               self.n_kv, s.workers, s.thin_warps))
+        self.address = ctypes.addressof(self._struct)
 
     def part_floats(self, v_dim: int) -> int:
         """float32 elements of the scratch for values `v_dim` wide: the rows' sums over the values, then their maxima and sums."""

@@ -20,7 +20,7 @@
 // rounding; their sum is taken before it), O rescaled only when a row's maximum has outgrown its reference by 2^8. Warps whose rows are all past the tile's end pass the barriers and
 // compute nothing. Waits are bounded (2 s), after which the kernel raises *err, lets its copies land, frees its tensor memory and returns.
 #include "attn_tcgen05.cuh"
-#include "share_plan.cuh"
+#include "share_merge.cuh"
 #include <type_traits>
 
 #define FS_THREADS 384       // warp 0: TMA, warps 1-2: the products of either half, warp 3: queries, warps 4-7 and 8-11: softmax of either half
@@ -766,29 +766,21 @@ static int fs_launch(const CUtensorMap& mk, const CUtensorMap& mv, const ShareAr
   return (int)sllm_launch(attn_share_kernel<KD, VD, STAGES>, dim3(workers), dim3(FS_THREADS), smem, stream, mk, mv, a, (uint32_t)smem);
 }
 
-// first [workers + 1], thin_first [workers * thin_warps + 1], items [.][8], toks [T]: a plan's for tiles of 256 rows in halves, with thin
-// ones of at most FS_THIN rows; part: part_rows * (vd + 2) floats.
-SLLM_EXPORT int sllm_share_attn_tc_bf16(const void* q, int q_ld, const int* tok_pos, const int* block_table, int max_pages, const void* kpages,
-                                        const void* vpages, long long n_pages, const int* first, const int* thin_first, const int* items,
-                                        const int* toks, int workers, int thin_warps, float* part, long long part_rows, int H, int G, int hd, int vd, float scale, float softcap,
-                                        int* err, cudaStream_t stream) {
-  if (workers <= 0) return 0;
-  if (hd < 8 || hd > 128 || hd % 8 || vd < 8 || vd > 128 || vd % 8 || G < 1 || H < 1 || H % G != 0 || H / G > 2 * FS_ROWS || q_ld < H * hd || (q_ld & 7) ||
-      n_pages < 1 || n_pages > 0x7fffffffLL || (long long)G * FS_BK > 0x7fffffffLL || part_rows < 1 || part_rows % 32 || max_pages < 1 ||
-      ((uintptr_t)q & 15) || ((uintptr_t)kpages & 15) || ((uintptr_t)vpages & 15) || ((uintptr_t)part & 15) || ((uintptr_t)items & 15))
+// The plan is one for tiles of 256 rows in halves, with thin ones of at most FS_THIN rows; part: plan->part_rows * (vd + 2) floats.
+SLLM_EXPORT int sllm_share_attn_tc_bf16(const SharePlanDev* plan, const void* q, int q_ld, const int* tok_pos, const int* block_table,
+                                        int max_pages, const void* kpages, const void* vpages, long long n_pages, float* part, void* out,
+                                        const float* sink, int hd, int vd, float scale, float softcap, int* err, cudaStream_t stream) {
+  if (hd < 8 || hd > 128 || hd % 8 || vd < 8 || vd > 128 || vd % 8 || (q_ld & 7) || !share_call_ok(*plan, 2 * FS_ROWS, q_ld, hd, n_pages, max_pages, part) ||
+      plan->thin_warps != (hd <= 64 && vd <= 64 ? fs_thin_warps<64, 64>() : fs_thin_warps<128, 128>()) || !share_aligned(q, 16) ||
+      !share_aligned(kpages, 16) || !share_aligned(vpages, 16) || !share_aligned(out, 16))
     return SLLM_ERR_ARG;
-  ShareArgs a{q, q_ld, tok_pos, block_table, max_pages, kpages, vpages, (int)n_pages, first, thin_first, items, toks, part, part_rows, H, G, hd, vd, scale,
-              softcap, err};
+  if (plan->T == 0) return 0;
+  const ShareArgs a = share_args(*plan, q, q_ld, tok_pos, block_table, max_pages, kpages, vpages, n_pages, part, hd, vd, scale, softcap, err);
   CUtensorMap mk, mv;
-  int rc = fs_make_map(&mk, kpages, n_pages, G, hd);
+  int rc = fs_make_map(&mk, kpages, n_pages, plan->G, hd);
+  if (rc == 0) rc = fs_make_map(&mv, vpages, n_pages, plan->G, vd);
   if (rc) return rc;
-  rc = fs_make_map(&mv, vpages, n_pages, G, vd);
-  if (rc) return rc;
-  if (thin_warps != (hd <= 64 && vd <= 64 ? fs_thin_warps<64, 64>() : fs_thin_warps<128, 128>())) return SLLM_ERR_ARG;
-  if (vd <= 64) {
-    if (hd <= 64) return fs_launch<64, 64, 10>(mk, mv, a, workers, stream);
-    return fs_launch<128, 64, 6>(mk, mv, a, workers, stream);
-  }
-  if (hd <= 64) return fs_launch<64, 128, 7>(mk, mv, a, workers, stream);
-  return fs_launch<128, 128, 5>(mk, mv, a, workers, stream);
+  if (vd <= 64) rc = hd <= 64 ? fs_launch<64, 64, 10>(mk, mv, a, plan->workers, stream) : fs_launch<128, 64, 6>(mk, mv, a, plan->workers, stream);
+  else rc = hd <= 64 ? fs_launch<64, 128, 7>(mk, mv, a, plan->workers, stream) : fs_launch<128, 128, 5>(mk, mv, a, plan->workers, stream);
+  return rc ? rc : share_merge_run<bf16>(*plan, part, out, sink, vd, stream);
 }

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
 from itertools import chain
 from operator import index as as_int      # a caller's number as the int it stands for; what is none (None, a float) is refused
@@ -1712,6 +1713,15 @@ def _one_device(what: str, *tensors) -> int:
     return here
 
 
+def _address(t, dtype) -> int:
+    """The address of a tensor that the caller has found on the device; of a contiguous one of this type."""
+    if t is None:
+        return 0
+    if t.dtype is not dtype or not t.is_contiguous():
+        raise KernelError(f"a {'contiguous ' if not t.is_contiguous() else ''}tensor of {dtype} is needed, not {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
 class SharedAttention:
     """Attention of a step whose sequences share pages, each shared run of pages read once for all that share it; any number of new
     tokens a sequence. `shape` says how the kernel for these widths wants its plan (cache/share.py), `attn` runs it."""
@@ -1723,11 +1733,12 @@ class SharedAttention:
         self.dtype, self.suffix = dtype, _SUFFIX[dtype]
         self.lib = load_library(f"share_{self.suffix}")
         self._shapes: dict[tuple, TileShape] = {}
-        self._attn, self._merge = (getattr(self.lib, f"sllm_share_{n}_{self.suffix}") for n in ("attn", "merge"))
+        self._attn = getattr(self.lib, f"sllm_share_attn_{self.suffix}")
         self._attn_tc = load_library("attn_share_tcgen05").sllm_share_attn_tc_bf16 if dtype == torch.bfloat16 else None
-        for fn in (self._attn, self._merge, self._attn_tc):
-            if fn is not None:
-                fn.restype = c_int
+        p, n = c_void_p, c_int
+        for fn in (self._attn, self._attn_tc):
+            if fn is not None:      # (addresses and sizes go over as plain integers: half the price of an object for each)
+                fn.restype, fn.argtypes = c_int, [p, p, n, p, p, n, p, p, c_longlong, p, p, p, n, n, c_float, c_float, p, p]
 
     @staticmethod
     def takes(head_dim: int, v_dim: int, rep: int = 1) -> bool:
@@ -1756,35 +1767,30 @@ class SharedAttention:
         elements. `softcap`: a score s becomes softcap * tanh(s / softcap) before the softmax; `sink` float32 [H]: exp(sink[h]) joins
         head h's denominator with no key and no value. A page id outside the storage or a position outside the table sets err_flag."""
         H, G, T = plan.n_heads, plan.n_kv, plan.n_rows
-        if kpages.dim() != 4 or vpages.dim() != 4 or kpages.shape[:3] != vpages.shape[:3] or tuple(kpages.shape[1:3]) != (G, PAGE):
-            raise KernelError(f"shared attention: pages {tuple(kpages.shape)} and {tuple(vpages.shape)} for {G} key/value heads")
-        hd, vd = kpages.shape[3], vpages.shape[3]
-        if not self.takes(hd, vd, H // G):
-            raise KernelError(f"shared attention takes widths in multiples of 4 up to 256 and up to {self.MAX_REP} query heads on a key/value "
-                              f"head, not keys of {hd}, values of {vd} and {H} heads on {G}")
-        if q.dim() != 2 or q.shape[0] != T or q.shape[1] < H * hd or (q.stride(1) != 1 and q.shape[1] > 1) or q.stride(0) % 4 or q.dtype != self.dtype:
-            raise KernelError(f"shared attention: queries {tuple(q.shape)} {q.dtype} (row stride {q.stride(0)}) for {T} rows of {H} heads of {hd}")
-        if tuple(out.shape) != (T, H * vd) or tuple(tok_pos.shape) != (T,) or block_table.dim() != 2 or block_table.shape[0] < plan.n_seqs:
-            raise KernelError(f"shared attention: out {tuple(out.shape)}, positions {tuple(tok_pos.shape)} and block table "
-                              f"{tuple(block_table.shape)} for {T} rows of {plan.n_seqs} sequences")
-        if (sink is not None and tuple(sink.shape) != (H,)) or part.numel() < plan.part_floats(vd):
-            raise KernelError(f"shared attention: a sink for each of {H} heads and a scratch of {plan.part_floats(vd)} floats")
+        ks, vs, qs = kpages.shape, vpages.shape, q.shape
+        if len(ks) != 4 or len(vs) != 4 or ks[:3] != vs[:3] or ks[1] != G or ks[2] != PAGE:
+            raise KernelError(f"shared attention: pages {tuple(ks)} and {tuple(vs)} for {G} key/value heads")
+        hd, vd = ks[3], vs[3]
         here = _one_device("shared attention", q, out, tok_pos, block_table, kpages, vpages, plan.dev, part, sink, err_flag)
         shape = self._shapes.get((here, hd, vd)) or self._shapes.setdefault((here, hd, vd), self.shape(hd, vd))
+        if H // G > self.MAX_REP:
+            raise KernelError(f"shared attention takes up to {self.MAX_REP} query heads on a key/value head, not {H} on {G}")
+        ld, step = q.stride()
+        if len(qs) != 2 or qs[0] != T or qs[1] < H * hd or step != 1 or ld % 4 or q.dtype != self.dtype:
+            raise KernelError(f"shared attention: queries {tuple(qs)} {q.dtype} (row stride {ld}) for {T} rows of {H} heads of {hd}")
+        if out.shape != (T, H * vd) or tok_pos.shape != (T,) or block_table.dim() != 2 or block_table.shape[0] < plan.n_seqs:
+            raise KernelError(f"shared attention: out {tuple(out.shape)}, positions {tuple(tok_pos.shape)} and block table "
+                              f"{tuple(block_table.shape)} for {T} rows of {plan.n_seqs} sequences")
+        if (sink is not None and sink.shape != (H,)) or part.numel() < plan.part_floats(vd):
+            raise KernelError(f"shared attention: a sink for each of {H} heads and a scratch of {plan.part_floats(vd)} floats")
         if plan.shape != shape:
             raise KernelError(f"shared attention: the plan is laid out for {plan.shape}, these widths want {shape}")
-        if T == 0:
-            return
-        rows = plan.scratch_rows
-        first, thin_first, items, toks, list_first, entries = plan.pointers()
-        thin = ((thin_first,), (as_int(shape.thin_warps),)) if shape.halves else ((), ())
+        laid_out = plan.address
+        LAUNCHES[0] += 1            # (two kernels: the tiles' and the one that joins what they leave)
         _check((self._attn_tc if shape.halves else self._attn)(
-            c_void_p(q.data_ptr()), q.stride(0), _ptr(tok_pos, torch.int32, "tok_pos"), _ptr(block_table, torch.int32, "block_table"),
-            block_table.shape[1], _ptr(kpages, self.dtype, "kpages"), _ptr(vpages, self.dtype, "vpages"), c_longlong(kpages.shape[0]),
-            first, *thin[0], items, toks, as_int(shape.workers), *thin[1], _ptr(part, torch.float32, "part"), c_longlong(rows), as_int(H), as_int(G), hd, vd, c_float(scale),
-            c_float(softcap or 0.0), _ptr(err_flag, torch.int32, "err_flag"), _stream()), "share_attn")
-        _check(self._merge(
-            _ptr(part, torch.float32, "part"), c_longlong(rows), list_first, entries, _ptr(out, self.dtype, "out"), _ptr(sink, torch.float32, "sink"), as_int(T), as_int(H), as_int(G), vd, _stream()), "share_merge")
+            laid_out, q.data_ptr(), ld, _address(tok_pos, torch.int32), _address(block_table, torch.int32), block_table.shape[1],
+            _address(kpages, self.dtype), _address(vpages, self.dtype), ks[0], _address(part, torch.float32), _address(out, self.dtype),
+            _address(sink, torch.float32), hd, vd, c_float(scale), c_float(softcap or 0.0), _address(err_flag, torch.int32), _stream()), "share_attn")
 
 
 class PageKernels:
@@ -1793,22 +1799,22 @@ class PageKernels:
 
     def __init__(self):
         self.lib = load_library("pages")
-        self.lib.sllm_page_copy.restype = c_int
+        fn = self.lib.sllm_page_copy
+        fn.restype, fn.argtypes = c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p]
 
     def _copy(self, what, areas, src, dst, rows, max_rows, err_flag):
         n = src.shape[0] if src.dim() == 1 else -1
-        if n < 0 or tuple(dst.shape) != (n,) or (rows is not None and tuple(rows.shape) != (n,)):
+        if n < 0 or dst.shape != (n,) or (rows is not None and rows.shape != (n,)):
             raise KernelError(f"{what}: ids {tuple(src.shape)} and {tuple(dst.shape)}"
                               + (f", rows {tuple(rows.shape)}" if rows is not None else "") + " are one list each, of equal lengths")
         _one_device(what, src, dst, rows, err_flag)
         if n == 0:
             return
+        lists = (_address(src, torch.int32), _address(dst, torch.int32), _address(rows, torch.int32))
         for i in range(0, len(areas), self.AREAS):
             some = areas[i:i + self.AREAS]
-            words = (c_longlong * (11 * len(some)))(*chain.from_iterable(some))
-            _check(self.lib.sllm_page_copy(words, len(some), _ptr(src, torch.int32, "src"), _ptr(dst, torch.int32, "dst"),
-                                           _ptr(rows, torch.int32, "rows"), n, as_int(max_rows), _ptr(err_flag, torch.int32, "err_flag"),
-                                           _stream()), what)
+            words = struct.pack(f"{11 * len(some)}q", *chain.from_iterable(some))
+            _check(self.lib.sllm_page_copy(words, len(some), *lists, n, as_int(max_rows), _address(err_flag, torch.int32), _stream()), what)
 
     def copy_pages(self, pairs, src, dst, rows, err_flag):
         """For every (a, b) of `pairs`, storages [units, pages, kv heads, 64, width] of one layout (the same tensor, or another number of
@@ -1818,14 +1824,15 @@ class PageKernels:
         outside 0..64, sets err_flag, and that pair is not copied."""
         areas = []
         for a, b in pairs:
-            if a.dim() != 5 or b.dim() != 5 or a.dtype != b.dtype or a.shape[0] != b.shape[0] or a.shape[2:] != b.shape[2:] or a.shape[3] != PAGE:
-                raise KernelError(f"copy_pages: storages {tuple(a.shape)} {a.dtype} and {tuple(b.shape)} {b.dtype}")
+            sa, sb = a.shape, b.shape
+            if len(sa) != 5 or len(sb) != 5 or a.dtype != b.dtype or sa[0] != sb[0] or sa[2:] != sb[2:] or sa[3] != PAGE:
+                raise KernelError(f"copy_pages: storages {tuple(sa)} {a.dtype} and {tuple(sb)} {b.dtype}")
             _one_device("copy_pages", a, b)
-            width, units, heads = a.element_size() * a.shape[4], a.shape[0], a.shape[2]
-            if a.numel() and b.numel():
-                item = width * PAGE * heads
-                areas.append((_ptr(a).value, _ptr(b).value, item * a.shape[1], item * b.shape[1], item, width * PAGE, width, units, heads,
-                              a.shape[1], b.shape[1]))
+            units, pages, heads, _, width = sa
+            row = a.element_size() * width
+            if units and heads and width and pages and sb[1]:
+                areas.append((_address(a, a.dtype), _address(b, a.dtype), row * PAGE * heads * pages, row * PAGE * heads * sb[1], row * PAGE * heads,
+                              row * PAGE, row, units, heads, pages, sb[1]))
         self._copy("copy_pages", areas, src, dst, rows, PAGE, err_flag)
 
     def copy_slots(self, pairs, src, dst, err_flag):
@@ -1837,7 +1844,7 @@ class PageKernels:
             _one_device("copy_slots", a, b)
             if a.numel() and b.numel():
                 item = a.element_size() * (a.numel() // a.shape[0])
-                areas.append((_ptr(a).value, _ptr(b).value, 0, 0, item, item, item, 1, 1, a.shape[0], b.shape[0]))
+                areas.append((_address(a, a.dtype), _address(b, a.dtype), 0, 0, item, item, item, 1, 1, a.shape[0], b.shape[0]))
         self._copy("copy_slots", areas, src, dst, None, 1, err_flag)
 
 

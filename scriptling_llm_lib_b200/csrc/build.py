@@ -35,7 +35,7 @@ LIBRARIES: dict[str, tuple[str, tuple[str, ...]]] = {
     "gemm_split": ("gemm_split_tcgen05.cu", ("common.cuh", "tcgen05.cuh")),
     "gemm_tcgen05": ("gemm_tcgen05.cu", ("common.cuh", "tcgen05.cuh")),
     "attn_prefill_tcgen05": ("attn_prefill_tcgen05.cu", ("common.cuh", "tcgen05.cuh", "attn_tcgen05.cuh")),
-    "attn_share_tcgen05": ("attn_share_tcgen05.cu", ("common.cuh", "tcgen05.cuh", "attn_tcgen05.cuh", "share_plan.cuh")),
+    "attn_share_tcgen05": ("attn_share_tcgen05.cu", ("common.cuh", "tcgen05.cuh", "attn_tcgen05.cuh", "share_plan.cuh", "share_merge.cuh")),
     "attn_prefill_mma": ("attn_prefill_mma.cu", ("common.cuh",)),
     "chunk_tcgen05": ("chunk_tcgen05.cu", ("common.cuh", "tcgen05.cuh", "split_mma.cuh")),
     "latent_mma": ("latent_mma.cu", ("common.cuh",)),
@@ -46,8 +46,8 @@ LIBRARIES: dict[str, tuple[str, tuple[str, ...]]] = {
     "ssd_f32": ("lib_ssd_f32.cu", ("common.cuh", "tcgen05.cuh", "state_step.cuh", "ssd_kernels.cuh", "ssd_launchers.inc")),
     "ssd_bf16": ("lib_ssd_bf16.cu", ("common.cuh", "tcgen05.cuh", "state_step.cuh", "ssd_kernels.cuh", "ssd_launchers.inc")),
     "pages": ("lib_pages.cu", ("common.cuh",)),
-    "share_f32": ("lib_share_f32.cu", ("common.cuh", "share_plan.cuh", "share_kernels.cuh", "share_launchers.inc")),
-    "share_bf16": ("lib_share_bf16.cu", ("common.cuh", "share_plan.cuh", "share_kernels.cuh", "share_launchers.inc")),
+    "share_f32": ("lib_share_f32.cu", ("common.cuh", "share_plan.cuh", "share_merge.cuh", "share_kernels.cuh", "share_launchers.inc")),
+    "share_bf16": ("lib_share_bf16.cu", ("common.cuh", "share_plan.cuh", "share_merge.cuh", "share_kernels.cuh", "share_launchers.inc")),
     "gate_f32": ("lib_gate_f32.cu", ("common.cuh", "gate_kernels.cuh", "gate_launchers.inc")),
     "gate_bf16": ("lib_gate_bf16.cu", ("common.cuh", "gate_kernels.cuh", "gate_launchers.inc")),
 }

@@ -5,6 +5,13 @@
 #define SHARE_LOG2E 1.4426950408889634f
 #define SHARE_ERR_PAGE 5          // what *err says: a page id outside the storage, or a position outside the block table
 
+// A plan on the device, as the host hands it over: one for every call that goes by it
+struct SharePlanDev {
+  const int *first, *thin_first, *items, *toks, *list_first, *list;
+  long long part_rows;
+  int T, H, G, workers, thin_warps;
+};
+
 struct ShareArgs {
   const void* q;             // [T, q_ld] queries that have their positions; head h at columns h * hd
   int q_ld;
@@ -95,4 +102,18 @@ __device__ __noinline__ float4 share_sum_by_key(const ShareArgs& p, const ShareI
     acc.w = fmaf(w, x.w, acc.w);
   }
   return acc;
+}
+
+// ------------------------------------------------------------------ host side
+static inline bool share_aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+static inline bool share_call_ok(const SharePlanDev& plan, int rows, int q_ld, int hd, long long n_pages, int max_pages, const float* part) {
+  return plan.T >= 0 && plan.G >= 1 && plan.H >= 1 && plan.H % plan.G == 0 && plan.H / plan.G <= rows && plan.workers >= 1 && plan.part_rows >= 1 &&
+         plan.part_rows % 32 == 0 && (long long)plan.T * plan.H <= 0x7fffffffLL && q_ld >= plan.H * hd && n_pages >= 1 && n_pages <= 0x7fffffffLL &&
+         (long long)plan.G * SLLM_PAGE <= 0x7fffffffLL && max_pages >= 1 && share_aligned(part, 16) && share_aligned(plan.items, 16);
+}
+static inline ShareArgs share_args(const SharePlanDev& plan, const void* q, int q_ld, const int* tok_pos, const int* block_table, int max_pages,
+                                   const void* kpages, const void* vpages, long long n_pages, float* part, int hd, int vd, float scale,
+                                   float softcap, int* err) {
+  return ShareArgs{q, q_ld, tok_pos, block_table, max_pages, kpages, vpages, (int)n_pages, plan.first, plan.thin_first, plan.items, plan.toks, part,
+                   plan.part_rows, plan.H, plan.G, hd, vd, scale, softcap, err};
 }
