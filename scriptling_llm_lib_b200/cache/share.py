@@ -83,12 +83,38 @@ def share_tree(table: np.ndarray, whole: np.ndarray):
     return order, nodes, np.asarray(own, dtype=np.int64)
 
 
-def share_pays(tree, held, new) -> bool:
-    """Whether a step of these sequences is faster by the tree than each sequence for itself."""
-    if tree is None:
+def share_pays(tree, held, new, n_heads: int, n_kv: int, width: int, floats: bool) -> bool:
+    """Whether a step of these sequences is estimated to be faster by the tree than each sequence for itself; `width`: of a key and a
+    value together. Measured on 148 SMs, each for itself / by the tree, us:
+    bfloat16, a token each (bound by the bytes: 25 MB more are 4 us, and the rotation and the cache write become a kernel of their
+    own): 32 heads of 64 on 8, 8 sequences behind 1,000 tokens 12.5 / 13.3 (14 MB saved), 32 behind 1,000 18.8 / 15.5 (61), 8 behind
+    16,000 41 / 20 (229), 64 behind 300 11.7 / 18.4 (33); 32 heads of 128 on 8, 64 behind 300 24 / 24 (66).
+    32-bit, a token each: each for itself costs a row, head and page 2.1 ns, the tree a key/value head of a sequence 75 ns and a
+    tile's page 17: 32 heads of 64 on 8, 64 behind 1,000 72 / 80, 16 behind 4,000 77 / 49; on 32, 64 behind 1,000 110 / 178.
+    Runs of tokens: tiles of 128 rows (64 in 32-bit) of a sequence and head, 4 ns a page (24) but no less than the 0.7 us (7) that a page
+    takes one tile, against tiles of 256 (64) rows of a node and key/value head, 7.5 ns a page (17), and 50 ns an item: bfloat16, 32 heads of
+    64 on 8, 16 of 20 tokens behind 300 18 / 22, behind 2,000 58 / 29, 8 of 60 behind 2,000 32 / 28; 16 of 150 behind 300 29 / 38,
+    behind 8,000 312 / 173."""
+    if tree is None or not tree[1]:
         return False
-    saved = sum((hi - lo - 1) * (b - a) for lo, hi, a, b in tree[1])
-    return saved > 0
+    order, nodes, own = tree
+    held, new = np.asarray(held, dtype=np.int64)[order], np.asarray(new, dtype=np.int64)[order]
+    rep, pages = n_heads // n_kv, (held + new - 1) // PAGE + 1
+    ends = np.concatenate([[0], np.cumsum(new)])
+    if new.max() <= 1:
+        if not floats:
+            saved = sum((int(ends[hi] - ends[lo]) - 1) * (b - a) for lo, hi, a, b in nodes)
+            return saved * n_kv * PAGE * width * 2 >= 48e6
+        alone = 8.0 + 0.0021 * n_heads * float(pages[new > 0].sum())
+        tiles = sum(-(-int(ends[hi] - ends[lo]) * rep // 64) * (b - a) for lo, hi, a, b in nodes)
+        return 1.4 * (14.0 + 0.075 * n_kv * int(new.sum()) + 0.017 * n_kv * tiles) * width / 128 < alone * width / 128
+    rows, page, wide_rows, wide_page, item = (64, 0.024, 64, 0.017, 0.05) if floats else (128, 0.0042, 256, 0.0075, 0.05)
+    scale = width / 128 if floats else 0.4 + 0.6 * width / 128
+    alone = max(scale * page * n_heads * float((-(-new // rows) * pages).sum()), scale * (7.0 if floats else 0.7) * int(pages.max())) + 4.0
+    by_tree = 14.0 + item * n_kv * int((-(-new * rep // wide_rows)).sum())
+    by_tree += scale * wide_page * n_kv * float((-(-new * rep // wide_rows) * (pages - own)).sum())
+    by_tree += scale * wide_page * n_kv * sum(-(-int(ends[hi] - ends[lo]) * rep // wide_rows) * (b - a) for lo, hi, a, b in nodes)
+    return by_tree < 0.9 * alone
 
 
 class SharePlan:

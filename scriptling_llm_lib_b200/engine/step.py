@@ -234,7 +234,7 @@ class Engine:
         self.cache = SequenceCache(self.model.cache_needs(), self.model.state_needs(), n_slots, n_pages, self.dtype,
                                    self.device)
         self.cache.err_flag = self.err_flag
-        self._sharing: list[int] | None = None
+        self._sharing: list[tuple[int, int, int]] | None = None
         self.max_positions = min(self.layout.max_positions, n_pages * PAGE)
         self.model.prepare(self.max_positions, self.device)
         padded = 1
@@ -327,10 +327,11 @@ class Engine:
         cache = self.cache
         if not cache.shares_pages or len(slots) < 2:
             return False
-        return any(cache.groups[g].pool.n_shared and share_pays(cache.share_tree(g, slots), held, new) for g in self._share_groups())
+        return any(cache.groups[g].pool.n_shared and share_pays(cache.share_tree(g, slots), held, new, heads, cache.groups[g].need.kv_heads, width,
+                                                                self.dtype == torch.float32) for g, heads, width in self._share_groups())
 
-    def _share_groups(self) -> list[int]:
-        """Cache groups with layers whose attention can read shared pages once."""
+    def _share_groups(self) -> list[tuple[int, int, int]]:
+        """Cache groups with layers whose attention can read shared pages once: (group, query heads, widths of a key and a value)."""
         if self._sharing is None:
             groups, ops = set(), self.kernels.shared
             for e in self.layout.schedule:
@@ -340,7 +341,7 @@ class Engine:
                 for part in self.model.blocks[e.layer].parts():
                     heads = part.shares_pages() if isinstance(part, Mixer) else None
                     if heads is not None and ops.takes(heads[1], heads[2], heads[0] // self.cache.groups[g].need.kv_heads):
-                        groups.add(g)
+                        groups.add((g, heads[0], heads[1] + heads[2]))
             self._sharing = sorted(groups)
         return self._sharing
 

@@ -36,6 +36,13 @@ def engine(tmp_path, raw, dtype, max_tokens=8192, max_seqs=32, **kw):
     return Engine.from_folder(f"random:{path}:3", dtype, max_tokens=max_tokens, max_seqs=max_seqs, **kw)
 
 
+@pytest.fixture(autouse=True)
+def shares_whatever_it_costs(monkeypatch, request):
+    """The tests' models are too small for shared reading to pay: here it does wherever sequences share a page."""
+    if "by_the_estimate" not in request.node.name:
+        monkeypatch.setattr("scriptling_llm_lib_b200.engine.step.share_pays", lambda tree, *a: bool(tree and tree[1]))
+
+
 def rel_err(got, want):
     return _rel_err(got.cpu(), want.cpu())
 
@@ -161,6 +168,21 @@ def test_compaction_leaves_sequences_as_they_are(tmp_path, dtype):
             eng.compact(wrong)
     go_on(7)
     for s in tokens:
+        s.close()
+
+
+def test_a_step_shares_by_the_estimate_alone(tmp_path):
+    """A tiny model's forks go on by the steps they had; with the weight of a long context the estimate turns."""
+    from scriptling_llm_lib_b200.cache import share_pays
+    eng = engine(tmp_path, LLAMA, "bfloat16")
+    root = eng.open()
+    eng.step([StepEntry(root, random_ids(900, LLAMA["vocab_size"], 1))])
+    seqs = [root] + root.fork(5)
+    eng.step([StepEntry(s, [i]) for i, s in enumerate(seqs)])
+    assert [k[2] for k in eng.decode_graphs.graphs] == [False]
+    tree = eng.cache.share_tree(0, [s.slot for s in seqs])
+    assert not share_pays(tree, [901] * 6, [1] * 6, 4, 2, 128, False) and share_pays(tree, [901] * 6, [1] * 6, 128, 128, 256, False)
+    for s in seqs:
         s.close()
 
 

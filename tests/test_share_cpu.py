@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from scriptling_llm_lib_b200.cache import (PAGE, CacheFull, CacheNeed, FreeList, PlanCapacity, SequenceCache, SharePlan, StateNeed, TileShape,
-                                           pages_for, share_tree)
+                                           pages_for, share_pays, share_tree)
 from scriptling_llm_lib_b200.csrc import bindings
 from scriptling_llm_lib_b200.engine.generate import Generator, plan_batches, request_pages, shared_runs
 
@@ -294,6 +294,23 @@ def test_equal_page_ids_are_shared_only_where_both_hold_the_whole_page():
     assert (own[list(order).index(0)], sorted(own.tolist())) == (4, [4, 10, 10]) and len(nodes) == 2
     assert share_tree(table, np.asarray([0, 0, 0]))[1] == []
     assert share_tree(np.full((3, 10), -1, dtype=np.int32), np.asarray([5, 5, 5]))[1] == []
+
+
+def test_which_steps_read_shared_pages_once():
+    """Around the lines that the measurements draw (bfloat16 / 32-bit, tokens each, 32 heads of 64)."""
+    def pays(n, prefix, new, kv, floats, own=100, groups=1):
+        pages = pages_for(prefix + own + new)
+        table = np.arange(n * pages, dtype=np.int32).reshape(n, pages)
+        table[:, :prefix // PAGE] = np.arange(prefix // PAGE) + 10 ** 6
+        held = np.full(n, prefix + own)
+        return share_pays(share_tree(table, held // PAGE), held, [new] * n, 32, kv, 128, floats)
+    assert [pays(8, p, 1, 8, False) for p in (300, 1000, 4000, 16000)] == [False, False, True, True]
+    assert [pays(n, 1000, 1, 32, False) for n in (2, 4, 16, 64)] == [False, False, True, True]
+    assert [pays(n, 4000, 1, 8, True) for n in (2, 16, 64)] == [False, True, True]
+    assert [pays(64, p, 1, 32, True) for p in (300, 1000)] == [False, False]
+    assert [pays(16, p, 20, 8, False) for p in (100, 2000, 8000)] == [False, True, True]
+    assert [pays(16, p, 150, 8, False) for p in (300, 8000)] == [False, True] and pays(4, 600, 30, 8, True)
+    assert not share_pays(None, [1], [1], 4, 4, 128, False) and not pays(1, 8000, 1, 8, False)
 
 
 # --------------------------------------------------------------------------- prompts that begin alike
