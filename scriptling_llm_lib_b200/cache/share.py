@@ -83,11 +83,12 @@ def share_tree(table: np.ndarray, whole: np.ndarray):
     return order, nodes, np.asarray(own, dtype=np.int64)
 
 
-def share_pays(tree, held, new, n_heads: int, n_kv: int, width: int, floats: bool) -> bool:
+def share_pays(tree, held, new, n_heads: int, n_kv: int, width: int, floats: bool, layers: int = 0) -> bool:
     """Whether a step of these sequences is estimated to be faster by the tree than each sequence for itself; `width`: of a key and a
-    value together. Measured on 148 SMs, each for itself / by the tree, us:
-    bfloat16, a token each (bound by the bytes: 25 MB more are 4 us, and the rotation and the cache write become a kernel of their
-    own): 32 heads of 64 on 8, 8 sequences behind 1,000 tokens 12.5 / 13.3 (14 MB saved), 32 behind 1,000 18.8 / 15.5 (61), 8 behind
+    value together; `layers`: those that go by a plan made for this step alone (0: the plan is kept for more steps), which costs the host
+    about 1.2 ms. Measured on 148 SMs, each for itself / by the tree, us:
+    bfloat16, a token each (bound by the bytes, and the rotation and the cache write become a kernel of their own: in whole steps the
+    line is between 50 and 100 MB saved a layer): 32 heads of 64 on 8, 8 sequences behind 1,000 tokens 12.5 / 13.3 (14 MB saved), 32 behind 1,000 18.8 / 15.5 (61), 8 behind
     16,000 41 / 20 (229), 64 behind 300 11.7 / 18.4 (33); 32 heads of 128 on 8, 64 behind 300 24 / 24 (66).
     32-bit, a token each: each for itself costs a row, head and page 2.1 ns, the tree a key/value head of a sequence 75 ns and a
     tile's page 17: 32 heads of 64 on 8, 64 behind 1,000 72 / 80, 16 behind 4,000 77 / 49; on 32, 64 behind 1,000 110 / 178.
@@ -101,17 +102,18 @@ def share_pays(tree, held, new, n_heads: int, n_kv: int, width: int, floats: boo
     held, new = np.asarray(held, dtype=np.int64)[order], np.asarray(new, dtype=np.int64)[order]
     rep, pages = n_heads // n_kv, (held + new - 1) // PAGE + 1
     ends = np.concatenate([[0], np.cumsum(new)])
+    by_plan = (1200.0 + 0.1 * n_kv * int(ends[-1])) / layers if layers else 0.0
     if new.max() <= 1:
         if not floats:
             saved = sum((int(ends[hi] - ends[lo]) - 1) * (b - a) for lo, hi, a, b in nodes)
-            return saved * n_kv * PAGE * width * 2 >= 48e6
+            return saved * n_kv * PAGE * width * 2 >= 80e6 + (by_plan * 6.5e6 if layers else 0.0)
         alone = 8.0 + 0.0021 * n_heads * float(pages[new > 0].sum())
         tiles = sum(-(-int(ends[hi] - ends[lo]) * rep // 64) * (b - a) for lo, hi, a, b in nodes)
-        return 1.4 * (14.0 + 0.075 * n_kv * int(new.sum()) + 0.017 * n_kv * tiles) * width / 128 < alone * width / 128
+        return (1.4 * (14.0 + 0.075 * n_kv * int(new.sum()) + 0.017 * n_kv * tiles) - alone) * width / 128 + by_plan < 0.0
     rows, page, wide_rows, wide_page, item = (64, 0.024, 64, 0.017, 0.05) if floats else (128, 0.0042, 256, 0.0075, 0.05)
     scale = width / 128 if floats else 0.4 + 0.6 * width / 128
     alone = max(scale * page * n_heads * float((-(-new // rows) * pages).sum()), scale * (7.0 if floats else 0.7) * int(pages.max())) + 4.0
-    by_tree = 14.0 + item * n_kv * int((-(-new * rep // wide_rows)).sum())
+    by_tree = 14.0 + by_plan + item * n_kv * int((-(-new * rep // wide_rows)).sum())
     by_tree += scale * wide_page * n_kv * float((-(-new * rep // wide_rows) * (pages - own)).sum())
     by_tree += scale * wide_page * n_kv * sum(-(-int(ends[hi] - ends[lo]) * rep // wide_rows) * (b - a) for lo, hi, a, b in nodes)
     return by_tree < 0.9 * alone

@@ -234,7 +234,7 @@ class Engine:
         self.cache = SequenceCache(self.model.cache_needs(), self.model.state_needs(), n_slots, n_pages, self.dtype,
                                    self.device)
         self.cache.err_flag = self.err_flag
-        self._sharing: list[tuple[int, int, int]] | None = None
+        self._sharing: dict[tuple[int, int, int], int] | None = None
         self.max_positions = min(self.layout.max_positions, n_pages * PAGE)
         self.model.prepare(self.max_positions, self.device)
         padded = 1
@@ -321,19 +321,21 @@ class Engine:
         self.model.prepare(self.max_positions, self.device)
         return moved
 
-    def _shares(self, slots, held, new) -> bool:
+    def _shares(self, slots, held, new, kept: bool = False) -> bool:
         """Whether a step of these sequences is to go by the plans of `SharedStep`: pages that it need not read again are worth the
-        partial results that reading them once leaves."""
+        partial results that reading them once leaves, and, unless a captured step keeps it, the plan."""
         cache = self.cache
         if not cache.shares_pages or len(slots) < 2:
             return False
         return any(cache.groups[g].pool.n_shared and share_pays(cache.share_tree(g, slots), held, new, heads, cache.groups[g].need.kv_heads, width,
-                                                                self.dtype == torch.float32) for g, heads, width in self._share_groups())
+                                                                self.dtype == torch.float32, 0 if kept else layers)
+                   for (g, heads, width), layers in self._share_groups().items())
 
-    def _share_groups(self) -> list[tuple[int, int, int]]:
-        """Cache groups with layers whose attention can read shared pages once: (group, query heads, widths of a key and a value)."""
+    def _share_groups(self) -> dict[tuple[int, int, int], int]:
+        """Cache groups with layers whose attention can read shared pages once: (group, query heads, widths of a key and a value) ->
+        how many such layers a step goes through."""
         if self._sharing is None:
-            groups, ops = set(), self.kernels.shared
+            groups, ops = {}, self.kernels.shared
             for e in self.layout.schedule:
                 g = self.cache.group_of_unit.get(e.cache_unit)
                 if g is None or self.cache.groups[g].need.kind != "full":
@@ -341,8 +343,9 @@ class Engine:
                 for part in self.model.blocks[e.layer].parts():
                     heads = part.shares_pages() if isinstance(part, Mixer) else None
                     if heads is not None and ops.takes(heads[1], heads[2], heads[0] // self.cache.groups[g].need.kv_heads):
-                        groups.add((g, heads[0], heads[1] + heads[2]))
-            self._sharing = sorted(groups)
+                        key = (g, heads[0], heads[1] + heads[2])
+                        groups[key] = groups.get(key, 0) + 1
+            self._sharing = groups
         return self._sharing
 
     def tickets(self, n: int) -> torch.Tensor:
@@ -405,7 +408,7 @@ class Engine:
         if self.use_graphs and T == B:
             slots = [e.sequence.slot for e in entries]
             tables = [self.cache.block_table(g, slots) for g in range(len(self.cache.groups))]
-            logits = self.decode_graphs.run(ids, pos0, slots, tables, self._shares(slots, pos0, lens))
+            logits = self.decode_graphs.run(ids, pos0, slots, tables, self._shares(slots, pos0, lens, kept=True))
             self.last_step = self.decode_graphs.last_index
             # the captured step's own buffer is overwritten by the next replay: the caller gets a copy
             if want_rows != list(range(B)):
@@ -506,7 +509,7 @@ class Engine:
         slots = [s.slot for s in sequences]
         tables = [self.cache.block_table(g, slots) for g in range(len(self.cache.groups))]
         held = [s.length for s in sequences]
-        logits = self.decode_graphs.run(ids.contiguous(), held, slots, tables, self._shares(slots, held, [1] * len(slots)))
+        logits = self.decode_graphs.run(ids.contiguous(), held, slots, tables, self._shares(slots, held, [1] * len(slots), kept=True))
         self.last_step = self.decode_graphs.last_index
         self.cache.advance(growth)
         return logits

@@ -298,18 +298,19 @@ def test_equal_page_ids_are_shared_only_where_both_hold_the_whole_page():
 
 def test_which_steps_read_shared_pages_once():
     """Around the lines that the measurements draw (bfloat16 / 32-bit, tokens each, 32 heads of 64)."""
-    def pays(n, prefix, new, kv, floats, own=100, groups=1):
+    def pays(n, prefix, new, kv, floats, own=100, layers=0):
         pages = pages_for(prefix + own + new)
         table = np.arange(n * pages, dtype=np.int32).reshape(n, pages)
         table[:, :prefix // PAGE] = np.arange(prefix // PAGE) + 10 ** 6
         held = np.full(n, prefix + own)
-        return share_pays(share_tree(table, held // PAGE), held, [new] * n, 32, kv, 128, floats)
-    assert [pays(8, p, 1, 8, False) for p in (300, 1000, 4000, 16000)] == [False, False, True, True]
-    assert [pays(n, 1000, 1, 32, False) for n in (2, 4, 16, 64)] == [False, False, True, True]
+        return share_pays(share_tree(table, held // PAGE), held, [new] * n, 32, kv, 128, floats, layers)
+    assert [pays(8, p, 1, 8, False) for p in (300, 1000, 4000, 16000)] == [False, False, False, True]
+    assert [pays(n, 1000, 1, 32, False) for n in (2, 4, 32, 64)] == [False, False, True, True]
     assert [pays(n, 4000, 1, 8, True) for n in (2, 16, 64)] == [False, True, True]
     assert [pays(64, p, 1, 32, True) for p in (300, 1000)] == [False, False]
     assert [pays(16, p, 20, 8, False) for p in (100, 2000, 8000)] == [False, True, True]
     assert [pays(16, p, 150, 8, False) for p in (300, 8000)] == [False, True] and pays(4, 600, 30, 8, True)
+    assert [pays(8, 4000, 20, 32, False, layers=n) for n in (0, 1, 24)] == [True, False, False] and pays(32, 4000, 20, 8, False, layers=24)
     assert not share_pays(None, [1], [1], 4, 4, 128, False) and not pays(1, 8000, 1, 8, False)
 
 
