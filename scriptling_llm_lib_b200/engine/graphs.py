@@ -152,7 +152,7 @@ class DecodeGraphs:
 
     def __init__(self, engine):
         self.engine = engine
-        self.graphs: dict[tuple[int, int, bool], DecodeGraph] = {}
+        self.graphs: dict[tuple, DecodeGraph] = {}
         self.pool = torch.cuda.graph_pool_handle() if torch.cuda.is_available() else None
         self.last_index = None
         self.last_graph: DecodeGraph | None = None
@@ -166,7 +166,7 @@ class DecodeGraphs:
         cap = -(-self.engine.max_positions // PAGE)
         width = min(max(8, _next_pow2(need)), max(cap, need))
         batch = _next_pow2(ids.shape[0] if isinstance(ids, torch.Tensor) else len(ids))
-        key = (batch, width, shared)
+        key = (batch, width, "shared") if shared else (batch, width)
         g = self.graphs.pop(key, None)
         if g is None:
             while len(self.graphs) >= self.MAX_GRAPHS:
