@@ -1726,6 +1726,7 @@ class SharedAttention:
     """Attention of a step whose sequences share pages, each shared run of pages read once for all that share it; any number of new
     tokens a sequence. `shape` says how the kernel for these widths wants its plan (cache/share.py), `attn` runs it."""
     MAX_REP = 64         # query heads on a key/value head
+    SCRATCH_BYTES = 1 << 28      # of partial results that an engine's step takes at most (a plan that needs more is not used)
 
     def __init__(self, dtype: torch.dtype):
         if dtype not in _SUFFIX:

@@ -162,7 +162,10 @@ class SharedStep:
         if key not in self.plans:
             need, ops = self.engine.cache.groups[group].need, self.engine.kernels.shared
             takes = need.kind == "full" and ops.takes(head_dim, v_dim, n_heads // need.kv_heads)
-            self.plans[key] = self._build(key) if takes else None
+            plan = self._build(key) if takes else None
+            if plan is not None and 4 * plan.part_floats(v_dim) > ops.SCRATCH_BYTES:       # a long prompt step of many heads
+                plan = None
+            self.plans[key] = plan
         return self.plans[key]
 
     def _build(self, key, device=True):

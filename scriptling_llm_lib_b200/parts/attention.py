@@ -66,7 +66,7 @@ import math
 import torch
 
 from ..cache.needs import CacheNeed
-from ..csrc.bindings import DecodeKernels, KernelSet, PrefillAttentionMMA, PrefillAttentionTC, gate_aligned
+from ..csrc.bindings import DecodeKernels, KernelSet, PrefillAttentionMMA, PrefillAttentionTC, SharedAttention, gate_aligned
 from ..cache.needs import StateNeed
 from ..weights.spec import TensorSpec
 from .base import MIXERS, POSITION_ENCODINGS, Folded, Mixer, PartSpec
@@ -308,6 +308,12 @@ class Attention(Mixer):
 
     def shares_pages(self):
         return None if self.span else (self.n_heads, self.head_dim, self.v_dim)
+
+    def scratch_bytes(self, rows):
+        """The partial results of attention over pages that a step's sequences share."""
+        widths = self.shares_pages()
+        takes = widths is not None and SharedAttention.takes(widths[1], widths[2], self.n_heads // self.n_kv_heads)
+        return SharedAttention.SCRATCH_BYTES if takes else 0
 
     def _share_plan(self, ctx, unit):
         """The step's plan where its sequences share pages and this layer sees all of them."""

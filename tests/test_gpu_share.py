@@ -156,6 +156,34 @@ def test_capped_scores_and_sinks(dtype, layout):
         c.check(c.run(**options), **options)
 
 
+@pytest.mark.parametrize("layout", [(48, 1, 64, 64), (64, 1, 128, 128), (64, 1, 32, 32), (40, 2, 16, 200)], ids=str)
+@pytest.mark.parametrize("dtype", [F, B16], ids=["f32", "bf16"])
+def test_many_query_heads_on_a_key_value_head(dtype, layout):
+    c = Case("nested", layout, dtype, seed=9)
+    c.check(c.run())
+    c = Case("runs", layout, dtype, seed=9)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("dtype", [F, B16], ids=["f32", "bf16"])
+def test_more_items_than_a_block_or_a_warp_holds_at_a_time(dtype):
+    """Over 64 tiles a block and over 32 thin ones a warp."""
+    c = Case([(path(("a", 2)) if i % 3 else path(), 128 + i % 70, 1) for i in range(620)], (64, 64, 16, 16), dtype, seed=4)
+    plan = c.plan()
+    assert max(np.diff(plan.parts["first"]).max(), np.diff(plan.parts["thin_first"]).max(initial=0)) > 32
+    c.check(c.run(plan))
+    c = Case([(path(("a", 1)), 64 + i % 3, 5 + i % 2) for i in range(150)], (64, 16, 24, 24), dtype, seed=4)      # 20 and 24 rows: not thin
+    plan = c.plan()
+    assert dtype == F or np.diff(plan.parts["first"]).max() > 8
+    c.check(c.run(plan))
+
+
+@pytest.mark.parametrize("dtype", [F, B16], ids=["f32", "bf16"])
+def test_a_step_of_no_tokens_writes_nothing(dtype):
+    c = Case([(path(("a", 3)), 200, 0), (path(("a", 3)), 210, 0)], (16, 4, 64, 64), dtype)
+    assert c.run().shape == (0, 1024)
+
+
 @pytest.mark.parametrize("dtype", [F, B16], ids=["f32", "bf16"])
 def test_rows_that_stand_apart_and_the_same_result_again(dtype):
     c = Case("nested", (16, 4, 64, 64), dtype, q_extra=72)
