@@ -39,7 +39,7 @@ class TileShape:
     workers: int
     halves: bool = False
     item_pages: float = 1.0      # what an item costs beside its pages, in pages
-    half_cost: float = 1.0       # what a page of a tile of at most half the rows costs, a full tile's page being 1
+    costs: tuple = ()            # (rows, what a page of a tile of at most so many rows costs), fewest rows first; a full tile's is 1
     min_pages: int = 2           # an item is not cut to fewer
     thin_rows: int = 0
     thin_warps: int = 0
@@ -88,10 +88,11 @@ def share_pays(tree, held, new, n_heads: int, n_kv: int, width: int, floats: boo
     value together; `layers`: those that go by a plan made for this step alone (0: the plan is kept for more steps), which costs the host
     about 1.2 ms. Measured on 148 SMs, each for itself / by the tree, us:
     bfloat16, a token each (bound by the bytes, and the rotation and the cache write become a kernel of their own: in whole steps the
-    line is between 50 and 100 MB saved a layer): 32 heads of 64 on 8, 8 sequences behind 1,000 tokens 12.5 / 13.3 (14 MB saved), 32 behind 1,000 18.8 / 15.5 (61), 8 behind
-    16,000 41 / 20 (229), 64 behind 300 11.7 / 18.4 (33); 32 heads of 128 on 8, 64 behind 300 24 / 24 (66).
-    32-bit, a token each: each for itself costs a row, head and page 2.1 ns, the tree a key/value head of a sequence 75 ns and a
-    tile's page 17: 32 heads of 64 on 8, 64 behind 1,000 72 / 80, 16 behind 4,000 77 / 49; on 32, 64 behind 1,000 110 / 178.
+    line is between 50 and 100 MB saved a layer): 32 heads of 64 on 8, 8 sequences behind 1,000 tokens 12.5 / 13.3 (14 MB saved), 32
+    behind 1,000 18.8 / 15.5 (61), 8 behind 16,000 41 / 20 (229), 64 behind 300 11.7 / 18.4 (33); 32 heads of 128 on 8, 64 behind 300
+    24 / 24 (66).
+    32-bit, a token each: each for itself costs a row, head and page 2.1 ns, the tree a key/value head of a sequence 56 ns and a
+    tile's page 24: 32 heads of 64 on 8, 64 behind 1,000 72 / 59, 16 behind 4,000 77 / 43; on 32, 64 behind 1,000 110 / 117.
     Runs of tokens: tiles of 128 rows (64 in 32-bit) of a sequence and head, 4 ns a page (24) but no less than the 0.7 us (7) that a page
     takes one tile, against tiles of 256 (64) rows of a node and key/value head, 7.5 ns a page (17), and 50 ns an item: bfloat16, 32 heads of
     64 on 8, 16 of 20 tokens behind 300 18 / 22, behind 2,000 58 / 29, 8 of 60 behind 2,000 32 / 28; 16 of 150 behind 300 29 / 38,
@@ -109,7 +110,7 @@ def share_pays(tree, held, new, n_heads: int, n_kv: int, width: int, floats: boo
             return saved * n_kv * PAGE * width * 2 >= 80e6 + (by_plan * 6.5e6 if layers else 0.0)
         alone = 8.0 + 0.0021 * n_heads * float(pages[new > 0].sum())
         tiles = sum(-(-int(ends[hi] - ends[lo]) * rep // 64) * (b - a) for lo, hi, a, b in nodes)
-        return (1.4 * (14.0 + 0.075 * n_kv * int(new.sum()) + 0.017 * n_kv * tiles) - alone) * width / 128 + by_plan < 0.0
+        return (1.4 * (14.0 + 0.04 * n_kv * int(new.sum()) + 0.017 * n_kv * tiles) - alone) * width / 128 + by_plan < 0.0
     rows, page, wide_rows, wide_page, item = (64, 0.024, 64, 0.017, 0.05) if floats else (128, 0.0042, 256, 0.0075, 0.05)
     scale = width / 128 if floats else 0.4 + 0.6 * width / 128
     alone = max(scale * page * n_heads * float((-(-new // rows) * pages).sum()), scale * (7.0 if floats else 0.7) * int(pages.max())) + 4.0
@@ -287,7 +288,10 @@ def _lay_out(order, nodes, own, held, new, rep: int, n_kv: int, shape: TileShape
     t_pages = t_end - page[s]
     thin = t_n * rep <= shape.thin_rows
     half = (t_n * rep <= shape.rows // 2) & ~thin if shape.halves else np.zeros(len(s), dtype=bool)
-    cost = t_pages * np.where(half, shape.half_cost, 1.0) + shape.item_pages
+    cost = np.ones(len(s))
+    for rows, page_cost in reversed(shape.costs):
+        cost[t_n * rep <= rows] = page_cost
+    cost = t_pages * cost + shape.item_pages
     cost[thin] = t_pages[thin] * shape.thin_cost + shape.thin_item
     # ---- a tile for every key/value head, the thin ones behind the others
     by = np.argsort(thin, kind="stable")

@@ -11,8 +11,8 @@
 //
 // Tiles of at most 16 rows (one token of a sequence's own pages, as a rule) are thin: 128 rows of tensor memory would be filled for a few.
 // They come behind the others, when the ring and its roles are done: each warp has its own list, fetches keys and values by TMA into
-// two or three buffers of its own and computes with mma.sync (16 rows fill one tile), so that six or eight chains run side by side and
-// memory is what bounds them. A plan gives every block its share of either kind.
+// two or three buffers of its own and computes with mma.sync, so that six to eight chains run side by side and memory is what
+// bounds them. A plan gives every block its share of either kind.
 //
 // Rows of a tile belong to several sequences and stand anywhere in the step, so a warp gathers them (16 bytes a lane, asynchronously,
 // into the 128-byte swizzle) where keys and values come by TMA, a page and head at a time. S = Q K^T (128 x 64) and O += P V as
@@ -59,7 +59,7 @@ __device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
 
 // warps with thin tiles, and the buffers (a page of keys or of values) that each has
 template <int KD, int VD>
-__host__ __device__ constexpr int fs_thin_warps() { return KD <= 64 && VD <= 64 ? 8 : 6; }
+__host__ __device__ constexpr int fs_thin_warps() { return KD <= 64 && VD <= 64 ? 8 : KD > 64 && VD > 64 ? 7 : 6; }
 template <int KD, int VD>
 __host__ __device__ constexpr int fs_thin_bufs() { return KD <= 64 && VD <= 64 ? 3 : 2; }
 
@@ -771,7 +771,7 @@ SLLM_EXPORT int sllm_share_attn_tc_bf16(const SharePlanDev* plan, const void* q,
                                         int max_pages, const void* kpages, const void* vpages, long long n_pages, float* part, void* out,
                                         const float* sink, int hd, int vd, float scale, float softcap, int* err, cudaStream_t stream) {
   if (hd < 8 || hd > 128 || hd % 8 || vd < 8 || vd > 128 || vd % 8 || (q_ld & 7) || !share_call_ok(*plan, 2 * FS_ROWS, q_ld, hd, n_pages, max_pages, part) ||
-      plan->thin_warps != (hd <= 64 && vd <= 64 ? fs_thin_warps<64, 64>() : fs_thin_warps<128, 128>()) || !share_aligned(q, 16) ||
+      plan->thin_warps != (hd <= 64 && vd <= 64 ? fs_thin_warps<64, 64>() : hd > 64 && vd > 64 ? fs_thin_warps<128, 128>() : fs_thin_warps<128, 64>()) || !share_aligned(q, 16) ||
       !share_aligned(kpages, 16) || !share_aligned(vpages, 16) || !share_aligned(out, 16))
     return SLLM_ERR_ARG;
   if (plan->T == 0) return 0;

@@ -1753,13 +1753,16 @@ class SharedAttention:
         if sm_count is None:
             sm_count = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
         if self.dtype == torch.bfloat16 and all(w % 8 == 0 and w <= 128 for w in (head_dim, v_dim)):
+            # tcgen05, and mma.sync for thin tiles. What an item and a thin page cost beside a page of 256 rows (1.05 us): measured
+            # over decode steps of 2 to 64 sequences and prompts of 16 to 64; half or twice of each is 3 to 20% slower
             narrow = max(head_dim, v_dim) <= 64
-            return TileShape(rows=256, workers=sm_count, halves=True, item_pages=6.0, half_cost=0.7, thin_rows=16, thin_warps=8 if narrow else 6,
-                             thin_cost=0.35 if narrow else 0.5, thin_item=0.2, thin_start=4.0)                                                   # tcgen05, and mma.sync for thin tiles
+            return TileShape(rows=256, workers=sm_count, halves=True, item_pages=6.0, costs=((128, 0.7),), thin_rows=16,
+                             thin_warps=8 if narrow else 7 if min(head_dim, v_dim) > 64 else 6, thin_cost=0.35 if narrow else 0.5, thin_item=0.2,
+                             thin_start=4.0)
         # FP32 FMA: two blocks on an SM where their rows of queries and weights and two pages fit twice
         size, smem = (4 if self.dtype == torch.float32 else 2), 4 * 64 * (head_dim + 4 + 68)
         smem += 2 * PAGE * (head_dim + v_dim + 32 // size) * size
-        return TileShape(rows=64, workers=(2 if smem <= 112 * 1024 else 1) * sm_count, min_pages=1)
+        return TileShape(rows=64, workers=(2 if smem <= 112 * 1024 else 1) * sm_count, costs=((4, 0.25), (16, 0.5)), min_pages=1)
 
     def attn(self, q, out, tok_pos, block_table, kpages, vpages, plan, part, scale, err_flag, softcap=None, sink=None):
         """out [T, H * vd] = attention of the step's queries q [T, H * hd or more] (rows may stand apart) at positions tok_pos over the

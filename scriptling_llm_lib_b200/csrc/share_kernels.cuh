@@ -185,15 +185,151 @@ __device__ __forceinline__ void share_fma_item(const ShareArgs& p, const ShareIt
   __syncthreads();                              // the next item's queries take this one's place
 }
 
-template <typename A, int NG>
-__global__ void __launch_bounds__(256) share_fma_kernel(ShareArgs p, int stages) {
+// The same for tiles of at most 4 rows, a decode step's token on a sequence's own pages as a rule: there the tiles above would read every
+// key and value from shared memory 4 times over for 4 times the rows. A key belongs to four neighbouring lanes (a quarter of its dims
+// each), a row's weights to one warp, and four dims of the values to a thread, for every kgs-th key; the threads' sums over their keys meet
+// once, behind the last page. Keys and values are read from shared memory once (64 sequences of 100 tokens of their own and 1,000 shared,
+// 32 heads of 64: 117 us a call, 178 on the tiles above).
+template <typename A>
+__device__ __forceinline__ void share_few_item(const ShareArgs& p, const ShareItem& it, int stages, float* sm) {
+  const int hd = p.hd, vd = p.vd, rep = p.H / p.G, n_rows = it.n_tok * rep, kq = hd >> 2, vq = vd >> 2;
+  const int ql = hd + 4, kl = share_row_len<A>(hd), vl = share_row_len<A>(vd), kgs = 256 / vq;
+  float* Qs = sm;                              // [4][ql]
+  float* Ps = Qs + SF_ROWS * ql;               // [4][64] weights, then the threads' sums
+  float* corr = Ps + SF_ROWS * SF_PS - 4;      // [4]
+  A* Ks = (A*)(Ps + SF_ROWS * SF_PS);
+  A* Vs = Ks + stages * SLLM_PAGE * kl;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, key = tid >> 2, sub = tid & 3, dg = 4 * (tid % vq), kg = tid / vq;
+  const int* row = p.block_table + (size_t)it.seq * p.max_pages;
+  const A *kp = (const A*)p.kpages, *vp = (const A*)p.vpages;
+
+  const int kd = 4 * (tid % kq), k0 = tid < 256 / kq * kq ? tid / kq : SLLM_PAGE, v0 = kg < kgs ? kg : SLLM_PAGE;
+  auto fetch = [&](int t) {                    // keys behind the last token, and a page that is none: zeros
+    const int page = share_page(p, row, t), n_keys = page < 0 ? 0 : min(SLLM_PAGE, it.last + 1 - t * SLLM_PAGE), s = (t - it.p0) % stages;
+    const size_t at = ((size_t)max(page, 0) * p.G + it.g) * SLLM_PAGE;
+    for (int kk = k0; kk < SLLM_PAGE; kk += 256 / kq) share_copy4(Ks + (s * SLLM_PAGE + kk) * kl + kd, kp + (at + kk) * hd + kd, kk < n_keys);
+    for (int kk = v0; kk < SLLM_PAGE; kk += kgs) share_copy4(Vs + (s * SLLM_PAGE + kk) * vl + dg, vp + (at + kk) * vd + dg, kk < n_keys);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if (it.p0 < it.p1) fetch(it.p0);
+  for (int e = tid; e < 4 * kq; e += 256) {
+    const int r = e / kq, d = 4 * (e % kq);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < n_rows) v = ld4((const A*)p.q + (size_t)p.toks[it.tok0 + r / rep] * p.q_ld + (size_t)(it.g * rep + r % rep) * hd + d);
+    *(float4*)(Qs + r * ql + d) = v;
+  }
+  const int sees = share_sees(it, sub, rep);   // of row `sub`
+  float m = -INFINITY, l = 0.f, o[4][4];       // m, l: of row `warp`, in warps 0 to 3
+#pragma unroll
+  for (int r = 0; r < 4; r++)
+#pragma unroll
+    for (int c = 0; c < 4; c++) o[r][c] = 0.f;
+  for (int t = it.p0; t < it.p1; t++) {
+    if (stages == 2 && t + 1 < it.p1) {
+      fetch(t + 1);
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+    } else {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    __syncthreads();
+    const A *K = Ks + (((t - it.p0) % stages) * SLLM_PAGE + key) * kl, *V = Vs + ((t - it.p0) % stages) * SLLM_PAGE * vl + dg;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int d = 4 * sub; d < hd; d += 16) {
+      const float4 k = ld4(K + d);
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float4 q = *(const float4*)(Qs + r * ql + d);
+        s[r] = fmaf(q.x, k.x, s[r]);
+        s[r] = fmaf(q.y, k.y, s[r]);
+        s[r] = fmaf(q.z, k.z, s[r]);
+        s[r] = fmaf(q.w, k.w, s[r]);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+      s[r] += __shfl_xor_sync(0xffffffffu, s[r], 1);
+      s[r] += __shfl_xor_sync(0xffffffffu, s[r], 2);
+    }
+    float v = (sub == 0 ? s[0] : sub == 1 ? s[1] : sub == 2 ? s[2] : s[3]) * p.scale;
+    if (p.softcap > 0.f) v = p.softcap * tanhf(v / p.softcap);
+    Ps[sub * SLLM_PAGE + key] = t * SLLM_PAGE + key <= sees ? v * SHARE_LOG2E : -INFINITY;
+    __syncthreads();
+    if (warp < 4) {
+      const float a = Ps[warp * SLLM_PAGE + lane], b = Ps[warp * SLLM_PAGE + lane + 32];
+      const float m_new = fmaxf(m, warp_max(fmaxf(a, b))), f = m_new == -INFINITY ? 1.f : exp2f(m - m_new);
+      const float x = a == -INFINITY ? 0.f : exp2f(a - m_new), y = b == -INFINITY ? 0.f : exp2f(b - m_new);
+      l = fmaf(l, f, warp_sum(x + y));
+      m = m_new;
+      Ps[warp * SLLM_PAGE + lane] = x;
+      Ps[warp * SLLM_PAGE + lane + 32] = y;
+      if (lane == 0) corr[warp] = f;
+    }
+    __syncthreads();
+    if (kg < kgs) {
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        const float f = corr[r];
+#pragma unroll
+        for (int c = 0; c < 4; c++) o[r][c] *= f;
+      }
+#pragma unroll 4
+      for (int kk = kg; kk < SLLM_PAGE; kk += kgs) {
+        const float4 x = ld4(V + kk * vl);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const float w = Ps[r * SLLM_PAGE + kk];
+          o[r][0] = fmaf(w, x.x, o[r][0]);
+          o[r][1] = fmaf(w, x.y, o[r][1]);
+          o[r][2] = fmaf(w, x.z, o[r][2]);
+          o[r][3] = fmaf(w, x.w, o[r][3]);
+        }
+      }
+    }
+    __syncthreads();                            // this page's place is free, and so are the weights
+    if (stages == 1 && t + 1 < it.p1) fetch(t + 1);
+  }
+  float* ml = p.part + (size_t)p.part_rows * vd;
+  if (warp < n_rows && lane == 0) {
+    *(float2*)(ml + 2 * ((size_t)it.part0 + warp)) = make_float2(m, l);
+    Qs[SF_ROWS * ql - 8 + 2 * warp] = m;        // (behind the queries)
+    Qs[SF_ROWS * ql - 7 + 2 * warp] = l;
+  }
+  if (kg < kgs)
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+      if (r < n_rows) *(float4*)(Ps + ((size_t)kg * n_rows + r) * vd + dg) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+  __syncthreads();
+  for (int e = tid; e < n_rows * vq; e += 256) {
+    const int r = e / vq, d = 4 * (e % vq);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < kgs; k++) {
+      const float4 b = *(const float4*)(Ps + ((size_t)k * n_rows + r) * vd + d);
+      a.x += b.x;
+      a.y += b.y;
+      a.z += b.z;
+      a.w += b.w;
+    }
+    const float mr = Qs[SF_ROWS * ql - 8 + 2 * r], lr = Qs[SF_ROWS * ql - 7 + 2 * r];
+    if (!(fabsf(a.x) + fabsf(a.y) + fabsf(a.z) + fabsf(a.w) < INFINITY) && lr < INFINITY)
+      a = share_sum_by_key(p, it, (const A*)p.q + (size_t)p.toks[it.tok0 + r / rep] * p.q_ld + (size_t)(it.g * rep + r % rep) * hd,
+                           share_sees(it, r, rep), mr, d, it.p0, 1);
+    *(float4*)(p.part + share_at((size_t)it.part0 + r, d, vd)) = a;
+  }
+  __syncthreads();                              // the next item takes this one's place
+}
+
+template <typename A, int NG, int BLOCKS>
+__global__ void __launch_bounds__(256, BLOCKS) share_fma_kernel(ShareArgs p, int stages) {
   extern __shared__ __align__(16) float share_sm[];
   pdl_launch_dependents();
   pdl_wait();
   const int i1 = p.first[blockIdx.x + 1];
   for (int i = p.first[blockIdx.x]; i < i1; i++) {
     const ShareItem it = share_item(p, i);
-    if (it.n_tok * (p.H / p.G) <= 16) share_fma_item<A, NG, 1>(p, it, stages, share_sm);
+    const int n_rows = it.n_tok * (p.H / p.G);
+    if (n_rows <= 4) share_few_item<A>(p, it, stages, share_sm);
+    else if (n_rows <= 16) share_fma_item<A, NG, 1>(p, it, stages, share_sm);
     else share_fma_item<A, NG, 4>(p, it, stages, share_sm);
   }
 }

@@ -204,8 +204,8 @@ def _batch(rng, n, rep, runs):
     return table, held, new
 
 
-@pytest.mark.parametrize("shape", [TileShape(256, 148, True, 1.0, 0.7), TileShape(64, 296), TileShape(64, 7, min_pages=1), TileShape(16, 40, True),
-                                   TileShape(256, 148, True, 2.0, 0.7, 2, 16, 8, 0.4, 0.2)], ids=str)
+@pytest.mark.parametrize("shape", [TileShape(256, 148, True, 1.0, ((128, 0.7),)), TileShape(64, 296), TileShape(64, 7, costs=((4, 0.2), (16, 0.5)), min_pages=1), TileShape(16, 40, True),
+                                   TileShape(256, 148, True, 2.0, ((128, 0.7),), 2, 16, 8, 0.4, 0.2)], ids=str)
 @pytest.mark.parametrize("runs", [False, True])
 def test_a_plan_covers_every_key_of_every_row_once(shape, runs):
     rng = random.Random(11)
@@ -262,7 +262,7 @@ def test_plans_share_the_work_evenly_among_blocks():
     table[:, :128] = np.arange(128)
     held = np.asarray([8192 + 40 * i for i in range(64)])
     for thin in (0, 16):
-        shape = TileShape(256, 148, True, 1.0, 0.7, 2, thin, 8 if thin else 0, 0.5, 0.25)
+        shape = TileShape(256, 148, True, 1.0, ((128, 0.7),), 2, thin, 8 if thin else 0, 0.5, 0.25)
         plan = SharePlan.build(table, held, [1] * 64, 32, 8, shape, None)
         items, first, warps = plan.parts["items"], plan.parts["first"], plan.parts["thin_first"]
         end = np.where(items[:, 5] < 0, held[items[:, 2]] // PAGE + 1, items[:, 5])
