@@ -57,6 +57,25 @@ __device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
   return r;
 }
 
+// the 32 lanes' rows of queries, from row r32 of a buffer's n on, into the buffer at sQ: 64-wide blocks of FS_ROWS rows, 128-byte swizzle;
+// `row`: this lane's row's address
+template <int KD>
+__device__ __forceinline__ void fs_gather32(unsigned long long row, uint32_t sQ, int r32, int n, int k_vecs, int k_used, int lane) {
+  constexpr int VECS = KD / 8;                    // 16-byte vectors of a row: 32 / VECS rows go together, a lane to a vector
+  const int c = lane % VECS;
+#pragma unroll
+  for (int e = 0; e < VECS; e++) {
+    const int r = r32 + e * (32 / VECS) + lane / VECS;
+    const char* from = (const char*)__shfl_sync(0xffffffffu, row, r & 31);
+    if (r < n && c < k_used)
+      cp_async16(sQ + (c >> 3) * (FS_ROWS * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4), from + (c < k_vecs ? 16 * c : 0), c < k_vecs);
+  }
+}
+__device__ __forceinline__ unsigned long long fs_row(const ShareArgs& p, const ShareItem& it, int rho, int rep) {
+  const int r = min(rho, it.n_tok * rep - 1);
+  return (unsigned long long)((const bf16*)p.q + (size_t)p.toks[it.tok0 + r / rep] * p.q_ld + (size_t)(it.g * rep + r % rep) * p.hd);
+}
+
 // warps with thin tiles, and the buffers (a page of keys or of values) that each has
 template <int KD, int VD>
 __host__ __device__ constexpr int fs_thin_warps() { return KD <= 64 && VD <= 64 ? 8 : KD > 64 && VD > 64 ? 7 : 6; }
@@ -432,6 +451,7 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   // Every role walks the same items and counts by itself the pages fetched (JU), the pages its half has taken (J) and the query
   // buffers used (Q: one by a tile of at most 128 rows, two by a larger one); a barrier's phase follows from those counts.
   const int rep = p.H / p.G, i0 = p.first[blockIdx.x], i1 = p.first[blockIdx.x + 1];
+  const int k_vecs = p.hd / 8, k_used = (p.hd + 15) / 16 * 2;      // of a query row: what it has, and what the products' steps of 16 dims read
   if (i1 > i0) {
     if (threadIdx.x < min(FS_CACHED, i1 - i0)) cached[threadIdx.x] = share_item(p, i0 + threadIdx.x);
     __syncthreads();
@@ -469,37 +489,26 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
       for (int j = max(0, JU - STAGES); j < JU; j++) mbar_wait(b_kvfull + 8 * (j % STAGES), (j / STAGES) & 1, &never);
     }
   } else if (warp == 3) {
-    constexpr int VECS = KD / 8;                    // 16-byte vectors of a row
-    const int k_vecs = p.hd / 8, k_used = (p.hd + 15) / 16 * 2;      // what the row has, and what the products' steps of 16 dims read
     int Q = 0;
     bool ok = true;
     for (int i = i0; ok && i < i1; i++) {
       const ShareItem it = item(i);
       const int n_rows = it.n_tok * rep;
       for (int b0 = 0; ok && b0 < n_rows; b0 += FS_ROWS, Q++) {
+        if (i == i0) continue;                       // (the softmax warps fetch the first item's, having nothing else to do)
         const int b = Q & 1;
         // the products that read what the buffer held are done
         ok = mbar_wait(b_qempty + 8 * b, ((Q >> 1) & 1) ^ 1, abort);
         if (!ok) break;
         __syncwarp();
-        // a lane finds four rows; then 32 / VECS rows go together, a lane to a vector
-        const int c = lane % VECS, n = min(FS_ROWS, n_rows - b0);
+        const int n = min(FS_ROWS, n_rows - b0);
         unsigned long long row[FS_ROWS / 32];
 #pragma unroll
-        for (int k = 0; k < FS_ROWS / 32; k++) {
-          const int rho = min(b0 + 32 * k + lane, n_rows - 1);
-          row[k] = (unsigned long long)((const bf16*)p.q + (size_t)p.toks[it.tok0 + rho / rep] * p.q_ld + (size_t)(it.g * rep + rho % rep) * p.hd);
-        }
+        for (int k = 0; k < FS_ROWS / 32; k++) row[k] = fs_row(p, it, b0 + 32 * k + lane, rep);
 #pragma unroll
         for (int k = 0; k < FS_ROWS / 32; k++) {
           if (32 * k >= n) break;
-#pragma unroll
-          for (int e = 0; e < VECS; e++) {
-            const int r = 32 * k + e * (32 / VECS) + lane / VECS;
-            const char* from = (const char*)__shfl_sync(0xffffffffu, row[k], r & 31);
-            if (r < n && c < k_used)
-              cp_async16(sQ + b * Q_BYTES + (c >> 3) * QA + r * 128 + (((c & 7) ^ (r & 7)) << 4), from + (c < k_vecs ? 16 * c : 0), c < k_vecs);
-          }
+          fs_gather32<KD>(row[k], sQ + b * Q_BYTES, 32 * k, n, k_vecs, k_used, lane);
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -588,6 +597,17 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     float* const ml = p.part + (size_t)p.part_rows * p.vd;
     int JU0 = 0, J0 = 0;
     bool ok = true;
+    if (i0 < i1) {                                 // the first item's queries: this half's buffer, 32 rows a warp
+      const ShareItem it = item(i0);
+      const int n_rows = it.n_tok * rep, n = min(FS_ROWS, n_rows - x * FS_ROWS);
+      if (n > 0) {
+        if (32 * q < n) fs_gather32<KD>(fs_row(p, it, x * FS_ROWS + r, rep), sQ + x * Q_BYTES, 32 * q, n, k_vecs, k_used, lane);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + x) : "memory");
+        if (q == 0 && lane == 0) mbar_arrive(b_qfull + 8 * x);
+      }
+    }
     for (int i = i0; ok && i < i1; i++) {
       const ShareItem it = item(i);
       const int n_rows = it.n_tok * rep;
