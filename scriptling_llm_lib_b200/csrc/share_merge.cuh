@@ -36,6 +36,22 @@ __global__ void __launch_bounds__(32 * SHARE_MERGE_WARPS) share_merge_kernel(Sha
   // ---- the largest score of this warp's entries; the first of them stay at hand
   int at = first + j * apart < n ? p.list[i0 + first + j * apart] + r : 0;
   float2 v = first + j * apart < n ? ml[at] : make_float2(-INFINITY, 0.f);
+  // four entries' sums, on their way beside the (m, l) that weigh them: what a row does not see is loaded and left out
+  float4 x[4][NQ];
+  auto load = [&](int e0, int m) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const size_t row = __shfl_sync(0xffffffffu, at, ((e0 + e) * RB + lane % RB) & 31);
+#pragma unroll
+      for (int k = 0; k < NQ; k++) {
+        const int d = 4 * (j + k * J);
+        if (e0 + e < m && d < p.vd) x[e][k] = *(const float4*)(p.part + share_at(row, d, p.vd));
+        else x[e][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+  };
+  auto held = [&](int base) { return min(J, (n - base + apart - 1) / apart); };
+  load(0, held(first));
   float M = v.x;
 #pragma unroll 4
   for (int i = first + step + j * apart; i < n; i += step) M = fmaxf(M, ml[p.list[i0 + i] + r].x);
@@ -51,34 +67,25 @@ __global__ void __launch_bounds__(32 * SHARE_MERGE_WARPS) share_merge_kernel(Sha
       at = base + j * apart < n ? p.list[i0 + base + j * apart] + r : 0;
       v = base + j * apart < n ? ml[at] : make_float2(-INFINITY, 0.f);
     }
-    // an entry none of whose keys this row sees, or none at all, weighs 0 and its values are not read; a sum that is NaN spoils the row
+    // an entry none of whose keys this row sees, or none at all, weighs 0 and its values are left out; a sum that is NaN spoils the row
     const float wgt = v.y != v.y ? v.y : exp2f(v.x - M0);
     if (wgt != 0.f) den = fmaf(wgt, v.y, den);
-    const int m = min(J, (n - base + apart - 1) / apart);
+    const int m = held(base);
     for (int e0 = 0; e0 < m; e0 += 4) {
-      float c[4];
-      float4 x[4][NQ];
+      if (base != first || e0 > 0) load(e0, m);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int from = ((e0 + e) * RB + lane % RB) & 31;
-        c[e] = __shfl_sync(0xffffffffu, wgt, from);
-        const size_t row = __shfl_sync(0xffffffffu, at, from);
-        if (e0 + e >= m) c[e] = 0.f;
+        const float c = __shfl_sync(0xffffffffu, wgt, ((e0 + e) * RB + lane % RB) & 31);
+        if (e0 + e < m && c != 0.f) {
 #pragma unroll
-        for (int k = 0; k < NQ; k++) {
-          const int d = 4 * (j + k * J);
-          x[e][k] = c[e] != 0.f && d < p.vd ? *(const float4*)(p.part + share_at(row, d, p.vd)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int k = 0; k < NQ; k++) {
+            a[k].x = fmaf(c, x[e][k].x, a[k].x);
+            a[k].y = fmaf(c, x[e][k].y, a[k].y);
+            a[k].z = fmaf(c, x[e][k].z, a[k].z);
+            a[k].w = fmaf(c, x[e][k].w, a[k].w);
+          }
         }
       }
-#pragma unroll
-      for (int e = 0; e < 4; e++)
-#pragma unroll
-        for (int k = 0; k < NQ; k++) {
-          a[k].x = fmaf(c[e], x[e][k].x, a[k].x);
-          a[k].y = fmaf(c[e], x[e][k].y, a[k].y);
-          a[k].z = fmaf(c[e], x[e][k].z, a[k].z);
-          a[k].w = fmaf(c[e], x[e][k].w, a[k].w);
-        }
     }
   }
 #pragma unroll
