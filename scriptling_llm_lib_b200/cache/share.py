@@ -234,9 +234,10 @@ class PlanCapacity:
         return cls(n_kv * tiles + shape.workers + thin, entries, entries * rep)
 
 
-def _cut(cost, pages, marks, least):
-    """Units that stand in a line, each as long as its cost, cut where the line is marked, but into no pieces of fewer than `least` pages (a
-    number for each unit): (unit, first page, page end, the number of marks in front of its middle) of every piece, in the line's order."""
+def _cut(cost, pages, marks, least, grain):
+    """Units that stand in a line, each as long as its cost, cut where the line is marked, at a multiple of `grain` pages and into no
+    pieces of fewer than `least` (a number for each unit): (unit, first page, page end, the number of marks in front of its middle) of
+    every piece, in the line's order."""
     ends = np.cumsum(cost)
     at = ends - cost
     k0, k1 = np.searchsorted(marks, at, "right"), np.searchsorted(marks, ends - 1e-6, "left")
@@ -244,10 +245,9 @@ def _cut(cost, pages, marks, least):
     cu = np.repeat(np.arange(len(cost)), n)
     k = np.arange(len(cu)) - np.repeat(np.cumsum(n) - n, n) + k0[cu]
     cut = np.rint((marks[k] - at[cu]) / cost[cu] * pages[cu]).astype(np.int64) if len(cu) else cu
-    # a unit's cuts that fall into one run of `least` pages are one cut
-    cut = np.rint(cut / least[cu]).astype(np.int64) * least[cu]
+    cut = np.rint(cut / grain[cu]).astype(np.int64) * grain[cu]
     fine = (cut >= least[cu]) & (pages[cu] - cut >= least[cu])
-    fine[1:] &= (cu[1:] != cu[:-1]) | (cut[1:] != cut[:-1])
+    fine[1:] &= (cu[1:] != cu[:-1]) | (cut[1:] - cut[:-1] >= least[cu[1:]])
     cu, cut = cu[fine], cut[fine]
     iu, begin = np.concatenate([np.arange(len(cost)), cu]), np.concatenate([np.zeros(len(cost), dtype=np.int64), cut])
     by = np.lexsort((begin, iu))
@@ -301,14 +301,15 @@ def _lay_out(order, nodes, own, held, new, rep: int, n_kv: int, shape: TileShape
     n_thick = n_kv * int((~thin).sum())
     share = max(float(c.sum()) / shape.workers, shape.min_pages + shape.item_pages)      # of a block
     # the line of the tiles' costs is cut into equal lengths, one for each block; what is left of each block's share is the warps'
-    i1, b1, e1, w1 = _cut(c[:n_thick], pages_u[:n_thick], share * np.arange(1, shape.workers), np.full(n_thick, shape.min_pages))
+    i1, b1, e1, w1 = _cut(c[:n_thick], pages_u[:n_thick], share * np.arange(1, shape.workers), np.full(n_thick, shape.min_pages),
+                          np.where(half[u[:n_thick]], 2, 1))         # (the halves of a block that take pages in turn have as many each)
     if n_thick < len(u):
         load = np.bincount(w1, weights=c[i1] * (e1 - b1) / np.maximum(1, pages_u[i1]), minlength=shape.workers)
         left = np.maximum(share - load - np.where(load > 0, shape.thin_start, 0.0), 0.0)
         left = np.repeat((left if left.any() else np.ones_like(left)) / shape.thin_warps, shape.thin_warps)
         line = np.cumsum(left)
-        i2, b2, e2, w2 = _cut(c[n_thick:], pages_u[n_thick:], line[:-1] * (float(c[n_thick:].sum()) / line[-1]),
-                              np.maximum(1, -(-pages_u[n_thick:] // MOST_PIECES)))
+        least = np.maximum(1, -(-pages_u[n_thick:] // MOST_PIECES))
+        i2, b2, e2, w2 = _cut(c[n_thick:], pages_u[n_thick:], line[:-1] * (float(c[n_thick:].sum()) / line[-1]), least, least)
     else:
         i2 = b2 = e2 = w2 = np.zeros(0, dtype=np.int64)
     iu, begin, stop = np.concatenate([i1, i2 + n_thick]), np.concatenate([b1, b2]), np.concatenate([e1, e2])
