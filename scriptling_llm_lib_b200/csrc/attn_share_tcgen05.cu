@@ -1,5 +1,5 @@
 // Attention of a step whose sequences share pages on tcgen05 tensor cores (bfloat16; keys and values of up to 128 dims in multiples of
-// 8): every shared run of pages is read once for all rows that see it. The mathematics and the plan are in share_kernels.cuh and
+// 8): every shared run of pages is read once for all rows that see it. The mathematics is at the head of share_kernels.cuh, the plan in
 // cache/share.py; results are partial and joined by share_merge_kernel.
 //
 // One block per SM stays and walks its list of items; barriers, tensor memory, the ring of pages and two query buffers live across items.
@@ -14,11 +14,18 @@
 // two or three buffers of its own and computes with mma.sync, so that six to eight chains run side by side and memory is what
 // bounds them. A plan gives every block its share of either kind.
 //
-// Rows of a tile belong to several sequences and stand anywhere in the step, so a warp gathers them (16 bytes a lane, asynchronously,
-// into the 128-byte swizzle) where keys and values come by TMA, a page and head at a time. S = Q K^T (128 x 64) and O += P V as
-// in attn_prefill_tcgen05.cu: thread = row = tensor-memory lane, P back into tensor memory as bfloat16 pairs (the weights' only
-// rounding; their sum is taken before it), O rescaled only when a row's maximum has outgrown its reference by 2^8. Warps whose rows are all past the tile's end pass the barriers and
-// compute nothing. Waits are bounded (2 s), after which the kernel raises *err, lets its copies land, frees its tensor memory and returns.
+// Rows of a tile belong to several sequences and stand anywhere in the step, so warps gather them (16 bytes a lane, asynchronously,
+// into the 128-byte swizzle; the first tile's the softmax warps, the others' a warp of its own) where keys and values come by TMA, a page
+// and head at a time. S = Q K^T (128 x 64) and O += P V as in attn_prefill_tcgen05.cu: thread = row = tensor-memory lane, P back into
+// tensor memory as bfloat16 pairs (the weights' only rounding; their sum is taken before it), O rescaled only when a row's maximum has
+// outgrown its reference by 2^8. Warps whose rows are all past the tile's end pass the barriers and compute nothing. Waits are bounded
+// (2 s), after which the kernel raises *err, lets its copies land, frees its tensor memory and returns.
+//
+// Bound by the chain of a page where tiles are full (1.05 us for 256 rows x 64 keys at heads of 128: 1.2 PFLOP/s while it runs, the
+// tensor pipe half busy, the exponentials 46% of their unit), by an item's start and end (5 us) and the thin tiles' chains (3 us a page and
+// warp) where there are few rows. With the joining kernel: 64 runs of up to 40 tokens behind 16,384 shared ones, 32 heads of 128 on 8, 389
+// us (0.92 PFLOP/s; 2,215 each for itself); 64 single tokens behind 8,192 and up to 300 of their own 38 us (73 MB to read and write; 343);
+// 8 behind 4,096 and up to 150, 32 heads of 64, 14 us (41).
 #include "attn_tcgen05.cuh"
 #include "share_merge.cuh"
 #include <type_traits>

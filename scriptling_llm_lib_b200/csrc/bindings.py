@@ -1754,7 +1754,8 @@ class SharedAttention:
             sm_count = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
         if self.dtype == torch.bfloat16 and all(w % 8 == 0 and w <= 128 for w in (head_dim, v_dim)):
             # tcgen05, and mma.sync for thin tiles. What an item and a thin page cost beside a page of 256 rows (1.05 us): measured
-            # over 17 decode steps of 2 to 64 sequences and prompts of 5 to 32; an item at 6 or 4 is 5% slower over them, half or twice of the others 3 to 20%
+            # over 17 decode steps of 2 to 64 sequences and prompts of 5 to 32; an item at 6 or 4 is 5% slower over them, half or twice of
+            # the others 3 to 20%
             narrow = max(head_dim, v_dim) <= 64
             return TileShape(rows=256, workers=sm_count, halves=True, item_pages=5.0, costs=((128, 0.85),), thin_rows=16,
                              thin_warps=8 if narrow else 7 if min(head_dim, v_dim) > 64 else 6, thin_cost=0.3 if narrow else 0.42, thin_item=1.0,
