@@ -6,7 +6,7 @@
 // A warp for a token and RB query heads that stand side by side in the scratch (a power of two that divides the heads of a key/value
 // head, so that their 16-byte pieces fill whole sectors). Lane j RB + r has head r of them: first entry base + j of the list (row of the
 // scratch, m, l), then the dims 4 (j + k 32 / RB) .. + 3 of the sum, of which NQ fit. Loads of four entries are under way at once. Bound by the chain of its loads (which entries, their m and l beside the
-// sums): 6 us where outputs are few, 26 for 146,688 rows of 128 from memory (75 MB; 16 warps on an SM).
+// sums): 4 to 8 us where outputs are few, 21 for 146,688 rows of 128 (75 MB; 16 warps on an SM).
 struct ShareMergeArgs {
   const float* part;
   long long part_rows;
