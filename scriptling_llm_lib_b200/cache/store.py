@@ -273,16 +273,17 @@ class SequenceCache:
 
     def compact(self, n_pages: int | None = None) -> int:
         """Move the held pages of every group to the front of its storage; with `n_pages`, into a new storage of that many (fewer give
-        memory back, more make room). Returns the number of pages that were copied; CacheFull, with nothing changed, where more are
-        held. Kernels that were captured with the old storage's addresses are the caller's to drop."""
+        memory back, more make room; both are held until the copies are done). Returns the number of pages that were copied; CacheFull,
+        with nothing changed, where more are held, and the allocator's error where there is no memory for the new storage. Kernels that were captured with the old storage's addresses are the caller's to drop."""
         if n_pages is not None:
             if n_pages < 1:
                 raise ValueError("the cache needs at least one page")
             for g in self.groups:
                 if g.pool.n_held > n_pages:
                     raise CacheFull(f"{g.pool.n_held} pages of the {g.need.kind} group are held; {n_pages} are to be kept")
+            fresh = [[torch.empty((t.shape[0], n_pages + 1, *t.shape[2:]), dtype=t.dtype, device=t.device) for t in (g.k, g.v)] for g in self.groups]
         moved = 0
-        for g in self.groups:
+        for at, g in enumerate(self.groups):
             held = [i for i in range(g.pool.n) if g.pool.is_held(i)]
             if n_pages is None:
                 k = len(held)
@@ -293,12 +294,8 @@ class SequenceCache:
                 self._copy([(g.k, g.k), (g.v, g.v)], src, [to[i] for i in src])
             else:
                 to, src = {i: j for j, i in enumerate(held)}, held
-                for name in ("k", "v"):        # (one after the other: both old and new are held meanwhile)
-                    old = getattr(g, name)
-                    new = torch.empty((old.shape[0], n_pages + 1, *old.shape[2:]), dtype=old.dtype, device=old.device)
-                    self._copy([(old, new)], src, [to[i] for i in src])
-                    setattr(g, name, new)
-                    del old
+                self._copy([(g.k, fresh[at][0]), (g.v, fresh[at][1])], src, [to[i] for i in src])
+                g.k, g.v = fresh[at]
             g.renumber(to, n_pages)
             moved += len(src)
         if n_pages is not None:

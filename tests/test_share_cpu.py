@@ -120,6 +120,33 @@ def test_a_random_life_of_forks_writes_closes_and_compactions():
     assert all(g.pool.n_free == g.pool.n and g.pool.n_shared == 0 for g in c.groups)
 
 
+def test_a_new_storage_that_finds_no_memory_changes_nothing(monkeypatch):
+    c = _cache()
+    slot, tokens = c.open(), list(range(1, 200))
+    _write(c, slot, tokens)
+    fork = c.fork(slot)[0]
+    before, pages, made = [(g.k, g.v) for g in c.groups], c.n_pages, []
+
+    def empty(*args, **kwargs):
+        made.append(1)
+        if len(made) == 4:                  # the second group's values
+            raise torch.OutOfMemoryError("no memory")
+        return torch.zeros(*args, **kwargs)
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "empty", empty)
+        with pytest.raises(torch.OutOfMemoryError):
+            c.compact(40)
+    assert len(made) == 4 and c.n_pages == pages and all(g.k is k and g.v is v and g.pool.n == pages for g, (k, v) in zip(c.groups, before))
+    _consistent(c)
+    for s in (slot, fork):
+        _check(c, s, tokens)
+    c.compact(40)
+    assert c.n_pages == 40
+    for s in (slot, fork):
+        _check(c, s, tokens)
+
+
 def test_the_writers_of_a_shared_page_get_their_own_and_the_last_keeps_it():
     c = _cache()
     a = c.open()
