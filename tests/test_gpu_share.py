@@ -271,6 +271,44 @@ def test_on_a_stream_of_its_own():
     c.check(out)
 
 
+@pytest.mark.parametrize("dtype", [F, B16], ids=["f32", "bf16"])
+def test_pages_behind_four_gigabytes_of_a_storage(dtype):
+    """Elements past 2^31 (bytes past 2^32), of attention and of copies: the same results as from a small storage."""
+    c = Case("runs", (32, 8, 128, 128), dtype, junk=False)
+    want, far = c.run(), 33_900
+    k, v = (torch.empty((far + 100, *t.shape[1:]), dtype=dtype, device="cuda") for t in (c.k, c.v))
+    k[far:far + c.n_pages], v[far:far + c.n_pages] = c.k, c.v
+    small, c.k, c.v = (c.k, c.v), k, v
+    c.table = np.where(c.table < 0, c.table, c.table + far).astype(np.int32)
+    assert torch.equal(c.run(), want)
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    src, dst = (torch.arange(a, a + c.n_pages, dtype=torch.int32, device="cuda") for a in (far, 0))
+    PageKernels().copy_pages([(k[None], k[None]), (v[None], v[None])], src, dst, None, err)
+    assert int(err) == 0 and torch.equal(k[:c.n_pages], small[0]) and torch.equal(v[:c.n_pages], small[1])
+    k[far:].zero_()
+    PageKernels().copy_pages([(k[None], k[None])], dst, src, None, err)
+    assert int(err) == 0 and torch.equal(k[far:far + c.n_pages], small[0])
+
+
+def test_two_calls_at_once_with_one_plan():
+    """Calls on two streams, with a scratch each, share nothing that they write."""
+    c = Case("many", (32, 8, 128, 128), B16)
+    plan, streams, outs = c.plan(), [torch.cuda.Stream() for _ in range(2)], []
+    want = c.run(plan)
+    ops, table, err = KernelSet(B16).shared, torch.from_numpy(c.table).cuda(), torch.zeros(1, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    for s in streams:
+        with torch.cuda.stream(s):
+            outs.append([])
+            part = torch.empty((plan.part_floats(128),), device="cuda")
+            for _ in range(20):
+                out = torch.zeros_like(want)
+                ops.attn(c.q, out, c.pos, table, c.k, c.v, plan, part, c.scale, err)
+                outs[-1].append(out)
+    torch.cuda.synchronize()
+    assert int(err) == 0 and all(torch.equal(o, want) for some in outs for o in some)
+
+
 def test_refusals():
     c = Case("two", (16, 4, 64, 64), B16)
     ops, plan = KernelSet(B16).shared, c.plan()
