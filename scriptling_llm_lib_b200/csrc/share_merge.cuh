@@ -5,8 +5,9 @@
 
 // A warp for a token and RB query heads that stand side by side in the scratch (a power of two that divides the heads of a key/value
 // head, so that their 16-byte pieces fill whole sectors). Lane j RB + r has head r of them: first entry base + j of the list (row of the
-// scratch, m, l), then the dims 4 (j + k 32 / RB) .. + 3 of the sum, of which NQ fit. Loads of four entries are under way at once. Bound by the chain of its loads (which entries, their m and l beside the
-// sums): 4 to 8 us where outputs are few, 21 for 146,688 rows of 128 (75 MB; 16 warps on an SM).
+// scratch, m, l), then the dims 4 (j + k 32 / RB) .. + 3 of the sum, of which NQ fit. Loads of two entries are under way at once (with four
+// fewer warps fit an SM: prompt steps of 700 rows 2 to 6% slower), of four with SPLIT. Bound by the chain of its loads (which entries,
+// their m and l beside the sums): 4 to 8 us where outputs are few, about 20 for 146,688 rows of 128 (75 MB).
 struct ShareMergeArgs {
   const float* part;
   long long part_rows;
@@ -19,10 +20,11 @@ struct ShareMergeArgs {
 // loads (a microsecond for every four entries) is what the kernel lasts.
 #define SHARE_MERGE_WARPS 8
 template <typename A, int RB, int NQ, bool SPLIT>
-__global__ void __launch_bounds__(32 * SHARE_MERGE_WARPS) share_merge_kernel(ShareMergeArgs p) {
+__global__ void __launch_bounds__(32 * SHARE_MERGE_WARPS, SPLIT ? 2 : 3) share_merge_kernel(ShareMergeArgs p) {
   pdl_launch_dependents();
   pdl_wait();
   constexpr int J = 32 / RB, W = SHARE_MERGE_WARPS, MET = SPLIT ? W : 1;      // J: entries that a warp holds at a time
+  constexpr int E = SPLIT ? 4 : 2;                                           // of which so many are under way at once
   __shared__ float4 met[MET][NQ][32];
   __shared__ float2 met_ml[MET][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, per = p.H / RB;
@@ -37,11 +39,11 @@ __global__ void __launch_bounds__(32 * SHARE_MERGE_WARPS) share_merge_kernel(Sha
   // ---- the largest score of this warp's entries; the first of them stay at hand
   int at = first + j * apart < n ? p.list[i0 + first + j * apart] + r : 0;
   float2 v = first + j * apart < n ? ml[at] : make_float2(-INFINITY, 0.f);
-  // four entries' sums, on their way beside the (m, l) that weigh them: what a row does not see is loaded and left out
-  float4 x[4][NQ];
+  // the first entries' sums, on their way beside the (m, l) that weigh them: what a row does not see is loaded and left out
+  float4 x[E][NQ];
   auto load = [&](int e0, int m) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
+    for (int e = 0; e < E; e++) {
       const size_t row = __shfl_sync(0xffffffffu, at, ((e0 + e) * RB + lane % RB) & 31);
 #pragma unroll
       for (int k = 0; k < NQ; k++) {
@@ -72,10 +74,10 @@ __global__ void __launch_bounds__(32 * SHARE_MERGE_WARPS) share_merge_kernel(Sha
     const float wgt = v.y != v.y ? v.y : exp2f(v.x - M0);
     if (wgt != 0.f) den = fmaf(wgt, v.y, den);
     const int m = held(base);
-    for (int e0 = 0; e0 < m; e0 += 4) {
+    for (int e0 = 0; e0 < m; e0 += E) {
       if (base != first || e0 > 0) load(e0, m);
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
+      for (int e = 0; e < E; e++) {
         const float c = __shfl_sync(0xffffffffu, wgt, ((e0 + e) * RB + lane % RB) & 31);
         if (e0 + e < m && c != 0.f) {
 #pragma unroll
