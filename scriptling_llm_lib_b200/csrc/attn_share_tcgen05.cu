@@ -23,9 +23,9 @@
 //
 // Bound by the chain of a page where tiles are full (1.05 us for 256 rows x 64 keys at heads of 128: 1.2 PFLOP/s while it runs, the
 // tensor pipe half busy, the exponentials 46% of their unit), by an item's start and end (5 us) and the thin tiles' chains (3 us a page and
-// warp) where there are few rows. With the joining kernel: 64 runs of up to 40 tokens behind 16,384 shared ones, 32 heads of 128 on 8, 389
-// us (0.92 PFLOP/s; 2,215 each for itself); 64 single tokens behind 8,192 and up to 300 of their own 38 us (73 MB to read and write; 343);
-// 8 behind 4,096 and up to 150, 32 heads of 64, 14 us (41).
+// warp) where there are few rows. With the joining kernel: 64 runs of up to 40 tokens behind 16,384 shared ones, 32 heads of 128 on 8, 395
+// us (0.91 PFLOP/s; 2,220 each for itself); 64 single tokens behind 8,192 and up to 300 of their own 37 us (73 MB to read and write; 344);
+// 8 behind 4,096 and up to 150, 32 heads of 64, 13.5 us (41).
 #include "attn_tcgen05.cuh"
 #include "share_merge.cuh"
 #include <type_traits>
