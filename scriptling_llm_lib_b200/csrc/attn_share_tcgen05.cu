@@ -18,7 +18,9 @@
 // into the 128-byte swizzle; the first tile's the softmax warps, the others' a warp of its own) where keys and values come by TMA, a page
 // and head at a time. S = Q K^T (128 x 64) and O += P V as in attn_prefill_tcgen05.cu: thread = row = tensor-memory lane, P back into
 // tensor memory as bfloat16 pairs (the weights' only rounding; their sum is taken before it), O rescaled only when a row's maximum has
-// outgrown its reference by 2^8. Warps whose rows are all past the tile's end pass the barriers and compute nothing. Waits are bounded
+// outgrown its reference by 2^8. With PARTS 2 the weights go into the product in two parts, P and L, that hold a weight to 2^-16 of
+// itself, for layers whose other kernels keep them in float32 (relative errors beside 32-bit sums rounded once 2e-5 to 4e-4, 1.8e-3 to
+// 2.6e-3 in one part; 8 single tokens behind 4,096, heads of 64, 13.7 us, 13.3 in one part; 64 behind 8,192, heads of 128, 41.6, 36.3). Warps whose rows are all past the tile's end pass the barriers and compute nothing. Waits are bounded
 // (2 s), after which the kernel raises *err, lets its copies land, frees its tensor memory and returns.
 //
 // Bound by the chain of a page where tiles are full (1.05 us for 256 rows x 64 keys at heads of 128: 1.2 PFLOP/s while it runs, the
@@ -68,6 +70,18 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// two weights as bfloat16 pairs: rounded (off by 2^-8 of a weight at most), and, with PARTS 2, what that left of them, rounded again (off by
+// 2^-16 of a weight: a 256th of what rounding the output to bfloat16 costs)
+template <int PARTS>
+__device__ __forceinline__ void fs_parts(float u, float v, uint32_t& hi, uint32_t& lo) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(u, v);
+  hi = *(const uint32_t*)&h;
+  if (PARTS == 2) {
+    const __nv_bfloat162 l = __floats2bfloat162_rn(u - __uint_as_float(hi << 16), v - __uint_as_float(hi & 0xffff0000u));
+    lo = *(const uint32_t*)&l;
+  }
+}
+
 // an 8 x 8 matrix of 16-bit elements, two of a row in each lane, turned over
 __device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
   uint32_t r;
@@ -105,7 +119,7 @@ __host__ __device__ constexpr int fs_thin_bufs() { return KD <= 64 && VD <= 64 ?
 // the tile's rows its 8 columns, twice where it has more than 8: half the products of the other way round for the usual tile, whose few
 // rows would leave most of 16 empty. Lane (r = lane / 4, c = lane % 4) has of the scores keys 16 n + r and + 8 of rows 2 c and 2 c + 1,
 // of the output their dims 16 d + r and + 8.
-template <int KD, int VD>
+template <int KD, int VD, int PARTS>
 __device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensorMap* map_v, const ShareArgs& p, int i0, int i1, uint8_t* buf,
                                         uint32_t bar, volatile int* abort) {
   constexpr uint32_t K_BYTES = FS_BK * KD * 2, V_BYTES = FS_BK * VD * 2, BUF = K_BYTES > V_BYTES ? K_BYTES : V_BYTES, KA = FS_BK * 128;
@@ -262,7 +276,7 @@ __device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensor
         __syncwarp();
         fetch();
       }
-      uint32_t w[GROUPS][4][2];                  // weights of 16 keys: the second operand of the product with their values
+      uint32_t w[PARTS][GROUPS][4][2];           // weights of 16 keys: the second operand of the product with their values
 #pragma unroll
       for (int x = 0; x < GROUPS; x++) {
         if (p.softcap > 0.f) {
@@ -310,9 +324,14 @@ __device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensor
           const float e0 = ft_ex2(fmaf(s[x][n][0], sc, a0)), e1 = ft_ex2(fmaf(s[x][n][1], sc, a1)), e2 = ft_ex2(fmaf(s[x][n][2], sc, a0)), e3 = ft_ex2(fmaf(s[x][n][3], sc, a1));
           l[x][0] += e0 + e2;
           l[x][1] += e1 + e3;
-          const __nv_bfloat162 u = __floats2bfloat162_rn(e0, e1), v = __floats2bfloat162_rn(e2, e3);
-          w[x][n][0] = transposed8x8(*(const uint32_t*)&u);
-          w[x][n][1] = transposed8x8(*(const uint32_t*)&v);
+          uint32_t u[2], v[2];
+          fs_parts<PARTS>(e0, e1, u[0], u[1]);
+          fs_parts<PARTS>(e2, e3, v[0], v[1]);
+#pragma unroll
+          for (int part = 0; part < PARTS; part++) {
+            w[part][x][n][0] = transposed8x8(u[part]);
+            w[part][x][n][1] = transposed8x8(v[part]);
+          }
         }
       }
       {
@@ -345,9 +364,11 @@ __device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensor
           for (int n = 0; n < 4; n++) {
             if (n < 3) load(n + 1, d4);
 #pragma unroll
-            for (int x = 0; x < GROUPS; x++)
+            for (int part = 0; part < PARTS; part++)
 #pragma unroll
-              for (int d = 0; d < 4; d++) mma16816(o[x][4 * d4 + d], r[n & 1][d], w[x][n][0], w[x][n][1]);
+              for (int x = 0; x < GROUPS; x++)
+#pragma unroll
+                for (int d = 0; d < 4; d++) mma16816(o[x][4 * d4 + d], r[n & 1][d], w[part][x][n][0], w[part][x][n][1]);
           }
         }
         taken++;
@@ -401,17 +422,18 @@ __device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensor
 }
 
 // Keys of up to KD and values of up to VD dims (64 or 128 either): narrower ones are filled up with zeros on the chip.
-template <int KD, int VD, int STAGES>
+template <int KD, int VD, int STAGES, int PARTS>
 __global__ void __launch_bounds__(FS_THREADS, 1)
 attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ ShareArgs p,
                   uint32_t smem_bytes) {
   constexpr uint32_t Q_BYTES = FS_ROWS * KD * 2, K_BYTES = FS_BK * KD * 2, V_BYTES = FS_BK * VD * 2;
   constexpr uint32_t QA = FS_ROWS * 128, KA = FS_BK * 128;     // bytes of one 64-wide block of Q and of a K or V page
   constexpr int NK = KD / 64, NV = VD / 64;
-  // tensor-memory columns of a half (256): values of 64 have S0 0-63, S1 64-127, O 128-191, P0 192-223, P1 224-255; values of 128,
-  // whose O takes 128-255, have one S 0-63 and P0 64-95, P1 96-127
-  constexpr int NBUF = VD > 64 ? 1 : 2;
-  constexpr uint32_t P_COL0 = VD > 64 ? 64 : 192, P_STEP = 32, SUB_COLS = 256;
+  // tensor-memory columns of a half (256): values of 64 have S0 0-63, S1 64-127, O 128-191, P0 192-223, P1 224-255, and in two parts L0
+  // 0-31, L1 64-95 in the place of the scores that they come from; values of 128, whose O takes 128-255, have one S 0-63 and P0 64-95,
+  // P1 96-127, and in two parts one P 64-95 and one L 96-127
+  constexpr int NBUF = VD > 64 ? 1 : 2, PBUF = VD > 64 && PARTS == 2 ? 1 : 2;
+  constexpr uint32_t P_COL0 = VD > 64 ? 64 : 192, P_STEP = 32, L_COL0 = VD > 64 ? 96 : 0, L_STEP = 64, SUB_COLS = 256;
   constexpr int THIN_BUF = K_BYTES > V_BYTES ? K_BYTES : V_BYTES, THIN_BUFS = fs_thin_bufs<KD, VD>(), THIN_WARPS = fs_thin_warps<KD, VD>();
   static_assert(THIN_WARPS * THIN_BUFS * THIN_BUF <= 2 * Q_BYTES + STAGES * (K_BYTES + V_BYTES), "the thin tiles' buffers take the ring's place");
   static_assert(STAGES >= 4, "a half that takes every other page has its next page's scores issued ahead");
@@ -555,8 +577,10 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         const int JUg = JU0 + u0 + j * step, s = JUg % STAGES, Jg = J0 + j, sb = Jg % NBUF;
         if (!mbar_wait(b_kvfull + 8 * s, (JUg / STAGES) & 1, abort)) return false;
         // S(Jg) takes the place of S(Jg - NBUF), which the softmax threads have taken into their registers: with two buffers their
-        // P(Jg - 2) was waited for; the single buffer has a barrier for it
+        // P(Jg - 2) was waited for (and L(Jg - 2) is there until the product that reads it is complete); the single buffer has a
+        // barrier for it
         if (NBUF == 1 && !mbar_wait(b_sempty + 8 * sb, ((Jg / NBUF) & 1) ^ 1, abort)) return false;
+        if (NBUF == 2 && PARTS == 2 && Jg >= 2 && !mbar_wait(b_ofull + 8 * sb, ((Jg - 2) >> 1) & 1, abort)) return false;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
         for (int k = 0; k < KD / 16; k++)         // 16 dims a step: four steps in each 64-wide block
@@ -587,9 +611,11 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll
         for (int k = 0; k < FS_BK / 16; k++)
-          if (one)
-            umma_bf16_ta(t_sub + 128, t_sub + P_COL0 + a * P_STEP + k * 8, umma_desc_sw128_mn(sV + s * V_BYTES + k * 2048, NV > 1 ? KA : 0),
-                         idesc_o, (j | k) ? 1u : 0u);
+          if (one) {
+            const uint64_t v = umma_desc_sw128_mn(sV + s * V_BYTES + k * 2048, NV > 1 ? KA : 0);
+            umma_bf16_ta(t_sub + 128, t_sub + P_COL0 + (PBUF == 2 ? a : 0) * P_STEP + k * 8, v, idesc_o, (j | k) ? 1u : 0u);
+            if (PARTS == 2) umma_bf16_ta(t_sub + 128, t_sub + L_COL0 + (PBUF == 2 ? a : 0) * L_STEP + k * 8, v, idesc_o, 1u);
+          }
         if (one) {
           umma_commit(b_ofull + 8 * a);
           umma_commit(b_kvempty + 8 * s);
@@ -638,7 +664,7 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
 #pragma unroll 1
       for (int j = 0; j < n_mine && ok; j++) {
         const int Jg = J0 + j, a = Jg & 1, bf = Jg % NBUF, u = u0 + j * step, t = it.p0 + u;
-        uint32_t pk[32];                              // 64 weights as bfloat16 pairs: keys 2i, 2i+1
+        uint32_t pk[32], pl[32];                      // 64 weights as bfloat16 pairs: keys 2i, 2i+1, and their second parts
         ok = mbar_wait(b_sfull + 8 * bf, (Jg / NBUF) & 1, abort);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -686,10 +712,15 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             l *= factor;
             if (grow) m_ref = mx;
           }
-          // ---- the weights, into tensor memory as they come (all at once behind the last: 3% slower). The product that read this
-          // buffer's last P, two pages ago, is complete: it was issued before S(Jg), and the commit that announced S(Jg) covers every
-          // product issued before it.
-          const uint32_t t_p = t_lane + P_COL0 + a * P_STEP;
+          // ---- the weights, into tensor memory as they come (all at once behind the last: 3% slower). With two buffers the product that
+          // read this one's last P, two pages ago, is complete: it was issued before S(Jg), and the commit that announced S(Jg) covers
+          // every product issued before it.
+          const uint32_t t_p = t_lane + P_COL0 + (PBUF == 2 ? a : 0) * P_STEP, t_l = t_lane + L_COL0 + (PBUF == 2 ? a : 0) * L_STEP;
+          if (PBUF == 1 && j >= 1) {                    // the one buffer's last P and L are read when the product of the page before is complete
+            ok = mbar_wait(b_ofull + 8 * (a ^ 1), ((Jg - 1) >> 1) & 1, abort);
+            if (!ok) break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          }
           const float msc = (m_ref == -INFINITY) ? 0.f : m_ref * sc;
           uint64_t rs2 = 0ull;                          // two partial sums side by side
           const uint64_t sc2 = ft_pack2(sc, sc), nm2 = ft_pack2(-msc, -msc);
@@ -700,13 +731,19 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
             ft_unpack2(ft_fma2(ft_pack2(__uint_as_float(s[2 * k + 2]), __uint_as_float(s[2 * k + 3])), sc2, nm2), x2, x3);
             const float e0 = ft_ex2(x0), e1 = ft_ex2(x1), e2 = ft_ex2(x2), e3 = ft_ex2(x3);
             rs2 = ft_add2(rs2, ft_add2(ft_pack2(e0, e1), ft_pack2(e2, e3)));
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(e0, e1), hi = __floats2bfloat162_rn(e2, e3);
-            pk[k] = *(const uint32_t*)&lo;
-            pk[k + 1] = *(const uint32_t*)&hi;
-            if (k == 14) tmem_st16(t_p, pk);
-            if (k == 22) tmem_st8(t_p + 16, pk + 16);
+            fs_parts<PARTS>(e0, e1, pk[k], pl[k]);
+            fs_parts<PARTS>(e2, e3, pk[k + 1], pl[k + 1]);
+            if (k == 14) {
+              tmem_st16(t_p, pk);
+              if (PARTS == 2) tmem_st16(t_l, pl);
+            }
+            if (k == 22) {
+              tmem_st8(t_p + 16, pk + 16);
+              if (PARTS == 2) tmem_st8(t_l + 16, pl + 16);
+            }
           }
           tmem_st8(t_p + 24, pk + 24);
+          if (PARTS == 2) tmem_st8(t_l + 24, pl + 24);
           float ra, rb;
           ft_unpack2(rs2, ra, rb);
           l += ra + rb;
@@ -773,7 +810,7 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
   __syncthreads();
   if (warp < THIN_WARPS && !*abort) {
     const int w = blockIdx.x * THIN_WARPS + warp;
-    fs_thin<KD, VD>(&map_k, &map_v, p, p.thin_first[w], p.thin_first[w + 1], smem + warp * THIN_BUFS * THIN_BUF, b_thin + 8 * warp * THIN_BUFS, abort);
+    fs_thin<KD, VD, PARTS>(&map_k, &map_v, p, p.thin_first[w], p.thin_first[w + 1], smem + warp * THIN_BUFS * THIN_BUF, b_thin + 8 * warp * THIN_BUFS, abort);
   }
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512) : "memory");
   if (lane == 0 && *abort) atomicExch(p.err, 2);
@@ -792,8 +829,8 @@ static int fs_make_map(CUtensorMap* map, const void* base, long long n_pages, in
   return r == CUDA_SUCCESS ? 0 : SLLM_ERR_ARG - 2;
 }
 
-template <int KD, int VD, int STAGES>
-static int fs_launch(const CUtensorMap& mk, const CUtensorMap& mv, const ShareArgs& a, int workers, cudaStream_t stream) {
+template <int KD, int VD, int STAGES, int PARTS>
+static int fs_launch_parts(const CUtensorMap& mk, const CUtensorMap& mv, const ShareArgs& a, int workers, cudaStream_t stream) {
   // what the kernel lays out after aligning to 1 KB; one block on an SM
   constexpr size_t need = 2 * FS_ROWS * KD * 2 + STAGES * FS_BK * (KD + VD) * 2 + (4 + 2 * STAGES + 16 + 2 + fs_thin_warps<KD, VD>() * fs_thin_bufs<KD, VD>()) * 8 +
                           FS_CACHED * sizeof(ShareItem);
@@ -801,15 +838,21 @@ static int fs_launch(const CUtensorMap& mk, const CUtensorMap& mv, const ShareAr
   constexpr size_t smem = need + 1024 <= room ? need + 1024 : room;     // the slack for the alignment, as far as it fits
   static_assert(need + 512 <= smem, "the block of this head width does not fit an SM");
   static SllmPerDevice allowed;
-  const cudaError_t e = sllm_allow_smem(allowed, attn_share_kernel<KD, VD, STAGES>, smem);
+  const cudaError_t e = sllm_allow_smem(allowed, attn_share_kernel<KD, VD, STAGES, PARTS>, smem);
   if (e != cudaSuccess) return (int)e;
-  return (int)sllm_launch(attn_share_kernel<KD, VD, STAGES>, dim3(workers), dim3(FS_THREADS), smem, stream, mk, mv, a, (uint32_t)smem);
+  return (int)sllm_launch(attn_share_kernel<KD, VD, STAGES, PARTS>, dim3(workers), dim3(FS_THREADS), smem, stream, mk, mv, a, (uint32_t)smem);
+}
+template <int KD, int VD, int STAGES>
+static int fs_launch(const CUtensorMap& mk, const CUtensorMap& mv, const ShareArgs& a, int workers, int exact, cudaStream_t stream) {
+  return exact ? fs_launch_parts<KD, VD, STAGES, 2>(mk, mv, a, workers, stream) : fs_launch_parts<KD, VD, STAGES, 1>(mk, mv, a, workers, stream);
 }
 
-// The plan is one for tiles of 256 rows in halves, with thin ones of at most FS_THIN rows; part: plan->part_rows * (vd + 2) floats.
+// The plan is one for tiles of 256 rows in halves, with thin ones of at most FS_THIN rows; part: plan->part_rows * (vd + 2) floats; exact:
+// the weights go into the product with the values in two parts.
 SLLM_EXPORT int sllm_share_attn_tc_bf16(const SharePlanDev* plan, const void* q, int q_ld, const int* tok_pos, const int* block_table,
                                         int max_pages, const void* kpages, const void* vpages, long long n_pages, float* part, void* out,
-                                        const float* sink, int hd, int vd, float scale, float softcap, int* err, cudaStream_t stream) {
+                                        const float* sink, int hd, int vd, float scale, float softcap, int exact, int* err,
+                                        cudaStream_t stream) {
   if (hd < 8 || hd > 128 || hd % 8 || vd < 8 || vd > 128 || vd % 8 || (q_ld & 7) || !share_call_ok(*plan, 2 * FS_ROWS, q_ld, hd, n_pages, max_pages, part) ||
       plan->thin_warps != (hd <= 64 && vd <= 64 ? fs_thin_warps<64, 64>() : hd > 64 && vd > 64 ? fs_thin_warps<128, 128>() : fs_thin_warps<128, 64>()) || !share_aligned(q, 16) ||
       !share_aligned(kpages, 16) || !share_aligned(vpages, 16) || !share_aligned(out, 16))
@@ -820,7 +863,8 @@ SLLM_EXPORT int sllm_share_attn_tc_bf16(const SharePlanDev* plan, const void* q,
   int rc = fs_make_map(&mk, kpages, n_pages, plan->G, hd);
   if (rc == 0) rc = fs_make_map(&mv, vpages, n_pages, plan->G, vd);
   if (rc) return rc;
-  if (vd <= 64) rc = hd <= 64 ? fs_launch<64, 64, 10>(mk, mv, a, plan->workers, stream) : fs_launch<128, 64, 6>(mk, mv, a, plan->workers, stream);
-  else rc = hd <= 64 ? fs_launch<64, 128, 7>(mk, mv, a, plan->workers, stream) : fs_launch<128, 128, 5>(mk, mv, a, plan->workers, stream);
+  const int workers = plan->workers;
+  if (vd <= 64) rc = hd <= 64 ? fs_launch<64, 64, 10>(mk, mv, a, workers, exact, stream) : fs_launch<128, 64, 6>(mk, mv, a, workers, exact, stream);
+  else rc = hd <= 64 ? fs_launch<64, 128, 7>(mk, mv, a, workers, exact, stream) : fs_launch<128, 128, 5>(mk, mv, a, workers, exact, stream);
   return rc ? rc : share_merge_run<bf16>(*plan, part, out, sink, vd, stream);
 }

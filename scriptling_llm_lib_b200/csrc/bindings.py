@@ -1739,7 +1739,7 @@ class SharedAttention:
         p, n = c_void_p, c_int
         for fn in (self._attn, self._attn_tc):
             if fn is not None:      # (addresses and sizes go over as plain integers: half the price of an object for each)
-                fn.restype, fn.argtypes = c_int, [p, p, n, p, p, n, p, p, c_longlong, p, p, p, n, n, c_float, c_float, p, p]
+                fn.restype, fn.argtypes = c_int, [p, p, n, p, p, n, p, p, c_longlong, p, p, p, n, n, c_float, c_float, n, p, p]
 
     @staticmethod
     def takes(head_dim: int, v_dim: int, rep: int = 1) -> bool:
@@ -1765,12 +1765,15 @@ class SharedAttention:
         smem += 2 * PAGE * (head_dim + v_dim + 32 // size) * size
         return TileShape(rows=64, workers=(2 if smem <= 112 * 1024 else 1) * sm_count, costs=((4, 0.25), (16, 0.5)), min_pages=1)
 
-    def attn(self, q, out, tok_pos, block_table, kpages, vpages, plan, part, scale, err_flag, softcap=None, sink=None):
+    def attn(self, q, out, tok_pos, block_table, kpages, vpages, plan, part, scale, err_flag, softcap=None, sink=None, exact_weights=False):
         """out [T, H * vd] = attention of the step's queries q [T, H * hd or more] (rows may stand apart) at positions tok_pos over the
         paged keys [pages, G, 64, hd] and values [pages, G, 64, vd] that block_table [sequences, pages] names; this step's own keys are
         there already. `plan`: a SharePlan for this step's rows, heads and `shape`; `part`: float32 scratch of plan.part_floats(vd)
         elements. `softcap`: a score s becomes softcap * tanh(s / softcap) before the softmax; `sink` float32 [H]: exp(sink[h]) joins
-        head h's denominator with no key and no value. A page id outside the storage or a position outside the table sets err_flag."""
+        head h's denominator with no key and no value. A page id outside the storage or a position outside the table sets err_flag.
+        bfloat16 widths up to 128 in multiples of 8 round the softmax weights to bfloat16 for the product with the values, as prompt
+        attention at 64 and 128 and decode attention of grouped heads do; with `exact_weights` they go in as two bfloat16 parts, 2^-16 of a
+        weight, which costs 2 to 5% at values of up to 64 and 7 to 25% past them. Everything else keeps them in float32."""
         H, G, T = plan.n_heads, plan.n_kv, plan.n_rows
         ks, vs, qs = kpages.shape, vpages.shape, q.shape
         if len(ks) != 4 or len(vs) != 4 or ks[:3] != vs[:3] or ks[1] != G or ks[2] != PAGE:
@@ -1795,7 +1798,8 @@ class SharedAttention:
         _check((self._attn_tc if shape.halves else self._attn)(
             laid_out, q.data_ptr(), ld, _address(tok_pos, torch.int32), _address(block_table, torch.int32), block_table.shape[1],
             _address(kpages, self.dtype), _address(vpages, self.dtype), ks[0], _address(part, torch.float32), _address(out, self.dtype),
-            _address(sink, torch.float32), hd, vd, c_float(scale), c_float(softcap or 0.0), _address(err_flag, torch.int32), _stream()), "share_attn")
+            _address(sink, torch.float32), hd, vd, c_float(scale), c_float(softcap or 0.0), 1 if exact_weights else 0, _address(err_flag, torch.int32), _stream()),
+            "share_attn")
 
 
 class PageKernels:

@@ -320,12 +320,24 @@ class Attention(Mixer):
         plan = getattr(ctx, "share_plan", None)
         return None if self.span or plan is None else plan(unit, self.n_heads, self.head_dim, self.v_dim)
 
+    def rounds_weights(self, decode: bool) -> bool:
+        """Whether the bfloat16 kernels that read each sequence for itself round this layer's softmax weights to bfloat16 for their product
+        with the values (tensor cores) in a decode step, or in one of runs; the others keep them in float32, and a step whose sequences
+        share pages keeps them where they do."""
+        widths = self.head_dim, self.v_dim
+        if self.general:
+            return DecodeKernels.general_takes(*widths) if decode else PrefillAttentionTC.takes(*widths) or PrefillAttentionMMA.takes(*widths)
+        plain = not self.other_widths and self.head_dim in PrefillAttentionTC.HEAD_DIMS
+        return plain and not (decode and self.n_heads == self.n_kv_heads)
+
     def _attend_shared(self, plan, q, ctx, kpages, vpages, block_table):
-        """The step's queries (the leading columns of `q`) over pages that are read once for all sequences that share them."""
+        """The step's queries (the leading columns of `q`) over pages that are read once for all sequences that share them. (In bfloat16 the
+        queries come rotated and rounded, as those of prompt steps do: off by 2^-8 of an element, where the decode kernel that rotates by
+        itself keeps them in float32 for one query head on a key/value head. Queries of two parts would double the scores' products.)"""
         attn = torch.empty((q.shape[0], self.n_heads * self.v_dim), dtype=q.dtype, device=q.device)
         part = torch.empty((plan.part_floats(self.v_dim),), dtype=torch.float32, device=q.device)
         ctx.kernels.shared.attn(q, attn, ctx.tok_pos, block_table, kpages, vpages, plan, part, self.scale, ctx.err_flag, softcap=self.softcap,
-                                sink=self.sink)
+                                sink=self.sink, exact_weights=not self.rounds_weights(ctx.is_decode))
         return attn
 
     def _attend(self, qkv, x, ctx, kpages, vpages, block_table, fast_decode, fusion, writes, unit=None):
