@@ -138,6 +138,7 @@ __device__ __forceinline__ void fs_thin(const CUtensorMap* map_k, const CUtensor
     hbase = base;
     if (base + lane < i1) {
       held = share_item(p, base + lane);
+      share_check(p, held);
       tok_first = p.toks[held.tok0];
       const int* row = p.block_table + (size_t)held.seq * p.max_pages;
 #pragma unroll
@@ -503,6 +504,7 @@ attn_share_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_consta
     bool ok = true;
     for (int i = i0; ok && i < i1; i++) {
       const ShareItem it = item(i);
+      share_check(p, it);
       const int* row = p.block_table + (size_t)it.seq * p.max_pages;
       for (int t0 = it.p0; ok && t0 < it.p1; t0 += 32) {
         // (a page that is none is fetched past the storage's end: zeros)

@@ -329,6 +329,7 @@ __global__ void __launch_bounds__(256, BLOCKS) share_fma_kernel(ShareArgs p, int
   const int i1 = p.first[blockIdx.x + 1];
   for (int i = p.first[blockIdx.x]; i < i1; i++) {
     const ShareItem it = share_item(p, i);
+    if (threadIdx.x == 0) share_check(p, it);
     const int n_rows = it.n_tok * (p.H / p.G);
     if (n_rows <= 4) share_few_item<A>(p, it, stages, share_sm);
     else if (n_rows <= 16) share_fma_item<A, NG, 1>(p, it, stages, share_sm);

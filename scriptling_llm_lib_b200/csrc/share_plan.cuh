@@ -46,14 +46,19 @@ __device__ __forceinline__ ShareItem share_item(const ShareArgs& p, int i) {
   ShareItem it;
   it.tok0 = a.x;
   it.n_tok = a.y;
-  it.last = a.z < 0 ? SHARE_NODE : min(p.tok_pos[a.z], SHARE_NODE - 1);
+  it.last = a.z < 0 ? SHARE_NODE : max(-1, min(p.tok_pos[a.z], SHARE_NODE - 1));
   it.g = a.w;
   it.p0 = b.x;
-  const int end = it.last / SLLM_PAGE + 1;         // (a plan may be older than the step, and its sequences longer now)
-  it.p1 = b.y < 0 || b.y > end ? end : b.y;
+  // (a plan may be older than the step, and its sequences longer now; of a position outside the table, the pages that are there)
+  const int end = (it.last + SLLM_PAGE) / SLLM_PAGE, most = it.last == SHARE_NODE ? end : min(end, p.max_pages);
+  it.p1 = b.y < 0 || b.y > most ? most : b.y;
   it.part0 = b.z;
   it.seq = b.w;
   return it;
+}
+// an item's last token may stand outside the table: one of those that read the item says so
+__device__ __forceinline__ void share_check(const ShareArgs& p, const ShareItem& it) {
+  if (it.last < 0 || (it.last != SHARE_NODE && it.last / SLLM_PAGE >= p.max_pages)) atomicExch(p.err, SHARE_ERR_PAGE);
 }
 // the position up to which row `rho` of an item's tile sees keys; -1 for a row past the tile's end
 __device__ __forceinline__ int share_sees(const ShareItem& it, int rho, int rep) {
