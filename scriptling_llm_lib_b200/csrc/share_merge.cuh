@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(32 * SHARE_MERGE_WARPS, SPLIT ? 2 : 3) share_m
     const int d = 4 * (j + warp * J);
     if (d < p.vd) st4(out + d, make_float4(b.x * inv, b.y * inv, b.z * inv, b.w * inv));
   } else {
-    const float c = exp2f(M0 - top0);
+    const float c = M == -INFINITY ? 0.f : exp2f(M0 - top0);      // (nothing seen: 2^-sink may be infinite, and times 0 is NaN)
     all = fmaf(c, den, all);
     const float inv = all > 0.f || all != all ? c / all : 0.f;
 #pragma unroll
