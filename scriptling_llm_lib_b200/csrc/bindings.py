@@ -8,6 +8,7 @@ CUDA device is an error.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import struct
 from ctypes import c_float, c_int, c_longlong, c_void_p
@@ -1774,6 +1775,9 @@ class SharedAttention:
         bfloat16 widths up to 128 in multiples of 8 round the softmax weights to bfloat16 for the product with the values, as prompt
         attention at 64 and 128 and decode attention of grouped heads do; with `exact_weights` they go in as two bfloat16 parts, 2^-16 of a
         weight, which costs 2 to 5% at values of up to 64 and 7 to 25% past them. Everything else keeps them in float32."""
+        if not 0.0 < scale < math.inf or not 0.0 <= (softcap or 0.0) < math.inf:
+            # (the tensor-core form takes a row's maximum before the scale, and caps by quotients of the two)
+            raise KernelError(f"shared attention: a scale above 0 and a cap above 0 (or none), both finite, not {scale} and {softcap}")
         H, G, T = plan.n_heads, plan.n_kv, plan.n_rows
         ks, vs, qs = kpages.shape, vpages.shape, q.shape
         if len(ks) != 4 or len(vs) != 4 or ks[:3] != vs[:3] or ks[1] != G or ks[2] != PAGE:

@@ -4,6 +4,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
+from scriptling_llm_lib_b200.csrc.bindings import KernelError, SharedAttention
 from scriptling_llm_lib_b200.parts.attention import Attention
 
 
@@ -29,3 +30,11 @@ def test_a_step_that_shares_pages_keeps_the_weights_that_each_sequence_for_itsel
     for ctx.is_decode in (True, False):
         part._attend_shared(plan, torch.zeros(3, part.n_heads * part.head_dim), ctx, None, None, None)
     assert seen == [not decode, not runs]
+
+
+@pytest.mark.parametrize("scale, softcap", [(0.0, None), (-0.125, None), (float("nan"), None), (float("inf"), None), (0.125, -30.0),
+                                            (0.125, float("nan")), (0.125, float("inf"))])
+def test_scales_and_caps_that_are_no_numbers_above_zero_are_refused(scale, softcap):
+    ops = SharedAttention.__new__(SharedAttention)            # (no library is loaded for a refusal)
+    with pytest.raises(KernelError, match="scale above 0"):
+        ops.attn(None, None, None, None, None, None, None, None, scale, None, softcap=softcap)
