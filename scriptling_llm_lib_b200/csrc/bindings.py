@@ -1747,13 +1747,18 @@ class SharedAttention:
         """Keys and values of these widths, `rep` query heads on a key/value head."""
         return all(w % 4 == 0 and 4 <= w <= 256 for w in (head_dim, v_dim)) and 1 <= rep <= SharedAttention.MAX_REP
 
+    @staticmethod
+    def tensor_cores(dtype: torch.dtype, head_dim: int, v_dim: int) -> bool:
+        """Whether these widths run on the tensor cores; the others, and all in 32-bit, on FP32 FMA."""
+        return dtype == torch.bfloat16 and all(w % 8 == 0 and w <= 128 for w in (head_dim, v_dim))
+
     def shape(self, head_dim: int, v_dim: int, sm_count: int | None = None) -> TileShape:
         """The tiles of a plan for these widths."""
         if not self.takes(head_dim, v_dim):
             raise KernelError(f"shared attention takes widths in multiples of 4 up to 256, not keys of {head_dim} and values of {v_dim}")
         if sm_count is None:
             sm_count = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
-        if self.dtype == torch.bfloat16 and all(w % 8 == 0 and w <= 128 for w in (head_dim, v_dim)):
+        if self.tensor_cores(self.dtype, head_dim, v_dim):
             # tcgen05, and mma.sync for thin tiles. What an item and a thin page cost beside a page of 256 rows (1.05 us): measured
             # over 17 decode steps of 2 to 64 sequences and prompts of 5 to 32; an item at 6 or 4 is 5% slower over them, half or twice of
             # the others 3 to 20%

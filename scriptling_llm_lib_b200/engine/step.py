@@ -18,7 +18,7 @@ import torch
 
 from ..cache import PAGE, PlanCapacity, SequenceCache, SharePlan, pages_for, share_pays
 from ..config.registry import architecture_for, architecture_name, load_config
-from ..csrc.bindings import CastKernels, KernelSet, SplitGemm
+from ..csrc.bindings import CastKernels, KernelSet, SharedAttention, SplitGemm
 from ..parts.base import Mixer, Part
 from ..parts.linear import linears
 from ..weights.loader import load_weights, stored_to_kept
@@ -237,7 +237,7 @@ class Engine:
         self.cache = SequenceCache(self.model.cache_needs(), self.model.state_needs(), n_slots, n_pages, self.dtype,
                                    self.device)
         self.cache.err_flag = self.err_flag
-        self._sharing: dict[tuple[int, int, int], int] | None = None
+        self._sharing: dict[bool, dict[tuple[int, int, int, int], int]] = {}
         self.max_positions = min(self.layout.max_positions, n_pages * PAGE)
         self.model.prepare(self.max_positions, self.device)
         padded = 1
@@ -330,26 +330,25 @@ class Engine:
         cache = self.cache
         if not cache.shares_pages or len(slots) < 2:
             return False
-        return any(cache.groups[g].pool.n_shared and share_pays(cache.share_tree(g, slots), held, new, heads, cache.groups[g].need.kv_heads, width,
-                                                                self.dtype == torch.float32, 0 if kept else layers)
-                   for (g, heads, width), layers in self._share_groups().items())
+        return any(cache.groups[g].pool.n_shared and share_pays(cache.share_tree(g, slots), held, new, heads, cache.groups[g].need.kv_heads, dim + v_dim,
+                                                                not SharedAttention.tensor_cores(self.dtype, dim, v_dim), 0 if kept else layers)
+                   for (g, heads, dim, v_dim), layers in self._share_groups(max(new) <= 1).items())
 
-    def _share_groups(self) -> dict[tuple[int, int, int], int]:
-        """Cache groups with layers whose attention can read shared pages once: (group, query heads, widths of a key and a value) ->
-        how many such layers a step goes through."""
-        if self._sharing is None:
-            groups, ops = {}, self.kernels.shared
+    def _share_groups(self, decode: bool) -> dict[tuple[int, int, int, int], int]:
+        """Cache groups with layers whose attention can read shared pages once, in decode steps or in steps of runs: (group, query heads,
+        widths of a key and of a value) -> how many such layers a step goes through."""
+        if decode not in self._sharing:
+            groups, ops = {}, SharedAttention
             for e in self.layout.schedule:
                 g = self.cache.group_of_unit.get(e.cache_unit)
                 if g is None or self.cache.groups[g].need.kind != "full":
                     continue
                 for part in self.model.blocks[e.layer].parts():
-                    heads = part.shares_pages() if isinstance(part, Mixer) else None
+                    heads = part.shares_pages(self.dtype, decode) if isinstance(part, Mixer) else None
                     if heads is not None and ops.takes(heads[1], heads[2], heads[0] // self.cache.groups[g].need.kv_heads):
-                        key = (g, heads[0], heads[1] + heads[2])
-                        groups[key] = groups.get(key, 0) + 1
-            self._sharing = groups
-        return self._sharing
+                        groups[g, *heads] = groups.get((g, *heads), 0) + 1
+            self._sharing[decode] = groups
+        return self._sharing[decode]
 
     def tickets(self, n: int) -> torch.Tensor:
         """Zeroed int32 counters that kernels of one stream draw tickets from and leave zero (which

@@ -306,8 +306,22 @@ class Attention(Mixer):
         path = self.out.fold_path(ctx, rows, ctx.dtype, finishing=True)
         return path is not None and (ctx.is_decode or path == "tiles")
 
-    def shares_pages(self):
-        return None if self.span else (self.n_heads, self.head_dim, self.v_dim)
+    def shares_pages(self, dtype=None, decode=False):
+        widths = self.head_dim, self.v_dim
+        if self.span:
+            return None
+        if dtype == torch.bfloat16 and not SharedAttention.tensor_cores(dtype, *widths):
+            # shared pages on FP32 FMA against each sequence for itself on the tensor cores: slower however much is shared (32 heads on 8, keys of
+            # 192 and values of 128, 16 runs of 150 tokens behind 4,000 3,782 us, 334 each for itself, 48 of 12 behind 2,000 565, 368; 64
+            # single ones behind 4,000 with a cap 288, 190). Where those are on FMA too, the costs are those of 32-bit: 64 single ones without a
+            # cap 288, 851; 16 heads of 256 on 4, 16 runs of 20 behind 2,000 271, 1,781.
+            if self.general:
+                other = DecodeKernels.general_takes(*widths) if decode else PrefillAttentionTC.takes(*widths) or PrefillAttentionMMA.takes(*widths)
+            else:
+                other = not decode and PrefillAttentionTC.takes(*widths, exact_weights=True)
+            if other:
+                return None
+        return self.n_heads, *widths
 
     def scratch_bytes(self, rows):
         """The partial results of attention over pages that a step's sequences share."""
@@ -318,7 +332,8 @@ class Attention(Mixer):
     def _share_plan(self, ctx, unit):
         """The step's plan where its sequences share pages and this layer sees all of them."""
         plan = getattr(ctx, "share_plan", None)
-        return None if self.span or plan is None else plan(unit, self.n_heads, self.head_dim, self.v_dim)
+        widths = self.shares_pages(ctx.dtype, ctx.is_decode) if plan is not None else None
+        return None if widths is None else plan(unit, *widths)
 
     def rounds_weights(self, decode: bool) -> bool:
         """Whether the bfloat16 kernels that read each sequence for itself round this layer's softmax weights to bfloat16 for their product

@@ -111,9 +111,9 @@ class Mixer(Part):
     def state_need(self) -> StateNeed | None:
         return None
 
-    def shares_pages(self) -> tuple[int, int, int] | None:
+    def shares_pages(self, dtype=None, decode: bool = False) -> tuple[int, int, int] | None:
         """(query heads, key width, value width) of a mixer that reads the pages of a step's sequences once where they share them
-        (`ctx.share_plan`); None: each sequence is read for itself."""
+        (`ctx.share_plan`), in decode steps or in steps of runs of this dtype (None: in any); None: each sequence is read for itself."""
         return None
 
     def forward(self, x, ctx, unit: int, writes: bool):
