@@ -1,7 +1,7 @@
 """CUDA graphs of the decode step.
 
 A decode step launches a few hundred small kernels whose sizes depend only on the batch size, so
-it is captured once per (padded batch size, block-table width, whether its sequences share pages) and replayed: the step's index
+it is captured once per (padded batch size, block-table width, layers that read shared pages once) and replayed: the step's index
 arrays live in one static device buffer that is refreshed from pinned host memory before each
 replay. Rows added to fill the batch up to its padded size read and write a spare cache page and a
 spare state slot of their own, so they change nothing a real row sees.
@@ -24,7 +24,7 @@ def _next_pow2(n: int) -> int:
 
 
 class DecodeGraph:
-    def __init__(self, engine, batch: int, width: int, shared: bool = False):
+    def __init__(self, engine, batch: int, width: int, shared: tuple = ()):
         from .step import SharedStep, StepContext
         self.engine, self.batch, self.width = engine, batch, width
         n_groups = len(engine.cache.groups)
@@ -47,7 +47,7 @@ class DecodeGraph:
         ctx.is_decode = True
         ctx.max_pages = width
         if shared:                  # plans with room for any batch; the warm-up's is of spare rows alone
-            ctx.share = SharedStep(engine, [], [], [], padded=B)
+            ctx.share = SharedStep(engine, shared, [], [], [], padded=B)
         self.ctx = ctx
         self._fill_host([], [], [], [])
         self.dev.copy_(self.host)
@@ -160,13 +160,14 @@ class DecodeGraphs:
     def clear(self):
         self.graphs.clear()
 
-    def run(self, ids, pos0, slots, tables, shared: bool = False) -> torch.Tensor:
-        """`shared`: the sequences share pages; the step is captured a second time, with attention that reads those once."""
+    def run(self, ids, pos0, slots, tables, shared: tuple = ()) -> torch.Tensor:
+        """`shared`: the layers (as `Engine._shares` names them) that read pages which the sequences share once; the step is captured
+        again for them."""
         need = max(1, max(t.shape[1] for t in tables)) if tables else 1
         cap = -(-self.engine.max_positions // PAGE)
         width = min(max(8, _next_pow2(need)), max(cap, need))
         batch = _next_pow2(ids.shape[0] if isinstance(ids, torch.Tensor) else len(ids))
-        key = (batch, width, "shared") if shared else (batch, width)
+        key = (batch, width, "shared", *shared) if shared else (batch, width)
         g = self.graphs.pop(key, None)
         if g is None:
             while len(self.graphs) >= self.MAX_GRAPHS:

@@ -146,12 +146,12 @@ class StepContext:
 
 
 class SharedStep:
-    """What a step whose sequences share pages keeps for its attention layers: a plan for every cache group and head layout that asks,
-    made when the first layer does. A captured decode step's plans have room for any of its batches and are laid out again
+    """What a step whose sequences share pages keeps for its attention layers: a plan for every cache group and head layout among `keys`
+    that asks, made when the first layer does. A captured decode step's plans have room for any of its batches and are laid out again
     (`refresh`) when slots come to hold other pages or the sequences have grown by a sixteenth."""
 
-    def __init__(self, engine: "Engine", slots, held, new, padded: int | None = None):
-        self.engine, self.padded = engine, padded
+    def __init__(self, engine: "Engine", keys, slots, held, new, padded: int | None = None):
+        self.engine, self.padded, self.keys = engine, padded, frozenset(keys)
         self.plans: dict[tuple, SharePlan | None] = {}
         self.laid_out: dict[tuple, tuple] = {}
         self.staging: dict[tuple, torch.Tensor] = {}
@@ -160,10 +160,8 @@ class SharedStep:
     def plan(self, group: int, n_heads: int, head_dim: int, v_dim: int):
         key = (group, n_heads, head_dim, v_dim)
         if key not in self.plans:
-            need, ops = self.engine.cache.groups[group].need, self.engine.kernels.shared
-            takes = need.kind == "full" and ops.takes(head_dim, v_dim, n_heads // need.kv_heads)
-            plan = self._build(key) if takes else None
-            if plan is not None and 4 * plan.part_floats(v_dim) > ops.SCRATCH_BYTES:       # a long prompt step of many heads
+            plan = self._build(key) if key in self.keys else None
+            if plan is not None and 4 * plan.part_floats(v_dim) > SharedAttention.SCRATCH_BYTES:       # a long prompt step of many heads
                 plan = None
             self.plans[key] = plan
         return self.plans[key]
@@ -324,15 +322,16 @@ class Engine:
         self.model.prepare(self.max_positions, self.device)
         return moved
 
-    def _shares(self, slots, held, new, kept: bool = False) -> bool:
-        """Whether a step of these sequences is to go by the plans of `SharedStep`: pages that it need not read again are worth the
-        partial results that reading them once leaves, and, unless a captured step keeps it, the plan."""
+    def _shares(self, slots, held, new, kept: bool = False) -> tuple:
+        """The layers of a step of these sequences that are to go by the plans of `SharedStep`, as (cache group, query heads, widths of a key
+        and of a value): those for which the pages that need not be read again are worth the partial results that reading them once
+        leaves, and, unless a captured step keeps it, the plan."""
         cache = self.cache
         if not cache.shares_pages or len(slots) < 2:
-            return False
-        return any(cache.groups[g].pool.n_shared and share_pays(cache.share_tree(g, slots), held, new, heads, cache.groups[g].need.kv_heads, dim + v_dim,
-                                                                not SharedAttention.tensor_cores(self.dtype, dim, v_dim), 0 if kept else layers)
-                   for (g, heads, dim, v_dim), layers in self._share_groups(max(new) <= 1).items())
+            return ()
+        return tuple((g, heads, dim, v_dim) for (g, heads, dim, v_dim), layers in self._share_groups(max(new) <= 1).items()
+                     if cache.groups[g].pool.n_shared and share_pays(cache.share_tree(g, slots), held, new, heads, cache.groups[g].need.kv_heads, dim + v_dim,
+                                                                     not SharedAttention.tensor_cores(self.dtype, dim, v_dim), 0 if kept else layers))
 
     def _share_groups(self, decode: bool) -> dict[tuple[int, int, int, int], int]:
         """Cache groups with layers whose attention can read shared pages once, in decode steps or in steps of runs: (group, query heads,
@@ -563,8 +562,9 @@ class Engine:
         ctx.token_ids, ctx.tok_pos, ctx.tok_seq, ctx.seq_start, ctx.seq_pos0, ctx.slots, ctx.want_rows, ctx.seq_pos_after = views[:8]
         ctx.block_tables = [v.view(B, t.shape[1]) for v, t in zip(views[8:], tables)]
         ctx.is_decode = bool((lens_a == 1).all())
-        if self._shares(slots, pos0, lens):
-            ctx.share = SharedStep(self, slots, pos0, lens)
+        shared = self._shares(slots, pos0, lens)
+        if shared:
+            ctx.share = SharedStep(self, shared, slots, pos0, lens)
         ctx.seq_lens_host = [int(n) for n in lens]
         ctx.from_start = not pos0_a.any()
         ctx.max_pages = int(-(-(int((pos0_a + lens_a).max())) // PAGE))

@@ -90,3 +90,17 @@ def test_wide_bfloat16_runs_are_not_charged_the_tensor_cores_price():
         held = [8040] * n
         eng = engine([part] * 24, BF16, [table(n, 125, 4)], held, 8)
         assert bool(eng._shares(list(range(n)), held, [new] * n, kept=new == 1)) is want
+
+
+def test_each_layer_shares_pages_by_its_own_gain():
+    """Two kinds of layers in a step: eight keys a token that 16 sequences share, and one. Reading the one once for all is worth less than the
+    partial results that it leaves; only the layers that gain have a plan, and only they are captured for it."""
+    from scriptling_llm_lib_b200.engine.step import SharedStep
+    n, held = 16, [4040] * 16
+    eng = engine([layer(32, 32, 64), layer(32, 1, 64)], BF16, [table(n, 62, 4)] * 2, held, 32)
+    eng.cache.groups[1].need = SimpleNamespace(kind="full", kv_heads=1)
+    shared = eng._shares(list(range(n)), held, [1] * n, kept=True)
+    assert shared == ((0, 32, 64, 64),)
+    step = SharedStep(eng, shared, list(range(n)), held, [1] * n)
+    step._build = lambda key: SimpleNamespace(part_floats=lambda v_dim: 0, key=key)
+    assert step.plan(0, 32, 64, 64).key == (0, 32, 64, 64) and step.plan(1, 32, 64, 64) is None
