@@ -121,6 +121,25 @@ def share_pays(tree, held, new, n_heads: int, n_kv: int, width: int, floats: boo
     return by_tree < 0.9 * alone
 
 
+def scratch_rows(rows: int) -> int:
+    """Rows of the scratch that `rows` partial results take: whole groups of 32."""
+    return -(-max(1, rows) // 32) * 32
+
+
+def most_part_rows(tree, new, n_heads: int, n_kv: int, shape: TileShape) -> int:
+    """Partial results that a plan for these sequences leaves at most: those of every tile, and of a tile more for each place that a
+    block's or a warp's list is cut at."""
+    order, nodes, _ = tree
+    new, rep = np.asarray(new, dtype=np.int64)[order], n_heads // n_kv
+    ends = np.concatenate([[0], np.cumsum(new)])
+    n = np.concatenate([new, [ends[hi] - ends[lo] for lo, hi, _, _ in nodes]]).astype(np.int64)
+    per = shape.rows // rep
+    rest = n % per * rep                       # rows of the tile that is not full; a full one leaves a result for each row unless it is half
+    twice = lambda rows: np.where((rows > shape.thin_rows) & (rows <= shape.rows // 2) & shape.halves, 2 * rows, rows)      # noqa: E731
+    tiles = n // per * int(twice(np.int64(per * rep))) + twice(rest)
+    return int(n_kv * tiles.sum()) + shape.workers * (min(shape.rows, 2 * int(n.max(initial=0)) * rep) + shape.thin_warps * shape.thin_rows)
+
+
 class SharePlan:
     """The items of one attention over a step's rows, in one int32 buffer on the device. Good for every layer of the step with these
     head counts, and for later steps of the same sequences with as many new tokens each: a leaf's last item goes on to where its
@@ -186,7 +205,7 @@ class SharePlan:
 
     @property
     def scratch_rows(self) -> int:
-        return -(-max(1, self.capacity.rows) // 32) * 32
+        return scratch_rows(self.capacity.rows)
 
     @classmethod
     def build(cls, table, held, new, n_heads: int, n_kv: int, shape: TileShape, device, capacity=None, tree=None) -> "SharePlan":

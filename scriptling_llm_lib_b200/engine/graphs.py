@@ -16,7 +16,7 @@ import torch
 from ..cache.needs import PAGE
 
 
-def _next_pow2(n: int) -> int:
+def next_pow2(n: int) -> int:
     p = 1
     while p < n:
         p <<= 1
@@ -165,8 +165,8 @@ class DecodeGraphs:
         again for them."""
         need = max(1, max(t.shape[1] for t in tables)) if tables else 1
         cap = -(-self.engine.max_positions // PAGE)
-        width = min(max(8, _next_pow2(need)), max(cap, need))
-        batch = _next_pow2(ids.shape[0] if isinstance(ids, torch.Tensor) else len(ids))
+        width = min(max(8, next_pow2(need)), max(cap, need))
+        batch = next_pow2(ids.shape[0] if isinstance(ids, torch.Tensor) else len(ids))
         key = (batch, width, "shared", *shared) if shared else (batch, width)
         g = self.graphs.pop(key, None)
         if g is None:

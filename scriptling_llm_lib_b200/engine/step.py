@@ -16,13 +16,13 @@ from itertools import chain
 import numpy as np
 import torch
 
-from ..cache import PAGE, PlanCapacity, SequenceCache, SharePlan, pages_for, share_pays
+from ..cache import PAGE, PlanCapacity, SequenceCache, SharePlan, most_part_rows, pages_for, scratch_rows, share_pays
 from ..config.registry import architecture_for, architecture_name, load_config
 from ..csrc.bindings import CastKernels, KernelSet, SharedAttention, SplitGemm
 from ..parts.base import Mixer, Part
 from ..parts.linear import linears
 from ..weights.loader import load_weights, stored_to_kept
-from .graphs import DecodeGraphs
+from .graphs import DecodeGraphs, next_pow2
 from .layout import ModelLayout
 from .model import DecoderModel
 
@@ -160,10 +160,7 @@ class SharedStep:
     def plan(self, group: int, n_heads: int, head_dim: int, v_dim: int):
         key = (group, n_heads, head_dim, v_dim)
         if key not in self.plans:
-            plan = self._build(key) if key in self.keys else None
-            if plan is not None and 4 * plan.part_floats(v_dim) > SharedAttention.SCRATCH_BYTES:       # a long prompt step of many heads
-                plan = None
-            self.plans[key] = plan
+            self.plans[key] = self._build(key) if key in self.keys else None
         return self.plans[key]
 
     def _build(self, key, device=True):
@@ -325,13 +322,23 @@ class Engine:
     def _shares(self, slots, held, new, kept: bool = False) -> tuple:
         """The layers of a step of these sequences that are to go by the plans of `SharedStep`, as (cache group, query heads, widths of a key
         and of a value): those for which the pages that need not be read again are worth the partial results that reading them once
-        leaves, and, unless a captured step keeps it, the plan."""
-        cache = self.cache
+        leaves, and, unless a captured step keeps it, the plan. Layers whose partial results would take more than
+        `SharedAttention.SCRATCH_BYTES` are none of them (`prompt_step` cuts its portions so that they fit)."""
+        return tuple(key for key, scratch in self._gains(slots, held, new, kept) if scratch <= SharedAttention.SCRATCH_BYTES)
+
+    def _gains(self, slots, held, new, kept: bool = False) -> list[tuple[tuple, int]]:
+        """The layers that `_shares` speaks of, each with the bytes that its partial results take at most (a captured step's: of any plan)."""
+        cache, out = self.cache, []
         if not cache.shares_pages or len(slots) < 2:
-            return ()
-        return tuple((g, heads, dim, v_dim) for (g, heads, dim, v_dim), layers in self._share_groups(max(new) <= 1).items()
-                     if cache.groups[g].pool.n_shared and share_pays(cache.share_tree(g, slots), held, new, heads, cache.groups[g].need.kv_heads, dim + v_dim,
-                                                                     not SharedAttention.tensor_cores(self.dtype, dim, v_dim), 0 if kept else layers))
+            return out
+        for (g, heads, dim, v_dim), layers in self._share_groups(max(new) <= 1).items():
+            group = cache.groups[g]
+            tree, kv = cache.share_tree(g, slots) if group.pool.n_shared else None, group.need.kv_heads
+            if share_pays(tree, held, new, heads, kv, dim + v_dim, not SharedAttention.tensor_cores(self.dtype, dim, v_dim), 0 if kept else layers):
+                shape = self.kernels.shared.shape(dim, v_dim, self.sm_count)
+                rows = PlanCapacity.of_decode(next_pow2(len(slots)), heads, kv, shape).rows if kept else most_part_rows(tree, new, heads, kv, shape)
+                out.append(((g, heads, dim, v_dim), 4 * scratch_rows(rows) * (v_dim + 2)))
+        return out
 
     def _share_groups(self, decode: bool) -> dict[tuple[int, int, int, int], int]:
         """Cache groups with layers whose attention can read shared pages once, in decode steps or in steps of runs: (group, query heads,
@@ -432,40 +439,54 @@ class Engine:
         each step at `max_tokens_per_step` rows or fewer: a sequence's run is cut into portions, each
         landing on what the portions before left in the cache. Returns the float32 logits of every
         entry's last token, [entries, vocab], and the StepIndex of those rows (for the sampler). The
-        numbers are those of one big step, beyond rounding: a row sees its own sequence's keys only."""
+        numbers are those of one big step, beyond rounding: a row sees its own sequence's keys only. Where sequences share pages, a
+        portion is also kept so small that the partial results of reading those once fit their scratch."""
         budget = max_tokens_per_step or self.PROMPT_TOKENS_PER_STEP
         if budget < 1:
             raise StepError("a step needs room for at least one token")
-        if sum(len(e.tokens) for e in entries) <= budget:
+        if sum(len(e.tokens) for e in entries) <= budget and self._portion_fits([(e.sequence, len(e.tokens)) for e in entries]):
             logits = self.step([StepEntry(e.sequence, e.tokens) for e in entries])
             return logits, self.last_step
         rows: list[torch.Tensor | None] = [None] * len(entries)
         done = [0] * len(entries)
         nxt = 0
         while nxt < len(entries):
-            step, room, finishing = [], budget, []
-            i = nxt
-            while i < len(entries) and room > 0:
-                toks = entries[i].tokens
-                take = min(room, len(toks) - done[i])
-                last = done[i] + take == len(toks)
-                step.append(StepEntry(entries[i].sequence, toks[done[i]:done[i] + take], [take - 1] if last else []))
-                done[i] += take
-                room -= take
+            step, finishing = [], []
+            for i, n in self._portion(entries, done, nxt, budget):
+                toks, at = entries[i].tokens, done[i]
+                done[i] += n
+                last = done[i] == len(toks)
+                step.append(StepEntry(entries[i].sequence, toks[at:done[i]], [n - 1] if last else []))
                 if last:
                     finishing.append(i)
-                    i += 1
-                else:
-                    break
             out = self.step(step)
             for j, k in enumerate(finishing):
                 rows[k] = out[j:j + 1]
-            nxt = i
+            nxt += len(finishing)
         slots = torch.tensor([e.sequence.slot for e in entries], dtype=torch.int32)
         held = torch.tensor([e.sequence.length for e in entries], dtype=torch.int32)
         both = torch.stack([slots, held]).pin_memory().to(self.device, non_blocking=True)
         self.last_step = StepIndex(both[0], both[1])
         return torch.cat(rows), self.last_step
+
+    def _portion(self, entries, done, first: int, budget: int) -> list[tuple[int, int]]:
+        """(entry, tokens) of a step of at most `budget` tokens: those of entry `first` behind the `done[first]` that have run, then those of the
+        entries behind it. Half as many as long as the step's partial results do not fit."""
+        while True:
+            takes, left = [], budget
+            for i in range(first, len(entries)):
+                if left == 0:
+                    break
+                takes.append((i, min(left, len(entries[i].tokens) - done[i])))
+                left -= takes[-1][1]
+            if len(takes) < 2 or self._portion_fits([(entries[i].sequence, n) for i, n in takes]):
+                return takes
+            budget = sum(n for _, n in takes) // 2
+
+    def _portion_fits(self, takes) -> bool:
+        """Whether the partial results of a prompt step of these (sequence, tokens) fit, where reading shared pages once is worth it."""
+        gains = self._gains([s.slot for s, _ in takes], [s.length for s, _ in takes], [n for _, n in takes])
+        return all(scratch <= SharedAttention.SCRATCH_BYTES for _, scratch in gains)
 
     def activation_reserve_bytes(self) -> int:
         """A generous bound on what a prompt step of PROMPT_TOKENS_PER_STEP rows allocates beside

@@ -1,0 +1,56 @@
+"""Steps of sequences that share pages, and which of them the shared kernel ran in: its calls are counted."""
+import pytest
+import torch
+
+from helpers import random_ids
+from scriptling_llm_lib_b200.csrc.bindings import SharedAttention
+from scriptling_llm_lib_b200.engine import StepEntry
+from test_gpu_fork import LLAMA, alone, engine, rel_err, tol
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def shares_whatever_it_costs(monkeypatch):
+    monkeypatch.setattr("scriptling_llm_lib_b200.engine.step.share_pays", lambda tree, *a: bool(tree and tree[1]))
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """(rows, sequences) of every call of the shared kernel."""
+    seen, attn = [], SharedAttention.attn
+
+    def counted(self, q, out, tok_pos, block_table, kpages, vpages, plan, *a, **k):
+        seen.append((plan.n_rows, plan.n_seqs))
+        return attn(self, q, out, tok_pos, block_table, kpages, vpages, plan, *a, **k)
+    monkeypatch.setattr(SharedAttention, "attn", counted)
+    return seen
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_batch_whose_partial_results_do_not_fit_goes_in_portions_that_share(tmp_path, monkeypatch, calls, dtype):
+    eng = engine(tmp_path, LLAMA, dtype, max_tokens=16384, max_seqs=40)
+    V, layers = LLAMA["vocab_size"], LLAMA["num_hidden_layers"]
+    front = random_ids(700, V, 1)
+    root = eng.open()
+    eng.step([StepEntry(root, front)])
+    seqs = [root] + root.fork(23)
+    entries = [StepEntry(s, random_ids(11 + i, V, 100 + i)) for i, s in enumerate(seqs)]
+    rows = sum(len(e.tokens) for e in entries)
+    key = next(iter(eng._share_groups(False)))
+    takes = lambda some: dict(eng._gains([e.sequence.slot for e in some], [700] * len(some), [len(e.tokens) for e in some]))[key]      # noqa: E731
+    assert takes(entries[:18]) < takes(entries)
+    monkeypatch.setattr(SharedAttention, "SCRATCH_BYTES", takes(entries[:18]))
+    logits, _ = eng.prompt_step(entries)
+    steps = [c for i, c in enumerate(calls) if i % layers == 0]
+    assert 2 <= len(steps) <= 3 and sum(r for r, _ in steps) == rows and len(calls) == layers * len(steps)
+    for i in (0, 7, 23):
+        assert rel_err(logits[i], alone(eng, front + entries[i].tokens)) < tol(dtype)
+    calls.clear()
+    monkeypatch.setattr(SharedAttention, "SCRATCH_BYTES", 1000)          # nothing fits: each for itself, and no second capture
+    before = len(eng.decode_graphs.graphs)
+    out = eng.step([StepEntry(s, [1 + i]) for i, s in enumerate(seqs)])
+    assert not calls and ["shared" in k for k in eng.decode_graphs.graphs][before:] == [False]
+    assert rel_err(out[7], alone(eng, front + entries[7].tokens + [8])) < tol(dtype)
+    for s in seqs:
+        s.close()

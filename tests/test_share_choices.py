@@ -70,7 +70,8 @@ def engine(parts, dtype, tables, held, kv_heads):
     groups = [SimpleNamespace(need=need, pool=SimpleNamespace(n_shared=1)) for _ in tables]
     trees = [share_tree(np.asarray(t, dtype=np.int32), np.asarray(held) // 64) for t in tables]
     eng = Engine.__new__(Engine)
-    eng.dtype, eng._sharing = dtype, {}
+    eng.dtype, eng._sharing, eng.sm_count, eng.kernels = dtype, {}, 148, SimpleNamespace(shared=SharedAttention.__new__(SharedAttention))
+    eng.kernels.shared.dtype = dtype
     eng.cache = SimpleNamespace(groups=groups, group_of_unit={i: min(i, len(tables) - 1) for i in range(len(parts))}, shares_pages=True,
                                 share_tree=lambda g, slots: trees[g])
     eng.layout = SimpleNamespace(schedule=[SimpleNamespace(cache_unit=i, layer=i) for i in range(len(parts))])
@@ -104,3 +105,70 @@ def test_each_layer_shares_pages_by_its_own_gain():
     step = SharedStep(eng, shared, list(range(n)), held, [1] * n)
     step._build = lambda key: SimpleNamespace(part_floats=lambda v_dim: 0, key=key)
     assert step.plan(0, 32, 64, 64).key == (0, 32, 64, 64) and step.plan(1, 32, 64, 64) is None
+
+
+def test_the_scratch_of_a_plan_is_known_before_it_is_laid_out():
+    import random
+    from scriptling_llm_lib_b200.cache import SharePlan, TileShape, most_part_rows, share_tree
+    from test_share_cpu import _batch
+    import numpy as np
+    rng = random.Random(5)
+    for shape in (TileShape(256, 148, True, 5.0, ((128, 0.85),), 2, 16, 8, 0.3, 1.0, 4.0), TileShape(64, 296, min_pages=1), TileShape(64, 148, costs=((4, 0.25),)), TileShape(16, 40, True)):
+        for n in (1, 2, 5, 23, 60, 200):
+            for runs in (False, True):
+                G, rep = rng.choice([1, 2, 8]), rng.choice([1, 3, 4, 8])
+                tables, held, new = _batch(rng, n, rep, runs)
+                tree = share_tree(tables, np.asarray(held) // 64)
+                rows = SharePlan.build(tables, held, new, G * rep, G, shape, None).part_rows
+                most = most_part_rows(tree, new, G * rep, G, shape)
+                assert rows <= most <= rows + shape.workers * (shape.rows + shape.thin_rows * shape.thin_warps)
+
+
+def prompts(n, new, prefix, part, kv, layers):
+    """An engine of such layers, entries of `new` tokens for each of `n` sequences behind a common prefix."""
+    held = [prefix + 40] * n
+    eng = engine([part] * layers, BF16, [table(n, prefix // 64, 2)], held, kv)
+    full = eng.cache.groups[0]
+    from scriptling_llm_lib_b200.cache.share import share_tree
+    import numpy as np
+    t = np.asarray(table(n, prefix // 64, 2), dtype=np.int32)
+    eng.cache.share_tree = lambda g, slots: share_tree(t[list(slots)], np.full(len(slots), held[0] // 64))
+    assert full.pool.n_shared
+    return eng, [SimpleNamespace(sequence=SimpleNamespace(slot=i, length=held[0]), tokens=list(range(new))) for i in range(n)], held
+
+
+@pytest.mark.parametrize("n, new, prefix", [(200, 32, 4096), (250, 32, 16384), (256, 40, 16384), (400, 40, 16384)])
+def test_long_batches_of_questions_go_in_portions_whose_partial_results_fit(n, new, prefix):
+    """32 heads of 128 on 8, 32 layers: 320 to 526 MB of partial results in one step, which is then each sequence for itself."""
+    from scriptling_llm_lib_b200.cache import SharePlan
+    import numpy as np
+    eng, entries, held = prompts(n, new, prefix, layer(32, 8, 128), 8, 32)
+    assert eng._gains(range(n), held, [new] * n) and not eng._shares(range(n), held, [new] * n)
+    done, first, steps = [0] * n, 0, 0
+    while first < n:
+        takes = eng._portion(entries, done, first, 16384)
+        slots, new_here = [i for i, _ in takes], [k for _, k in takes]
+        assert slots == list(range(first, first + len(takes))) and all(k > 0 for k in new_here)
+        assert eng._shares(slots, [held[0]] * len(slots), new_here) == ((0, 32, 128, 128),)
+        plan = SharePlan.build(np.asarray(table(n, prefix // 64, 3), dtype=np.int32)[slots], [held[0]] * len(slots), new_here, 32, 8,
+                               eng.kernels.shared.shape(128, 128, 148), None)
+        assert 4 * plan.part_floats(128) <= SharedAttention.SCRATCH_BYTES
+        for i, k in takes:
+            done[i] += k
+        while first < n and done[first] == new:
+            first += 1
+        steps += 1
+    assert done == [new] * n and 2 <= steps <= 5
+
+
+def test_a_captured_step_whose_partial_results_do_not_fit_is_not_captured_again():
+    eng, _, held = prompts(1024, 1, 4096, layer(64, 8, 128), 8, 32)
+    assert eng._gains(range(1024), held, [1] * 1024, kept=True) and eng._shares(range(1024), held, [1] * 1024, kept=True) == ()
+    assert eng._shares(range(256), held[:256], [1] * 256, kept=True) == ((0, 64, 128, 128),)
+
+
+def test_prompts_that_share_nothing_go_in_portions_of_the_budget():
+    eng, entries, _ = prompts(6, 100, 4096, layer(32, 8, 128), 8, 32)
+    eng.cache.shares_pages = False
+    assert eng._portion(entries, [0, 30, 0, 0, 0, 0], 1, 250) == [(1, 70), (2, 100), (3, 80)]
+    assert eng._portion(entries, [0] * 6, 0, 10 ** 6) == [(i, 100) for i in range(6)] and eng._portion(entries, [0] * 6, 5, 1) == [(5, 1)]
