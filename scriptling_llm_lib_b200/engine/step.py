@@ -488,13 +488,17 @@ class Engine:
         gains = self._gains([s.slot for s, _ in takes], [s.length for s, _ in takes], [n for _, n in takes])
         return all(scratch <= SharedAttention.SCRATCH_BYTES for _, scratch in gains)
 
-    def activation_reserve_bytes(self) -> int:
+    def activation_reserve_bytes(self, sharing: bool = False) -> int:
         """A generous bound on what a prompt step of PROMPT_TOKENS_PER_STEP rows allocates beside
         weights and cache (residual, products' outputs), plus the logits of the captured decode steps: what the
         cache must leave free. Where a matrix is kept in 32-bit, the planes of its product count too, and once more
-        for captured decode steps of many rows, whose graphs hold theirs beside what prompts allocate."""
+        for captured decode steps of many rows, whose graphs hold theirs beside what prompts allocate. With `sharing`, for sequences
+        that share pages, the partial results of attention over those count (of layers that take it; they are not there while other
+        parts' scratch is)."""
         width = 64 * self.layout.hidden_size                        # bytes a row, all buffers of a layer alive at once
         scratch = max(p.scratch_bytes(self.PROMPT_TOKENS_PER_STEP) for p in self.model.parts() if isinstance(p, Part))
+        if sharing and (self._share_groups(True) or self._share_groups(False)):
+            scratch = max(scratch, SharedAttention.SCRATCH_BYTES)
         if any(lin.weight is not None and lin.weight.dtype == torch.float32 for p in self.model.parts() for lin in linears(p)):
             scratch += (2 if getattr(self, "use_graphs", False) else 1) * SplitGemm.SCRATCH_BYTES
         return self.PROMPT_TOKENS_PER_STEP * width + scratch + 4 * self.layout.vocab_size * 4 * 1024

@@ -49,8 +49,9 @@ def unload(model_dir=None) -> None:
             del _models[key]
 
 
-def _fit_cache(eng: Engine, prompts, max_tokens, max_batch, n: int = 1):
-    """Grow the engine's cache so the requests run in as few batches as memory allows. `n` continuations of a prompt hold its pages once."""
+def _fit_cache(eng: Engine, prompts, max_tokens, max_batch, n: int = 1, share_prefix: bool = False):
+    """Grow the engine's cache so the requests run in as few batches as memory allows. `n` continuations of a prompt hold its pages once;
+    where requests share pages, the partial results of reading those once have to find room beside the cache."""
     import torch
     pages = [(min(eng.layout.max_positions, len(p) + max_tokens - 1) + PAGE - 1) // PAGE for p in prompts]
     if n > 1:
@@ -64,7 +65,7 @@ def _fit_cache(eng: Engine, prompts, max_tokens, max_batch, n: int = 1):
     free, _ = torch.cuda.mem_get_info(eng.device)
     have = eng.cache.n_pages * eng.bytes_per_page()
     # what a prompt step's activations and the captured decode steps need stays free
-    afford = max(0, int((free + have - eng.activation_reserve_bytes()) * 0.9)) // max(1, eng.bytes_per_page())
+    afford = max(0, int((free + have - eng.activation_reserve_bytes(sharing=n > 1 or share_prefix)) * 0.9)) // max(1, eng.bytes_per_page())
     n_pages = max(max(pages), min(want_pages, afford), eng.cache.n_pages)
     eng.resize_cache(n_pages * PAGE, max(want_seqs, eng.cache.n_slots))
 
@@ -98,7 +99,7 @@ def generate(model_dir, prompt_ids, max_tokens: int = 100, strategy: str = "gree
         n = as_int(n)
         if n < 1:
             raise ValueError(f"{n} continuations of a prompt")
-        _fit_cache(eng, prompts, max_tokens, max_batch, n)
+        _fit_cache(eng, prompts, max_tokens, max_batch, n, bool(share_prefix))
         results = Generator(eng, sampler).generate(prompts, max_tokens, options, stop_ids, seed, max_batch, on_step, n, bool(share_prefix))
     ids, st = [r.tokens for r in results], _stats(results)
     if n > 1:

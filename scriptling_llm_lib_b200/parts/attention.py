@@ -323,12 +323,6 @@ class Attention(Mixer):
                 return None
         return self.n_heads, *widths
 
-    def scratch_bytes(self, rows):
-        """The partial results of attention over pages that a step's sequences share."""
-        widths = self.shares_pages()
-        takes = widths is not None and SharedAttention.takes(widths[1], widths[2], self.n_heads // self.n_kv_heads)
-        return SharedAttention.SCRATCH_BYTES if takes else 0
-
     def _share_plan(self, ctx, unit):
         """The step's plan where its sequences share pages and this layer sees all of them."""
         plan = getattr(ctx, "share_plan", None)

@@ -172,3 +172,27 @@ def test_prompts_that_share_nothing_go_in_portions_of_the_budget():
     eng.cache.shares_pages = False
     assert eng._portion(entries, [0, 30, 0, 0, 0, 0], 1, 250) == [(1, 70), (2, 100), (3, 80)]
     assert eng._portion(entries, [0] * 6, 0, 10 ** 6) == [(i, 100) for i in range(6)] and eng._portion(entries, [0] * 6, 5, 1) == [(5, 1)]
+
+
+def test_only_requests_that_share_pages_keep_room_for_their_partial_results(monkeypatch):
+    """The cache of requests that share nothing is as large as it would be without shared attention."""
+    from scriptling_llm_lib_b200 import llm
+    from scriptling_llm_lib_b200.engine.step import Engine
+    part = layer(32, 8, 64)
+    eng = engine([part] * 2, BF16, [table(2, 4, 1)], [300] * 2, 8)
+    eng.model.parts, eng.use_graphs = lambda: [part], False
+    eng.layout.hidden_size, eng.layout.vocab_size, eng.layout.max_positions = 2048, 512, 4096
+    plain = Engine.activation_reserve_bytes(eng)
+    assert Engine.activation_reserve_bytes(eng, sharing=True) == plain + SharedAttention.SCRATCH_BYTES and part.scratch_bytes(16384) == 0
+    window = layer(32, 8, 64, window=128)
+    other = engine([window], BF16, [table(2, 4, 1)], [300] * 2, 8)
+    other.model.parts, other.use_graphs, other.layout.hidden_size, other.layout.vocab_size = lambda: [window], False, 2048, 512
+    assert Engine.activation_reserve_bytes(other, sharing=True) == Engine.activation_reserve_bytes(other) == plain
+    monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (1 << 30, 1 << 31))
+    eng.device, eng.cache.n_pages, eng.cache.n_slots, sizes = None, 1, 1, []
+    eng.bytes_per_page = lambda: 1 << 16
+    eng.activation_reserve_bytes = lambda sharing=False: (1 << 28) + (SharedAttention.SCRATCH_BYTES if sharing else 0)
+    eng.resize_cache = lambda tokens, seqs: sizes.append(tokens // 64)
+    for how in (dict(), dict(n=2), dict(share_prefix=True)):
+        llm._fit_cache(eng, [[1] * 4000] * 1000, 50, None, **how)
+    assert sizes[0] > sizes[1] == sizes[2]
