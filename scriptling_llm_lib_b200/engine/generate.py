@@ -49,7 +49,8 @@ def plan_batches(prompt_lens: Seq[int], max_tokens: int, max_seqs: int, page_cap
     for i, length in enumerate(prompt_lens):
         own, shared = request_pages(length, max_tokens, max_positions)
         if own + shared > page_capacity:
-            raise ValueError(f"request {i} needs {own + shared} cache pages; the cache has {page_capacity}")
+            held = min(max_positions, min(length, max_positions) + max_tokens - 1)
+            raise ValueError(f"request {i} needs {own + shared} cache pages ({held} tokens); the cache has {page_capacity}")
         again = bool(cur) and i % n != 0
         if cur and (len(cur) >= max_seqs or cur_pages + own + (0 if again else shared) > page_capacity):
             batches.append(cur)
