@@ -54,3 +54,17 @@ def test_a_batch_whose_partial_results_do_not_fit_goes_in_portions_that_share(tm
     assert rel_err(out[7], alone(eng, front + entries[7].tokens + [8])) < tol(dtype)
     for s in seqs:
         s.close()
+
+
+def test_a_trace_that_forks_what_is_not_live_ends_with_a_message(tmp_path):
+    import json
+    import subprocess
+    import sys
+    from pathlib import Path
+    from helpers import make_model_dir
+    d = make_model_dir(tmp_path / "m", LLAMA, 3)
+    records = [{"step": 0, "entries": [{"id": "a", "tokens": [1, 2], "want": []}], "end": ["a"]}, {"step": 1, "fork": [{"id": "b", "of": "a"}]}]
+    run = subprocess.run([sys.executable, str(Path(__file__).resolve().parent.parent / "bin" / "trace_run"), "--model", str(d), "--dtype", "float32", "--out",
+                          str(tmp_path / "o"), "--max-tokens", "640"], input="\n".join(json.dumps(r) for r in records), capture_output=True, text=True, timeout=300)
+    assert run.returncode != 0 and "done 0" in run.stdout
+    assert "the request 'a' to fork is not live" in run.stderr and "Traceback" not in run.stderr
