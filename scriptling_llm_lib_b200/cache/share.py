@@ -156,8 +156,10 @@ class SharePlan:
             raise ValueError(f"a plan of {self.n_items} items, {self.n_list} list entries and {self.part_rows} rows of scratch; there is "
                              f"room for {cap.items}, {cap.entries} and {cap.rows}")
         if device is not None:
-            host = self.host()
-            self.dev = torch.from_numpy(host).to(device)
+            host = torch.from_numpy(self.host())
+            if torch.device(device).type == "cuda":     # (out of pageable memory the copy would wait for all that is queued)
+                host = host.pin_memory()
+            self.dev = host.to(device, non_blocking=True)
             self._views()
 
     def again(self, other: "SharePlan") -> np.ndarray:

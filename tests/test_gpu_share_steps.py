@@ -68,3 +68,20 @@ def test_a_trace_that_forks_what_is_not_live_ends_with_a_message(tmp_path):
                           str(tmp_path / "o"), "--max-tokens", "640"], input="\n".join(json.dumps(r) for r in records), capture_output=True, text=True, timeout=300)
     assert run.returncode != 0 and "done 0" in run.stdout
     assert "the request 'a' to fork is not live" in run.stderr and "Traceback" not in run.stderr
+
+
+def test_a_plan_goes_to_the_device_without_waiting_for_what_is_queued():
+    from scriptling_llm_lib_b200.cache import SharePlan
+    from scriptling_llm_lib_b200.csrc.bindings import KernelSet
+    from test_gpu_share import B16, Case
+    c = Case("runs", (16, 4, 64, 64), B16)
+    want, shape = c.run(), KernelSet(B16).shared.shape(64, 64)
+    done = torch.cuda.Event()
+    torch.cuda._sleep(400_000_000)                                     # about 0.2 s
+    done.record()
+    plan = SharePlan.build(c.table, c.held, c.new, 16, 4, shape, "cuda")
+    assert not done.query()
+    others = [torch.zeros(n, dtype=torch.int32).pin_memory() for n in (plan.dev.numel(),) * 4]      # (its pinned memory is not handed on meanwhile)
+    for t in others:
+        t.fill_(-1)
+    assert torch.equal(c.run(plan), want)
