@@ -143,7 +143,7 @@ def most_part_rows(tree, new, n_heads: int, n_kv: int, shape: TileShape) -> int:
 class SharePlan:
     """The items of one attention over a step's rows, in one int32 buffer on the device. Good for every layer of the step with these
     head counts, and for later steps of the same sequences with as many new tokens each: a leaf's last item goes on to where its
-    tokens stand now."""
+    tokens stand now. `width`: pages of the block table that the layout reaches."""
 
     def __init__(self, n_seqs: int, n_rows: int, n_heads: int, n_kv: int, shape: TileShape, width: int, parts: dict, device,
                  capacity: "PlanCapacity | None" = None):
@@ -167,7 +167,7 @@ class SharePlan:
         same = lambda p: (p.n_seqs, p.n_rows, p.n_heads, p.n_kv, p.shape, p.capacity)        # noqa: E731
         if same(other) != same(self):
             raise ValueError(f"a plan of {same(other)} cannot stand where one of {same(self)} does")
-        self.parts, self.n_items, self.n_list, self.part_rows = other.parts, other.n_items, other.n_list, other.part_rows
+        self.parts, self.n_items, self.n_list, self.part_rows, self.width = other.parts, other.n_items, other.n_list, other.part_rows, other.width
         return self.host()
 
     def fits(self, cap: "PlanCapacity") -> bool:
@@ -232,7 +232,7 @@ class SharePlan:
             tree = share_tree(table, held // PAGE)
         order, nodes, own = tree
         parts = _lay_out(order, nodes, own, held, new, rep, n_kv, shape)
-        return cls(n_seqs, int(new.sum()), n_heads, n_kv, shape, width, parts, device, capacity)
+        return cls(n_seqs, int(new.sum()), n_heads, n_kv, shape, parts["width"], parts, device, capacity)
 
 
 @dataclass(frozen=True)
@@ -360,4 +360,5 @@ def _lay_out(order, nodes, own, held, new, rep: int, n_kv: int, shape: TileShape
     by = np.argsort(key, kind="stable")
     list_first = np.zeros(T * n_kv + 1, dtype=np.int64)
     np.cumsum(np.bincount(key, minlength=T * n_kv), out=list_first[1:])
-    return {"first": first, "thin_first": thin_first, "items": items, "toks": toks, "list_first": list_first, "list": entry[by], "part_rows": int(rows.sum())}
+    return {"first": first, "thin_first": thin_first, "items": items, "toks": toks, "list_first": list_first, "list": entry[by], "part_rows": int(rows.sum()),
+            "width": int(t_end.max(initial=0))}

@@ -1795,9 +1795,10 @@ class SharedAttention:
         ld, step = q.stride()
         if len(qs) != 2 or qs[0] != T or qs[1] < H * hd or step != 1 or ld % 4 or q.dtype != self.dtype:
             raise KernelError(f"shared attention: queries {tuple(qs)} {q.dtype} (row stride {ld}) for {T} rows of {H} heads of {hd}")
-        if out.shape != (T, H * vd) or tok_pos.shape != (T,) or block_table.dim() != 2 or block_table.shape[0] < plan.n_seqs:
+        if (out.shape != (T, H * vd) or tok_pos.shape != (T,) or block_table.dim() != 2 or block_table.shape[0] < plan.n_seqs
+                or block_table.shape[1] < plan.width):
             raise KernelError(f"shared attention: out {tuple(out.shape)}, positions {tuple(tok_pos.shape)} and block table "
-                              f"{tuple(block_table.shape)} for {T} rows of {plan.n_seqs} sequences")
+                              f"{tuple(block_table.shape)} for {T} rows of {plan.n_seqs} sequences of up to {plan.width} pages")
         if (sink is not None and sink.shape != (H,)) or part.numel() < plan.part_floats(vd):
             raise KernelError(f"shared attention: a sink for each of {H} heads and a scratch of {plan.part_floats(vd)} floats")
         if plan.shape != shape:

@@ -48,3 +48,16 @@ def test_a_row_that_sees_nothing_is_zero_however_deep_its_sink(dtype, seqs):
         u = 2.0 ** -24
         slack = 4 * u * ((64 + 8) * S[..., None] + n[:, None, None] + 8) * mean + (2.0 ** -8 * (mean + want.abs()) if dtype == B16 else 0) + 1e-30
         assert bool((off <= slack[~blind]).all())
+
+
+@pytest.mark.parametrize("dtype", [F, B16], ids=["f32", "bf16"])
+def test_a_block_table_narrower_than_the_plan_is_refused(dtype):
+    from scriptling_llm_lib_b200.csrc.bindings import KernelError
+    c = Case("nested", (16, 4, 64, 64), dtype)
+    good, plan = c.run(), c.plan()
+    wide = c.table
+    c.table = np.ascontiguousarray(wide[:, :-1])
+    with pytest.raises(KernelError, match="pages"):
+        c.run(plan)
+    c.table = np.concatenate([wide, np.full((len(wide), 3), -1, dtype=np.int32)], axis=1)
+    assert torch.equal(c.run(plan), good)
