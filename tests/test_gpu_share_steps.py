@@ -85,3 +85,60 @@ def test_a_plan_goes_to_the_device_without_waiting_for_what_is_queued():
     for t in others:
         t.fill_(-1)
     assert torch.equal(c.run(plan), want)
+
+
+def followed(calls, eng, dtype, vocab, prompt, n=5):
+    """What `follow` of test_gpu_fork.py checks, and the calls for steps of single tokens and for steps of runs."""
+    from test_gpu_fork import follow
+    follow(eng, dtype, vocab, prompt, depth=1, n=n)
+    single = sum(rows == seqs for rows, seqs in calls)
+    return single, len(calls) - single
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("graphs", [True, False], ids=["replayed", "launched"])
+@pytest.mark.parametrize("name", ["LLAMA", "WIDE", "ODD", "WINDOW"])
+def test_every_layer_that_sees_all_keys_reads_shared_pages_once(tmp_path, calls, name, dtype, graphs):
+    import test_gpu_fork
+    raw = getattr(test_gpu_fork, name)
+    eng = engine(tmp_path, raw, dtype, use_graphs=graphs)
+    single, runs = followed(calls, eng, dtype, raw["vocab_size"], random_ids(700, raw["vocab_size"], 7))
+    if name == "WINDOW":
+        assert single == runs == 0
+    else:
+        layers = raw["num_hidden_layers"]
+        assert runs == 2 * layers                                  # two steps of runs, not captured
+        assert single > 0 and single % layers == 0
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["sozilix", "muvorax", "belasun", "tufazen", "fopezen", "debusun"])
+def test_architectures_whose_layers_see_all_keys_share_them(tmp_path, calls, name, dtype):
+    """Two of them: the others' layers have windows or chunks, latent keys, or widths that the shared kernels do not take."""
+    from test_gpu_fork import other_architectures
+    raw = other_architectures()[name]
+    eng = engine(tmp_path, raw, dtype, max_tokens=4096, max_seqs=12)
+    vocab = eng.layout.vocab_size
+    single, runs = followed(calls, eng, dtype, vocab, random_ids(min(330, eng.max_positions - 40), vocab, 5), n=3)
+    assert (single > 0, runs > 0) == (name in ("belasun", "tufazen"),) * 2
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_generation_of_requests_that_share_reads_shared_pages_once(tmp_path, calls, dtype):
+    from helpers import make_model_dir
+    from scriptling_llm_lib_b200 import llm
+    d = make_model_dir(tmp_path / "m", LLAMA, 3)
+    V = LLAMA["vocab_size"]
+    front = random_ids(300, V, 1)
+    prompts = [front + random_ids(n, V, 50 + n) for n in (5, 90, 17)]
+    llm.unload()
+    kw = dict(dtype=dtype, stop_ids=[], temperature=0.0)
+    llm.generate(d, prompts, 6, **kw)
+    assert not calls
+    llm.generate(d, prompts, 6, share_prefix=True, **kw)
+    assert any(rows > seqs for rows, seqs in calls) and any(rows == seqs for rows, seqs in calls)      # the questions, then their answers
+    calls.clear()
+    llm.unload()                                                      # (its captured steps with it)
+    llm.generate(d, prompts[0], 6, n=4, **kw)
+    assert any(rows == seqs for rows, seqs in calls)
+    llm.unload()
