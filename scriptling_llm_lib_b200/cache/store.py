@@ -109,15 +109,22 @@ class KVGroup:
                 writers[page] = writers.get(page, 0) + 1
         return sum(min(k, self.pool.holders(page) - 1) for page, k in writers.items())
 
-    def own_written(self, slot: int, length: int, n: int) -> list[tuple[int, int, int]]:
-        """Give the slot pages of its own where it would write shared ones: (from, to, positions held) of each."""
+    def own_written(self, slot: int, length: int, n: int) -> list[tuple[int, int, int, int, int]]:
+        """Give the slot pages of its own where it would write shared ones: (from, to, positions held, slot, place) of each."""
         out = []
         for i in self.shared_written(slot, length, n):
             page, mine = self.pages[slot][i], self.pool.alloc()
             self.pool.free(page)
             self.pages[slot][i] = self.table[slot, i] = mine
-            out.append((page, mine, max(0, length - i * PAGE)))
+            out.append((page, mine, max(0, length - i * PAGE), slot, i))
         return out
+
+    def disown(self, own) -> None:
+        """What `own_written` gave, taken back: the copies were not made."""
+        for page, mine, _, slot, i in reversed(own):
+            self.pool.share(page)
+            self.pool.free(mine)
+            self.pages[slot][i] = self.table[slot, i] = page
 
     def renumber(self, to: dict[int, int], n: int | None = None) -> None:
         self.pool.renumber(to, n)
@@ -255,7 +262,7 @@ class SequenceCache:
 
     def fork(self, slot: int, n: int = 1) -> list[int]:
         """`n` new slots that hold what `slot` holds: the same pages, copies of its states and of its record (its sampling stream goes on
-        in each: `seed` starts others). All or CacheFull."""
+        in each: `seed` starts others). All, or an error (CacheFull, or what the copy of the states met) and none."""
         if not self.slots.is_held(slot):
             raise ValueError(f"cache slot {slot} is not held; it cannot be forked")
         if n < 0:
@@ -267,8 +274,13 @@ class SequenceCache:
             self.length[s] = self.length[slot]
             for g in self.groups:
                 g.fork(slot, s, self.length[slot])
-        self._copy([(t, t) for t in self._states()], [slot] * n, new, slots=True)
         self.version += 1
+        try:
+            self._copy([(t, t) for t in self._states()], [slot] * n, new, slots=True)
+        except BaseException:
+            for s in new:
+                self.close(s)
+            raise
         return new
 
     def compact(self, n_pages: int | None = None) -> int:
@@ -323,7 +335,8 @@ class SequenceCache:
     # ------------------------------------------------------------------ growth
     def reserve(self, growth: list[tuple[int, int]]) -> None:
         """Pages for `n_new` more tokens of each (slot, n_new); either all are had or CacheFull is
-        raised and nothing has changed. A slot that would write a page that others hold too gets a copy of its own."""
+        raised and nothing has changed. A slot that would write a page that others hold too gets a copy of its own (where that
+        copy meets an error, the slots hold the pages that they held)."""
         for g in self.groups:
             want = sum(g.pages_needed(slot, self.length[slot] + n) for slot, n in growth) + g.copies_needed(growth, self.length)
             if want > g.pool.n_free:
@@ -334,7 +347,11 @@ class SequenceCache:
                 own = [c for slot, n in growth for c in g.own_written(slot, self.length[slot], n)]
                 if own:
                     self.version += 1
-                    self._copy([(g.k, g.k), (g.v, g.v)], *(list(c) for c in zip(*own)))
+                    try:
+                        self._copy([(g.k, g.k), (g.v, g.v)], *(list(c) for c in list(zip(*own))[:3]))
+                    except BaseException:
+                        g.disown(own)
+                        raise
             for slot, n in growth:
                 g.grow(slot, self.length[slot] + n)
 

@@ -25,3 +25,37 @@ def test_a_plan_knows_how_many_pages_its_layout_reaches():
     plan = build([400, 500, 3], [1, 1, 1], capacity=cap)
     plan.again(build([400, 1000, 3], [1, 1, 1], capacity=cap))
     assert plan.width == 16
+
+
+def test_a_copy_that_fails_leaves_forks_and_writers_as_they_were(monkeypatch):
+    """The copies' ids find no memory: no slot is taken, no page is held for nothing, and the writers hold the pages that they shared."""
+    from test_share_cpu import _cache, _check, _consistent, _write
+    c = _cache()
+    a = c.open()
+    _write(c, a, list(range(1, 151)))
+    b, d = c.fork(a, 2)
+    copy = c._copy
+
+    def fails(*args, **kw):
+        raise MemoryError("no memory")
+    before = [(g.pool.n_held, g.pool.n_shared, {s: list(p) for s, p in g.pages.items()}, g.table.copy()) for g in c.groups]
+
+    def unchanged():
+        return all((g.pool.n_held, g.pool.n_shared, {s: list(p) for s, p in g.pages.items()}) == was[:3] and (g.table == was[3]).all()
+                   for g, was in zip(c.groups, before))
+    monkeypatch.setattr(c, "_copy", fails)
+    with pytest.raises(MemoryError):
+        c.fork(a, 3)
+    assert c.slots.n_held == 3 and unchanged()
+    for growth in ([(b, 1)], [(a, 2), (b, 1), (d, 70)]):
+        with pytest.raises(MemoryError):
+            c.reserve(growth)
+        assert unchanged()
+    monkeypatch.setattr(c, "_copy", copy)
+    for s, t in ((a, 7), (b, 8), (d, 9)):
+        _write(c, s, [t])
+        _check(c, s, list(range(1, 151)) + [t])
+    _consistent(c)
+    for s in (a, b, d):
+        c.close(s)
+    assert all(g.pool.n_held == 0 for g in c.groups)
