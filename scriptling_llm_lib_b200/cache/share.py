@@ -146,7 +146,7 @@ class SharePlan:
     tokens stand now. `width`: pages of the block table that the layout reaches."""
 
     def __init__(self, n_seqs: int, n_rows: int, n_heads: int, n_kv: int, shape: TileShape, width: int, parts: dict, device,
-                 capacity: "PlanCapacity | None" = None):
+                 capacity: "PlanCapacity | None" = None, queued: bool = False):
         self.n_seqs, self.n_rows, self.n_heads, self.n_kv, self.shape, self.width = n_seqs, n_rows, n_heads, n_kv, shape, width
         self.n_items, self.n_list, self.part_rows = len(parts["items"]), len(parts["list"]), parts["part_rows"]
         self.parts = parts
@@ -157,9 +157,7 @@ class SharePlan:
                              f"room for {cap.items}, {cap.entries} and {cap.rows}")
         if device is not None:
             host = torch.from_numpy(self.host())
-            if torch.device(device).type == "cuda":     # (out of pageable memory the copy would wait for all that is queued)
-                host = host.pin_memory()
-            self.dev = host.to(device, non_blocking=True)
+            self.dev = host.pin_memory().to(device, non_blocking=True) if queued else host.to(device)
             self._views()
 
     def again(self, other: "SharePlan") -> np.ndarray:
@@ -210,9 +208,11 @@ class SharePlan:
         return scratch_rows(self.capacity.rows)
 
     @classmethod
-    def build(cls, table, held, new, n_heads: int, n_kv: int, shape: TileShape, device, capacity=None, tree=None) -> "SharePlan":
+    def build(cls, table, held, new, n_heads: int, n_kv: int, shape: TileShape, device, capacity=None, tree=None, queued: bool = False) -> "SharePlan":
         """`table` [seqs, width] page ids on the host; `held` and `new`: tokens that each sequence holds before the step and brings (0:
-        none). `tree`: what `share_tree` gave for these sequences, if it is at hand."""
+        none). `tree`: what `share_tree` gave for these sequences, if it is at hand. The plan is on the device when this returns, for any
+        stream; `queued`: its copy is one more operation of the current stream, for calls on this stream (or on one that waits for it),
+        and nothing that is queued is waited for."""
         table = np.asarray(table)
         if table.ndim != 2 or table.dtype.kind not in "iu" or table.shape[0] == 0:
             raise ValueError(f"a block table of page ids [sequences, pages], not {table.dtype} {table.shape}")
@@ -232,7 +232,7 @@ class SharePlan:
             tree = share_tree(table, held // PAGE)
         order, nodes, own = tree
         parts = _lay_out(order, nodes, own, held, new, rep, n_kv, shape)
-        return cls(n_seqs, int(new.sum()), n_heads, n_kv, shape, parts["width"], parts, device, capacity)
+        return cls(n_seqs, int(new.sum()), n_heads, n_kv, shape, parts["width"], parts, device, capacity, queued)
 
 
 @dataclass(frozen=True)

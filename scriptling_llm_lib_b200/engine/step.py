@@ -175,7 +175,7 @@ class SharedStep:
             table = np.concatenate([table, np.full((n, table.shape[1]), cache.n_pages, dtype=np.int32)])
             held, new = held + [0] * n, new + [1] * n
         capacity = None if B is None else PlanCapacity.of_decode(B, n_heads, n_kv, shape)
-        return SharePlan.build(table, held, new, n_heads, n_kv, shape, self.engine.device if device else None, capacity, tree)
+        return SharePlan.build(table, held, new, n_heads, n_kv, shape, self.engine.device if device else None, capacity, tree, queued=True)
 
     def refresh(self, slots, held) -> None:
         """Lay the plans out for these sequences, at the addresses that they have (the stream's order keeps steps apart)."""

@@ -79,7 +79,7 @@ def test_a_plan_goes_to_the_device_without_waiting_for_what_is_queued():
     done = torch.cuda.Event()
     torch.cuda._sleep(400_000_000)                                     # about 0.2 s
     done.record()
-    plan = SharePlan.build(c.table, c.held, c.new, 16, 4, shape, "cuda")
+    plan = SharePlan.build(c.table, c.held, c.new, 16, 4, shape, "cuda", queued=True)
     assert not done.query()
     others = [torch.zeros(n, dtype=torch.int32).pin_memory() for n in (plan.dev.numel(),) * 4]      # (its pinned memory is not handed on meanwhile)
     for t in others:
@@ -142,3 +142,18 @@ def test_generation_of_requests_that_share_reads_shared_pages_once(tmp_path, cal
     llm.generate(d, prompts[0], 6, n=4, **kw)
     assert any(rows == seqs for rows, seqs in calls)
     llm.unload()
+
+
+def test_a_plan_that_is_not_queued_is_there_for_any_stream():
+    from scriptling_llm_lib_b200.cache import SharePlan
+    from scriptling_llm_lib_b200.csrc.bindings import KernelSet
+    from test_gpu_share import B16, Case
+    c = Case("runs", (16, 4, 64, 64), B16)
+    want, shape, side = c.run(), KernelSet(B16).shared.shape(64, 64), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)                                     # the current stream is busy; the other one is not
+    plan = SharePlan.build(c.table, c.held, c.new, 16, 4, shape, "cuda")
+    with torch.cuda.stream(side):
+        got = c.run(plan)
+    side.synchronize()
+    assert torch.equal(got, want)
