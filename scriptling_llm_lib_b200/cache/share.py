@@ -86,8 +86,10 @@ def share_tree(table: np.ndarray, whole: np.ndarray):
 def share_pays(tree, held, new, n_heads: int, n_kv: int, width: int, floats: bool, layers: int = 0) -> bool:
     """Whether a step of these sequences is estimated to be faster by the tree than each sequence for itself; `width`: of a key and a
     value together; `floats`: the shared pages go on FP32 FMA, in 32-bit and for bfloat16 widths that the tensor-core form does not take; `layers`:
-    those that go by a plan made for this step alone (0: the plan is kept for more steps), which costs the host about 1.2 ms. Measured on
-    148 SMs, each for itself / by the tree, us:
+    those that go by a plan made for this step alone (0: the plan is kept for more steps), which is counted as 1.2 ms of the host's and 0.1 us
+    for each row and key/value head (728 rows on 8 take it 0.9 ms, 15,000 7 ms). The answer leans to each for itself: 32-bit steps of a token
+    each have to be estimated 1.4 times as fast by the tree, and bfloat16 ones to save 80 MB a layer. Measured on 148 SMs, each for itself /
+    by the tree, us:
     bfloat16, a token each (bound by the bytes, and the rotation and the cache write become a kernel of their own: in whole steps the
     line is between 50 and 100 MB saved a layer): 32 heads of 64 on 8, 8 sequences behind 1,000 tokens 12.5 / 13.3 (14 MB saved), 32
     behind 1,000 18.8 / 15.5 (61), 8 behind 16,000 41 / 20 (229), 64 behind 300 11.7 / 18.4 (33); 32 heads of 128 on 8, 64 behind 300

@@ -19,9 +19,10 @@
 // and head at a time. S = Q K^T (128 x 64) and O += P V as in attn_prefill_tcgen05.cu: thread = row = tensor-memory lane, P back into
 // tensor memory as bfloat16 pairs (the weights' only rounding; their sum is taken before it), O rescaled only when a row's maximum has
 // outgrown its reference by 2^8. With PARTS 2 the weights go into the product in two parts, P and L, that hold a weight to 2^-16 of
-// itself, for layers whose other kernels keep them in float32 (relative errors beside 32-bit sums rounded once 2e-5 to 4e-4, 1.8e-3 to
-// 2.6e-3 in one part; 8 single tokens behind 4,096, heads of 64, 13.7 us, 13.3 in one part; 64 behind 8,192, heads of 128, 41.6, 36.3). Warps whose rows are all past the tile's end pass the barriers and compute nothing. Waits are bounded
-// (2 s), after which the kernel raises *err, lets its copies land, frees its tensor memory and returns.
+// itself, for layers whose other kernels keep them in float32 (outputs 1e-5 to 4e-4 from 32-bit sums rounded once, 1.8e-3 to 2.6e-3 in one
+// part; 8 single tokens behind 4,096, heads of 64, 13.7 us, 13.3 in one part; 64 behind 8,192, heads of 128, 41.6, 36.3). Warps whose rows
+// are all past the tile's end pass the barriers and compute nothing. Waits are bounded (2 s), after which the kernel raises *err, lets its
+// copies land, frees its tensor memory and returns.
 //
 // Bound by the chain of a page where tiles are full (1.05 us for 256 rows x 64 keys at heads of 128: 1.2 PFLOP/s while it runs, the
 // tensor pipe half busy, the exponentials 46% of their unit), by an item's start and end (5 us) and the thin tiles' chains (3 us a page and

@@ -86,7 +86,8 @@ def generate(model_dir, prompt_ids, max_tokens: int = 100, strategy: str = "gree
     `n` > 1: that many continuations of every prompt, each with a sampling stream of its own (seed + n * prompt + continuation);
     every prompt's list of ids becomes a list of `n` such lists, and its entries of `stats` lists of `n`. The prompt goes through the
     model once and its pages are held and read once. `share_prefix`: the same for whatever the prompts of a batch begin with in
-    common (a system prompt, a document). Both leave the numbers as they are but for rounding.
+    common (a system prompt, a document). Both leave the numbers as they are but for rounding: a step that reads shared pages once
+    adds its sums in another order, and in bfloat16 rounds the rotated queries of decode steps as prompt steps do.
     """
     single = len(prompt_ids) > 0 and not isinstance(prompt_ids[0], (list, tuple))
     prompts = [list(prompt_ids)] if single else [list(p) for p in prompt_ids]
