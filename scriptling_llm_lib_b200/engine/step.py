@@ -485,6 +485,8 @@ class Engine:
 
     def _portion_fits(self, takes) -> bool:
         """Whether the partial results of a prompt step of these (sequence, tokens) fit, where reading shared pages once is worth it."""
+        if any(s.closed or s.engine is not self for s, _ in takes):          # (the step refuses them)
+            return True
         gains = self._gains([s.slot for s, _ in takes], [s.length for s, _ in takes], [n for _, n in takes])
         return all(scratch <= SharedAttention.SCRATCH_BYTES for _, scratch in gains)
 

@@ -157,3 +157,16 @@ def test_a_plan_that_is_not_queued_is_there_for_any_stream():
         got = c.run(plan)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_prompts_of_closed_or_foreign_sequences_are_refused_beside_shared_ones(tmp_path):
+    from scriptling_llm_lib_b200.engine.step import StepError
+    eng, other = engine(tmp_path, LLAMA, "bfloat16", max_seqs=6), engine(tmp_path, LLAMA, "bfloat16", max_seqs=6)
+    root = eng.open()
+    eng.step([StepEntry(root, random_ids(300, LLAMA["vocab_size"], 1))])
+    seqs = [root] + root.fork(3)
+    seqs[2].close()
+    for wrong in (seqs[2], other.open()):
+        for budget in (None, 3):
+            with pytest.raises(StepError, match="closed or belongs to another engine"):
+                eng.prompt_step([StepEntry(seqs[0], [1, 2]), StepEntry(wrong, [3, 4])], budget)

@@ -134,7 +134,7 @@ def prompts(n, new, prefix, part, kv, layers):
     t = np.asarray(table(n, prefix // 64, 2), dtype=np.int32)
     eng.cache.share_tree = lambda g, slots: share_tree(t[list(slots)], np.full(len(slots), held[0] // 64))
     assert full.pool.n_shared
-    return eng, [SimpleNamespace(sequence=SimpleNamespace(slot=i, length=held[0]), tokens=list(range(new))) for i in range(n)], held
+    return eng, [SimpleNamespace(sequence=SimpleNamespace(slot=i, length=held[0], closed=False, engine=eng), tokens=list(range(new))) for i in range(n)], held
 
 
 @pytest.mark.parametrize("n, new, prefix", [(200, 32, 4096), (250, 32, 16384), (256, 40, 16384), (400, 40, 16384)])
