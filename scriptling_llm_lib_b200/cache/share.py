@@ -157,6 +157,7 @@ class SharePlan:
         if not self.fits(cap):
             raise ValueError(f"a plan of {self.n_items} items, {self.n_list} list entries and {self.part_rows} rows of scratch; there is "
                              f"room for {cap.items}, {cap.entries} and {cap.rows}")
+        self.dev, self.address = None, 0              # (a plan that is to take another's place, or to be looked at, is on the host alone)
         if device is not None:
             host = torch.from_numpy(self.host())
             self.dev = host.pin_memory().to(device, non_blocking=True) if queued else host.to(device)

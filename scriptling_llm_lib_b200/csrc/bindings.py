@@ -1783,6 +1783,8 @@ class SharedAttention:
         if not 0.0 < scale < math.inf or not 0.0 <= (softcap or 0.0) < math.inf:
             # (the tensor-core form takes a row's maximum before the scale, and caps by quotients of the two)
             raise KernelError(f"shared attention: a scale above 0 and a cap above 0 (or none), both finite, not {scale} and {softcap}")
+        if not plan.address:
+            raise KernelError("shared attention: the plan is on the host alone")
         H, G, T = plan.n_heads, plan.n_kv, plan.n_rows
         ks, vs, qs = kpages.shape, vpages.shape, q.shape
         if len(ks) != 4 or len(vs) != 4 or ks[:3] != vs[:3] or ks[1] != G or ks[2] != PAGE:

@@ -196,3 +196,12 @@ def test_only_requests_that_share_pages_keep_room_for_their_partial_results(monk
     for how in (dict(), dict(n=2), dict(share_prefix=True)):
         llm._fit_cache(eng, [[1] * 4000] * 1000, 50, None, **how)
     assert sizes[0] > sizes[1] == sizes[2]
+
+
+def test_a_plan_on_the_host_alone_is_refused():
+    import numpy as np
+    from scriptling_llm_lib_b200.cache import SharePlan, TileShape
+    plan = SharePlan.build(np.zeros((2, 3), dtype=np.int32), [10, 20], [1, 1], 4, 2, TileShape(64, 10), None)
+    ops = SharedAttention.__new__(SharedAttention)
+    with pytest.raises(KernelError, match="host alone"):
+        ops.attn(None, None, None, None, None, None, plan, None, 0.125, None)
